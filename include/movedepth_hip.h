@@ -389,6 +389,52 @@ int md_bn_relu_bwd_dx(const float *dy, const float *x, const float *mean, const 
                       const float *beta, const float *sums, long long n_total, long long nvox, int C, float *dx,
                       md_stream_t stream);
 
+/* ---- token operators: layer norm, 8-bit activation checkpoints, attention between two frames' tokens ------------------
+ * (no counterpart in the reference.)  dtype: 0 float32, 1 bfloat16, 2 float16, as md_bn_*; statistics, parameters, parameter
+ * gradients and every sum are float32.
+ *
+ * md_layer_norm_fwd: rows of C elements, row i at x + i * ldx; y [rows][C] = (x - mean) * rstd * w + b (w, b [C] or NULL);
+ *   stat [rows][2] = mean, rstd (or NULL).  codes / scales (both or neither): x in 8 bits for the backward pass, codes [rows][C],
+ *   scales [rows][ceil(C / 32)] (md_act8_pack's format, groups of 32 along a row).
+ * md_layer_norm_bwd: g [rows] at stride ldg; x at stride ldx, or its 8-bit codes / scales; dx [rows][C], dw, db [C], each or NULL.
+ *   ws: md_layer_norm_bwd_ws_bytes(rows, C) when dw or db is asked for.  Sums have a fixed order: the same inputs give the same bits. */
+int md_layer_norm_fwd(const void *x, int dtype, long long rows, int C, long long ldx, const float *w, const float *b, float eps,
+                      void *y, float *stat, void *codes, void *scales, md_stream_t stream);
+size_t md_layer_norm_bwd_ws_bytes(long long rows, int C);
+int md_layer_norm_bwd(const void *g, long long ldg, const void *x, long long ldx, const void *codes, const void *scales, int dtype,
+                      const float *stat, const float *w, long long rows, int C, void *dx, float *dw, float *db, void *ws,
+                      size_t ws_bytes, md_stream_t stream);
+
+/* 8-bit activations: every 32 neighbours share a scale 2^e, e the least exponent for which the largest of them rounds to 127 or
+ * less; value = n * 2^e, n in [-127, 127].  n is x * 2^-e correctly rounded (ties to even) and n * 2^e is exact in x's type, so
+ * packing what came back gives the same codes.  e stays in [-126, 121] (float16: [-24, 9]; n is cut off at 127 at the upper end).
+ * A group that holds a NaN or an infinity comes back as NaN.  codes [n] int8, scales [ceil(n / 32)] int8 (e; -128 = NaN). */
+int md_act8_pack(const void *x, int dtype, long long n, void *codes, void *scales, md_stream_t stream);
+int md_act8_unpack(const void *codes, const void *scales, int dtype, long long n, void *x, md_stream_t stream);
+
+/* Attention of queries [B][Nq][Hq][d] to keys / values [B][Nk][Hk][d] of another sequence; query head i reads key head
+ * i / (Hq / Hk).  key_mask [B][Nk] bytes (NULL: every key is valid): a key whose byte is 0 takes no part, whatever stands in its
+ * row; a query left without a key gets o = 0 and gives no gradients; dk, dv of masked keys are 0.
+ * The last axis of q, k, v, g is contiguous, *_sb / *_sn / *_sh are the strides of sequence, token and head in elements (0 allowed);
+ * o, dq [B][Nq][Hq][d] and dk, dv [B][Nk][Hk][d] are contiguous.  lse [B][Hq][Nq]: log2 of the softmax denominator including its
+ * maximum, +inf without a key; written by the forward pass (or NULL there), read by the backward pass.  dq may be NULL, dk and dv both may.
+ * ws: md_cross_attn_ws_bytes(desc, backward) bytes, 256-byte aligned. */
+#define MD_ATTN_MAX_D 128
+typedef struct {
+    int dtype, B, Nq, Nk, Hq, Hk, d;
+    float scale;
+    const void *q, *k, *v, *key_mask;
+    void *o;
+    float *lse;
+    const void *g;
+    void *dq, *dk, *dv;
+    long long q_sb, q_sn, q_sh, k_sb, k_sn, k_sh, v_sb, v_sn, v_sh, g_sb, g_sn, g_sh, mask_sb;
+} md_attn_desc;
+size_t md_attn_desc_bytes(void);
+size_t md_cross_attn_ws_bytes(const md_attn_desc *desc, int backward);
+int md_cross_attn_fwd(const md_attn_desc *desc, void *ws, size_t ws_bytes, md_stream_t stream);
+int md_cross_attn_bwd(const md_attn_desc *desc, void *ws, size_t ws_bytes, md_stream_t stream);
+
 /* ---- pose parameters -> 4x4 -------------------------------------------------------------------
  * transformation_from_parameters (layers.py:412-429; rot_from_axisangle :479-518, get_translation_matrix :464-477):
  * axisangle, translation [B,3] -> T [B,4,4]; invert != 0: R^T . T(-t), else T(t) . R.  The reference's

@@ -93,6 +93,15 @@ SIGNATURES = {
     "md_pose_matrix_bwd": (_i, [_vp, _vp, _vp, _i, _i, _vp, _vp, _vp]),
     "md_backproject": (_i, [_vp, _vp, _i, _i, _i, _i, _vp, _vp]),
     "md_project3d": (_i, [_vp, _vp, _vp, _i, _i, _i, _i, _f, _vp, _vp]),
+    "md_layer_norm_fwd": (_i, [_vp, _i, _ll, _i, _ll, _vp, _vp, _f, _vp, _vp, _vp, _vp, _vp]),
+    "md_layer_norm_bwd_ws_bytes": (_sz, [_ll, _i]),
+    "md_layer_norm_bwd": (_i, [_vp, _ll, _vp, _ll, _vp, _vp, _i, _vp, _vp, _ll, _i, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "md_act8_pack": (_i, [_vp, _i, _ll, _vp, _vp, _vp]),
+    "md_act8_unpack": (_i, [_vp, _vp, _i, _ll, _vp, _vp]),
+    "md_attn_desc_bytes": (_sz, []),
+    "md_cross_attn_ws_bytes": (_sz, [_vp, _i]),
+    "md_cross_attn_fwd": (_i, [_vp, _vp, _sz, _vp]),
+    "md_cross_attn_bwd": (_i, [_vp, _vp, _sz, _vp]),
     "md_kernel_timing_enable": (_i, [_i]),
     "md_costvol_stats": (_i, [_i, ctypes.POINTER(ctypes.c_ulonglong)]),
     "md_costvol_stats_wg": (_i, [ctypes.POINTER(ctypes.c_ulonglong), _i]),
@@ -119,6 +128,16 @@ class PhotoDesc(ctypes.Structure):
         ("mask", _vp * PHOTO_MAX_SCALES), ("sel", _vp * PHOTO_MAX_SCALES), ("loss", _vp),
         ("gloss", _vp * PHOTO_MAX_SCALES), ("d_dz", _vp * PHOTO_MAX_SCALES), ("d_T", _vp * PHOTO_MAX_FRAMES),
     ]
+
+
+ATTN_MAX_D = 128   # MD_ATTN_MAX_D
+
+
+class AttnDesc(ctypes.Structure):
+    """md_attn_desc of include/movedepth_hip.h (field for field)."""
+    _fields_ = [(n, _i) for n in ("dtype", "B", "Nq", "Nk", "Hq", "Hk", "d")] + [("scale", _f)] + \
+        [(n, _vp) for n in ("q", "k", "v", "key_mask", "o", "lse", "g", "dq", "dk", "dv")] + \
+        [(n, _ll) for n in ("q_sb", "q_sn", "q_sh", "k_sb", "k_sn", "k_sh", "v_sb", "v_sn", "v_sh", "g_sb", "g_sn", "g_sh", "mask_sb")]
 
 
 _lib = None
@@ -150,6 +169,9 @@ def load():
     if lib.md_photo_desc_bytes() != ctypes.sizeof(PhotoDesc):
         raise MovedepthHipError("md_photo_desc is %d bytes in the library, %d in the binding: stale build?"
                                 % (lib.md_photo_desc_bytes(), ctypes.sizeof(PhotoDesc)))
+    if lib.md_attn_desc_bytes() != ctypes.sizeof(AttnDesc):
+        raise MovedepthHipError("md_attn_desc is %d bytes in the library, %d in the binding: stale build?"
+                                % (lib.md_attn_desc_bytes(), ctypes.sizeof(AttnDesc)))
     _lib = lib
     return lib
 

@@ -42,6 +42,9 @@ def predict_depth(models, data, opt, vol_layout="ndhwc", details=False):
     relative_poses = torch.stack([data[("relative_pose", idx)] for idx in opt.matching_ids[1:]], 1)
     ref_feat, ref_context = models["mvs_encoder"](color)
     src_feats = [models["mvs_encoder"](data["color_aug", f_i, 0])[0] for f_i in opt.matching_ids[1:]]
+    if "match_attn" in models:
+        attn = models["match_attn"]
+        ref_feat, src_feats = attn(ref_feat, src_feats), [attn(f, [ref_feat]) for f in src_feats]
 
     disp_prior = output[("disp", opt.prior_scale)]
     depth_prior = 1 / (1 / opt.max_depth + disp_prior * (1 / opt.min_depth - 1 / opt.max_depth))

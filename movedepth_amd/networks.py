@@ -637,3 +637,51 @@ class convex_upsample_layer(nn.Module):
         from .layers import convex_upsample
 
         return convex_upsample(depth, self.upsample_mask(feat), self.scale)
+
+
+# --------------------------------------------------------------------------- attention between the frames' matching features
+class LayerNorm(nn.Module):
+    """nn.LayerNorm over the last axis with its parameter names, on ops.layer_norm.  act_bits = 8: the input is kept for the backward pass in
+    8 bits.  On the CPU it is the torch op."""
+
+    def __init__(self, num_features, eps=1e-5, act_bits=0):
+        super().__init__()
+        self.num_features, self.eps, self.act_bits = num_features, eps, act_bits
+        self.weight = nn.Parameter(torch.ones(num_features))
+        self.bias = nn.Parameter(torch.zeros(num_features))
+
+    def forward(self, x):
+        if x.is_cuda:
+            return ops.layer_norm(x, self.weight, self.bias, self.eps, self.act_bits)
+        return F.layer_norm(x, (self.num_features,), self.weight, self.bias, self.eps)
+
+
+class MatchAttention(nn.Module):
+    """x + out(attention of norm(x)'s tokens to norm(others)'s tokens): one frame's matching features (B,C,h,w), a token per pixel, look
+    up the other frames' before the plane sweep compares them.  `others`: a list of (B,C,h,w), their tokens one behind the other.  `out`
+    starts at zero, so an untrained module hands its input through."""
+
+    def __init__(self, channels, heads=2, act_bits=0):
+        super().__init__()
+        if channels % heads:
+            raise ValueError("MatchAttention: %d channels on %d heads" % (channels, heads))
+        self.heads = heads
+        self.norm = LayerNorm(channels, act_bits=act_bits)
+        self.q = nn.Linear(channels, channels, bias=False)
+        self.kv = nn.Linear(channels, 2 * channels, bias=False)
+        self.out = nn.Linear(channels, channels, bias=False)
+        nn.init.zeros_(self.out.weight)
+
+    @staticmethod
+    def _tokens(x):
+        return x.permute(0, 2, 3, 1).flatten(1, 2)      # (B, h*w, C): a view of channels-last features
+
+    def forward(self, x, others, key_mask=None):
+        B, C, h, w = x.shape
+        t = self._tokens(x)
+        q = self.q(self.norm(t)).view(B, h * w, self.heads, C // self.heads)
+        o = others[0] if len(others) == 1 else None
+        kv = self.kv(self.norm(self._tokens(o) if o is not None else torch.cat([self._tokens(f) for f in others], 1)))
+        k, v = kv.view(B, -1, 2, self.heads, C // self.heads).unbind(2)
+        a = ops.cross_attention(q, k, v, key_mask).reshape(B, h * w, C)
+        return x + self.out(a).view(B, h, w, C).permute(0, 3, 1, 2)

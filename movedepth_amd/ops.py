@@ -1460,3 +1460,245 @@ def project3d(points, K, T, batch_size, height, width, eps=1e-7):
         out = torch.empty(batch_size, height, width, 2, device=points.device, dtype=torch.float32)
         _lib.call("md_project3d", _p(points), _p(K), _p(T), batch_size, nk, height, width, float(eps), _p(out), _stream())
     return out
+
+
+# --------------------------------------------------------------------------- token operators: shared checks
+_TOKEN_DTYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}   # `dtype` of md_layer_norm_*, md_act8_*, md_cross_attn_*
+
+
+def _token_check(t, name, what):
+    if not t.is_cuda:
+        raise _lib.MovedepthHipError("%s: %s must be a GPU tensor (got %s): the HIP path has no CPU fallback" % (what, name, t.device))
+    if t.dtype not in _TOKEN_DTYPE:
+        raise _lib.MovedepthHipError("%s: %s is %s (float32, bfloat16 or float16)" % (what, name, t.dtype))
+
+
+def _wants_grad(*tensors):
+    """a backward pass may follow: keep what it reads"""
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def _stream_of(device):
+    """raw current stream of the tensors' own device (which need not be the current device: callers hold torch.cuda.device(device))"""
+    return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+# --------------------------------------------------------------------------- 8-bit activation checkpoints
+class Act8:
+    """A tensor in 8 bits (act8_pack): `codes` int8 per element in storage order, `scales` int8 per 32 of them (the exponent of
+    their shared power of two), and what is needed to restore shape, strides and type."""
+
+    __slots__ = ("codes", "scales", "shape", "stride", "dtype")
+
+    def __init__(self, codes, scales, shape, stride, dtype):
+        self.codes, self.scales, self.shape, self.stride, self.dtype = codes, scales, shape, stride, dtype
+
+    def nbytes(self):
+        return self.codes.numel() + self.scales.numel()
+
+
+def _is_dense(t):
+    """the elements fill one block of memory without gaps or overlap, in whatever order"""
+    expect = 1
+    for st, n in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n != 1):
+        if st != expect:
+            return False
+        expect *= n
+    return True
+
+
+def act8_pack(x):
+    """x (any shape; float32, bfloat16 or float16) -> Act8, 1 + 1/32 bytes per element: whole numbers of [-127, 127] times a power of two
+    that 32 neighbours in memory share -- the least one that keeps the largest of them at 127 or below, so the error is at most half a
+    step: 2^-7 of the group's largest magnitude (at the far end of the type's range, where that power would overflow, up to one part in
+    128 of the value).  32 neighbours that hold an infinity or a NaN come back as NaN.  No gradient."""
+    _token_check(x, "x", "act8_pack")
+    with torch.no_grad(), torch.cuda.device(x.device):
+        x = x.detach()
+        if not _is_dense(x):
+            x = x.contiguous()
+        n = x.numel()
+        codes = torch.empty(n, device=x.device, dtype=torch.int8)
+        scales = torch.empty((n + 31) // 32, device=x.device, dtype=torch.int8)
+        _timed_call("md_act8_pack", _p(x), _TOKEN_DTYPE[x.dtype], n, _p(codes), _p(scales), _stream_of(x.device))
+    return Act8(codes, scales, x.shape, x.stride(), x.dtype)
+
+
+def act8_unpack(packed):
+    """Act8 -> tensor of the packed one's shape, strides and type (exact: the stored values are representable in it)."""
+    dev = packed.codes.device
+    with torch.cuda.device(dev):
+        x = torch.empty_strided(packed.shape, packed.stride, device=dev, dtype=packed.dtype)
+        _timed_call("md_act8_unpack", _p(packed.codes), _p(packed.scales), _TOKEN_DTYPE[packed.dtype], x.numel(), _p(x), _stream_of(dev))
+    return x
+
+
+def saved_act8(min_numel=1 << 20):
+    """Context manager: activations that autograd keeps for the backward pass inside it are kept in 8 bits (act8_pack) and restored when the
+    backward pass reads them.  Left as they are: parameters and other leaves, tensors below `min_numel` elements (statistics, weights cast
+    by autocast), other types, CPU tensors, and tensors that do not fill their memory (expanded or cut-out views).  Gradients then
+    carry the rounding of the kept activations; the forward pass does not change."""
+
+    def pack(t):
+        if t.is_cuda and t.dtype in _TOKEN_DTYPE and t.numel() >= min_numel and not (t.is_leaf and t.requires_grad) and _is_dense(t):
+            return act8_pack(t)
+        return t
+
+    def unpack(p):
+        return act8_unpack(p) if isinstance(p, Act8) else p
+
+    return torch.autograd.graph.saved_tensors_hooks(pack, unpack)
+
+
+# --------------------------------------------------------------------------- layer norm
+def _rows(t, C):
+    """(..., C) -> ((rows, C) tensor with contiguous columns, row stride); a copy only if the rows are not evenly spaced already"""
+    t = t.reshape(-1, C)
+    if (C > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < C):
+        t = t.contiguous()
+    return t, (t.stride(0) if t.shape[0] > 1 else C)
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps, act_bits, keep):
+        C = x.shape[-1]
+        w = None if weight is None else _f32c(weight)
+        b = None if bias is None else _f32c(bias)
+        with torch.cuda.device(x.device):
+            x2, ldx = _rows(x, C)
+            rows = x2.shape[0]
+            y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+            stat = torch.empty(rows, 2, device=x.device, dtype=torch.float32) if keep else None
+            codes = scales = None
+            if keep and act_bits:
+                codes = torch.empty(rows, C, device=x.device, dtype=torch.int8)
+                scales = torch.empty(rows, (C + 31) // 32, device=x.device, dtype=torch.int8)
+            _timed_call("md_layer_norm_fwd", _p(x2), _TOKEN_DTYPE[x.dtype], rows, C, ldx, _p(w), _p(b), eps, _p(y), _p(stat), _p(codes),
+                        _p(scales), _stream_of(x.device))
+        if keep:
+            ctx.save_for_backward(None if codes is not None else x2, codes, scales, stat, w)
+            ctx.dtype, ctx.wdtype, ctx.bdtype = x.dtype, None if weight is None else weight.dtype, None if bias is None else bias.dtype
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gy):
+        x2, codes, scales, stat, w = ctx.saved_tensors
+        C, dev = gy.shape[-1], gy.device
+        with torch.cuda.device(dev):
+            g, ldg = _rows(gy.to(ctx.dtype), C)
+            rows = g.shape[0]
+            ldx = C if x2 is None or rows <= 1 else x2.stride(0)
+            need_x, need_w, need_b = ctx.needs_input_grad[:3]
+            dx = torch.empty(gy.shape, device=dev, dtype=ctx.dtype) if need_x else None
+            dwb = torch.empty(2, C, device=dev, dtype=torch.float32) if need_w or need_b else None
+            nbytes = 0 if dwb is None else _lib.load().md_layer_norm_bwd_ws_bytes(rows, C)
+            ws = _ws(nbytes, dev) if nbytes else None
+            _timed_call("md_layer_norm_bwd", _p(g), ldg, _p(x2), ldx, _p(codes), _p(scales), _TOKEN_DTYPE[ctx.dtype], _p(stat), _p(w), rows, C,
+                        _p(dx), _p(dwb[0]) if need_w else None, _p(dwb[1]) if need_b else None, _p(ws), nbytes, _stream_of(dev))
+        return dx, dwb[0].to(ctx.wdtype) if need_w else None, dwb[1].to(ctx.bdtype) if need_b else None, None, None, None
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5, act_bits=0):
+    """(x - mean) / sqrt(var + eps) * weight + bias over the last axis (biased variance, as torch's layer_norm).  x (..., C) float32, bfloat16 or
+    float16, read in place where its rows are evenly spaced; statistics, sums and parameter gradients in float32; weight and bias (C,) or None.
+    act_bits=8: the backward pass reads x from 8 bits (act8_pack's format, groups of 32 along the last axis) written by the forward
+    kernel instead of keeping x; the result does not change."""
+    _token_check(x, "x", "layer_norm")
+    if x.dim() < 1 or not 1 <= x.shape[-1] <= 1 << 20:
+        raise _lib.MovedepthHipError("layer_norm: x %s (at least one axis, 1 .. 2^20 elements in the last)" % (tuple(x.shape),))
+    for t, nm in ((weight, "weight"), (bias, "bias")):
+        if t is not None and (t.device != x.device or tuple(t.shape) != (x.shape[-1],)):
+            raise _lib.MovedepthHipError("layer_norm: %s %s on %s does not match x %s on %s" % (nm, tuple(t.shape), t.device, tuple(x.shape), x.device))
+    if act_bits not in (0, 8):
+        raise _lib.MovedepthHipError("layer_norm: act_bits = %r (0 or 8)" % (act_bits,))
+    if not eps >= 0:
+        raise _lib.MovedepthHipError("layer_norm: eps = %r" % (eps,))
+    return _LayerNorm.apply(x, weight, bias, float(eps), int(act_bits), _wants_grad(x, weight, bias))
+
+
+# --------------------------------------------------------------------------- attention to another sequence's tokens
+def _attn_strides(t):
+    """t (B, N, H, d) with a contiguous last axis, read in place (any strides of the other three, 0 among them)"""
+    if t.shape[3] > 1 and t.stride(3) != 1:
+        t = t.contiguous()
+    return t, t.stride()[:3]
+
+
+def _attn_desc(q, k, v, key_mask, scale):
+    a = _lib.AttnDesc()
+    a.dtype, a.scale = _TOKEN_DTYPE[q.dtype], scale
+    a.B, a.Nq, a.Hq, a.d = q.shape
+    a.Nk, a.Hk = k.shape[1], k.shape[2]
+    a.q, a.k, a.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
+    (a.q_sb, a.q_sn, a.q_sh), (a.k_sb, a.k_sn, a.k_sh), (a.v_sb, a.v_sn, a.v_sh) = q.stride()[:3], k.stride()[:3], v.stride()[:3]
+    if key_mask is not None:
+        a.key_mask, a.mask_sb = key_mask.data_ptr(), key_mask.stride(0)
+    return a
+
+
+class _CrossAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, key_mask, scale, keep):
+        dev = q.device
+        with torch.cuda.device(dev):
+            (q, _), (k, _), (v, _) = _attn_strides(q), _attn_strides(k), _attn_strides(v)
+            if key_mask is not None and key_mask.shape[1] > 1 and key_mask.stride(1) != 1:
+                key_mask = key_mask.contiguous()
+            a = _attn_desc(q, k, v, key_mask, scale)
+            o = torch.empty(q.shape, device=dev, dtype=q.dtype)
+            lse = torch.empty(a.B, a.Hq, a.Nq, device=dev, dtype=torch.float32) if keep else None
+            a.o, a.lse = o.data_ptr(), None if lse is None else lse.data_ptr()
+            nbytes = _lib.load().md_cross_attn_ws_bytes(ctypes.byref(a), 0)
+            ws = _ws(nbytes, dev) if nbytes else None
+            _timed_call("md_cross_attn_fwd", ctypes.byref(a), _p(ws), nbytes, _stream_of(dev))
+        if keep:
+            ctx.save_for_backward(q, k, v, key_mask, o, lse)
+            ctx.scale = scale
+        return o
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        q, k, v, key_mask, o, lse = ctx.saved_tensors
+        dev = q.device
+        with torch.cuda.device(dev):
+            g, gs = _attn_strides(g.to(q.dtype))
+            o = o.contiguous()
+            a = _attn_desc(q, k, v, key_mask, ctx.scale)
+            a.o, a.lse, a.g = o.data_ptr(), lse.data_ptr(), g.data_ptr()
+            a.g_sb, a.g_sn, a.g_sh = gs
+            dq = torch.empty(q.shape, device=dev, dtype=q.dtype) if ctx.needs_input_grad[0] else None
+            both = ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
+            dk = torch.empty(k.shape, device=dev, dtype=k.dtype) if both else None
+            dv = torch.empty(v.shape, device=dev, dtype=v.dtype) if both else None
+            a.dq, a.dk, a.dv = (None if t is None else t.data_ptr() for t in (dq, dk, dv))
+            nbytes = _lib.load().md_cross_attn_ws_bytes(ctypes.byref(a), 1)
+            ws = _ws(nbytes, dev) if nbytes else None
+            _timed_call("md_cross_attn_bwd", ctypes.byref(a), _p(ws), nbytes, _stream_of(dev))
+        return dq, dk if ctx.needs_input_grad[1] else None, dv if ctx.needs_input_grad[2] else None, None, None, None
+
+
+def cross_attention(q, k, v, key_mask=None, scale=None):
+    """softmax(scale q k^T) v per head: q (B, Nq, Hq, d) attends to another sequence's k, v (B, Nk, Hk, d) -> (B, Nq, Hq, d).  Hq is a multiple of
+    Hk (query head i reads key head i // (Hq // Hk)), d <= 128, scale defaults to d ** -0.5; float32, bfloat16 or float16, all alike; any
+    strides (the last axis is copied if it is not contiguous).  key_mask (B, Nk) bool, True where a key takes part: what stands in the
+    other rows of k and v is not used, whatever it is, and their gradients are 0; a query without any key gets zeros and gives no gradients.
+    Softmax statistics and sums are float32; with 2-byte types the softmax weights are rounded to that type before the product with v."""
+    for t, nm in ((q, "q"), (k, "k"), (v, "v")):
+        _token_check(t, nm, "cross_attention")
+        if t.dim() != 4:
+            raise _lib.MovedepthHipError("cross_attention: %s %s is not (batch, tokens, heads, head size)" % (nm, tuple(t.shape)))
+        if t.device != q.device or t.dtype != q.dtype:
+            raise _lib.MovedepthHipError("cross_attention: %s is %s on %s, q is %s on %s" % (nm, t.dtype, t.device, q.dtype, q.device))
+    B, Nq, Hq, d = q.shape
+    if k.shape != v.shape or k.shape[0] != B or k.shape[3] != d:
+        raise _lib.MovedepthHipError("cross_attention: q %s, k %s, v %s do not match" % (tuple(q.shape), tuple(k.shape), tuple(v.shape)))
+    if not 1 <= d <= _lib.ATTN_MAX_D or k.shape[2] < 1 or Hq < 1 or Hq % k.shape[2]:
+        raise _lib.MovedepthHipError("cross_attention: head size %d (1 .. %d), %d query heads on %d key heads (a multiple)"
+                                     % (d, _lib.ATTN_MAX_D, Hq, k.shape[2]))
+    if key_mask is not None and (key_mask.dtype != torch.bool or key_mask.device != q.device or tuple(key_mask.shape) != (B, k.shape[1])):
+        raise _lib.MovedepthHipError("cross_attention: key_mask %s %s on %s (bool (%d, %d) on %s: True where a key takes part)"
+                                     % (key_mask.dtype, tuple(key_mask.shape), key_mask.device, B, k.shape[1], q.device))
+    return _CrossAttention.apply(q, k, v, key_mask, float(d ** -0.5 if scale is None else scale), _wants_grad(q, k, v))

@@ -114,6 +114,12 @@ class MonodepthOptions:
                        help="with --fused_photometric: outputs[(\"sample\", f, s)] -- which nothing on the training path reads "
                             "(reference trainer.py:524-529 only hands it to grid_sample) -- is computed when first accessed "
                             "instead of being stored by every step (8 maps, 47 MB per step at config 2); the same bits either way")
+        p.add_argument("--match_attention", type=int, default=0,
+                       help="heads of the attention between the frames' matching features ahead of the plane sweep "
+                            "(networks.MatchAttention, sub-model 'match_attn'); 0: none, as the reference")
+        p.add_argument("--act_bits", type=int, default=0, choices=[0, 8],
+                       help="8: the 3-D regulariser's activations of a million elements and more, and the matching attention's "
+                            "inputs, are kept for the backward pass in 8 bits (ops.saved_act8); 0: as they are")
         p.add_argument("--amp", default="none", choices=["none", "bf16", "fp16"],
                        help="mixed precision (BASELINE configs 4 / 5): networks under autocast, 2-byte cost volume; the "
                             "headline bench is fp32")

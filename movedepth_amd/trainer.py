@@ -10,6 +10,7 @@ Deliberate differences from the reference's host code (values unchanged):
   * the masked-consistency loss is a masked mean instead of boolean indexing: no device->host sync in the step;
   * one gradient reducer over all parameters instead of 8 DDP wrappers (movedepth_amd/dp.py).
 """
+import contextlib
 import json
 import os
 import time
@@ -47,6 +48,9 @@ def build_models(opt, num_pose_frames=2):
     else:
         models["reg3d"] = networks.reg2d(opt.reg3d_c, opt.reg3d_c)
     mvs = ["mask_cnn", "mvs_encoder", "reg3d"]
+    if getattr(opt, "match_attention", 0):
+        models["match_attn"] = networks.MatchAttention(8 * 2 ** opt.prior_scale, opt.match_attention, getattr(opt, "act_bits", 0))
+        mvs.append("match_attn")
     if opt.convex_up:
         models["up"] = networks.convex_upsample_layer(feature_dim=8 * 2 ** opt.prior_scale, scale=opt.prior_scale)
         main.append("up")
@@ -318,6 +322,10 @@ class Trainer:
         # mvs feature extraction
         ref_match_feat, ref_context_feat = self.models["mvs_encoder"](inputs["color_aug", 0, 0])
         src_match_feats = [self.models["mvs_encoder"](inputs["color_aug", f_i, 0])[0] for f_i in self.matching_ids[1:]]
+        match_attn = self.models.get("match_attn")
+        frame_feats = src_match_feats                # as they come from the encoder: what the reference features attend to
+        if match_attn is not None:
+            src_match_feats = [match_attn(f, [ref_match_feat]) for f in frame_feats]
 
         # single frame path + mono reprojection loss
         feats = self.models["mono_encoder"](inputs["color_aug", 0, 0])
@@ -350,11 +358,14 @@ class Trainer:
         min_inv, max_inv = 1 / end_planes[:, 1], 1 / end_planes[:, 0]  # swapped on purpose (App. B-6)
 
         def mvs_branch(ref_feat, want_prob=False):
+            if match_attn is not None:
+                ref_feat = match_attn(ref_feat, frame_feats)
             vols = [ops.costvol_grouped(ref_feat, src_match_feats[f_idx], inputs[("K", 2)], inputs[("inv_K", 2)],
                                         relative_poses[:, f_idx], opt.reg3d_c, layout=self.vol_layout, **sched)
                     for f_idx in range(len(self.matching_ids) - 1)]
             cor_feats, _ = ops.fuse_volumes(vols, layout=self.vol_layout)
-            logits = self.models["reg3d"](cor_feats)  # B D h w
+            with ops.saved_act8() if getattr(opt, "act_bits", 0) else contextlib.nullcontext():
+                logits = self.models["reg3d"](cor_feats)  # B D h w
             return ops.softmax_entropy_localmax(logits, min_inv, max_inv, opt.norm_radius, want_prob=want_prob)
 
         depth_mvs, cost_prob_entropy, _ = mvs_branch(ref_match_feat)
@@ -673,6 +684,12 @@ class Trainer:
         assert os.path.isdir(folder), "Cannot find folder {}".format(folder)
         for n in self.opt.models_to_load:
             self._load_one(folder, n)
+        if "match_attn" in self.models and "match_attn" not in self.opt.models_to_load:
+            # not one of the reference's sub-models, so not in the default list: taken where the folder has it
+            if os.path.isfile(os.path.join(folder, "match_attn.pth")):
+                self._load_one(folder, "match_attn")
+            else:
+                print("load_model: no match_attn.pth in %s, 'match_attn' keeps its initial weights" % folder)
         adam = os.path.join(folder, "adam.pth")
         if os.path.isfile(adam):
             try:
