@@ -1,101 +1,872 @@
 // Attention from queries (B, Nq, Hq, d) to another sequence's keys and values (B, Nk, Hk, d), Hq a multiple of Hk (query head i reads key head
 // i / (Hq / Hk)), with an optional mask of valid keys (B, Nk):
 //   S = scale q k^T over the valid keys, P = softmax S, O = P V;   D = sum g O, dV = P^T g, dS = P (g V^T - D), dQ = scale dS K, dK = scale dS^T Q.
-// One pass over the keys: running maximum m and sum l per query, O rescaled when m grows.  A masked key is not read into any product (what stands
-// there may be NaN); a query without a valid key gets zeros and gives zero gradients.  `lse` = m + log l per query, in units of log 2; +inf without a key.
+//
+// The problem is taken as Z = B Hk independent ones of M = (Hq / Hk) Nq query rows (the heads that share a key head, one behind the other) and
+// N keys.  Nothing of size M x N is stored: a running maximum m and sum l per query row, O rescaled when m grows, and in the backward
+// pass P again from S and the row's log-sum `lse` = m + log2 l (all exponents are in units of log 2; +inf for a row without keys).
+//
+// Long problems run in three steps: xa_compact lists the valid keys (so a masked key costs nothing and what stands in its row, NaN
+// among it, is never touched), xa_pack writes every operand in the order in which the matrix instruction's lanes take it, and the tile kernels
+// copy such fragments to shared memory with 1 KB direct loads and read them back without bank conflicts.  A few query rows against long keys
+// (serving) are bound by reading K and V once and go to xa_few, which reads them in place.
+//
+// Fragments of v_mfma_f32_32x32x16 (A, B: lane l holds row / column l % 32 and 8 neighbours of the contraction axis; C: lane l holds column l % 32 and
+// rows 8 (r / 4) + 4 (l / 32) + r % 4, r = 0 .. 15):
+//   "R": 32 rows x 16 dims, lane l: row l % 32, dims 8 (l / 32) + 0 .. 7.  Both operands of S and g V^T.
+//   "T": 32 dims x 16 rows, lane l: dim l % 32, rows 8 (j / 4) + 4 (l / 32) + j % 4, j = 0 .. 7 -- the order in which C leaves its rows in
+//        a lane's registers, so P and dS go from the accumulators of one product into the operand of the next without crossing lanes.
+// Products run transposed (S^T = K Q^T, O^T = V^T P^T): a lane then owns one query, its softmax is in-lane but for one exchange of halves.
+//
+// float32 runs on the bf16 instructions too: every operand as the sum of three bf16 pieces (8 + 8 + 8 bits), six products of pieces whose
+// magnitudes matter to 2^-24, which is 6 / 16 of what the float32 matrix instruction costs.  2-byte types: P and dS are rounded to
+// the type before their products (half a step relative).  float16 holds P times 2^7 (forward) or 2^15 (backward) and dS times a power
+// of two from the largest |g| |v|, so that the small weights of long rows do not fall below its range.
 #include "md_types.hpp"
 
 namespace {
 
 constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LAZY = 8.f;     // m is raised only when a score passes it by more than 2^8: the sums stay exact, O is rarely rescaled
 
-// one wave per query row; a lane holds elements lane and lane + 64 of a row
-template <class T>
-__global__ __launch_bounds__(64) void xa_fwd_kernel(md_attn_desc a) {
-    const int t = threadIdx.x, qi = blockIdx.x, hq = blockIdx.y, b = blockIdx.z, hk = hq / (a.Hq / a.Hk);
-    const T *q = (const T *)a.q + b * a.q_sb + qi * a.q_sn + hq * a.q_sh;
-    const T *k = (const T *)a.k + b * a.k_sb + hk * a.k_sh, *v = (const T *)a.v + b * a.v_sb + hk * a.v_sh;
-    const unsigned char *mask = a.key_mask ? (const unsigned char *)a.key_mask + b * a.mask_sb : nullptr;
-    const bool in0 = t < a.d, in1 = t + 64 < a.d;
-    const float c = a.scale * LOG2E, q0 = in0 ? (float)q[t] : 0.f, q1 = in1 ? (float)q[t + 64] : 0.f;
-    float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
-    for (int i = 0; i < a.Nk; ++i) {
-        if (mask && !mask[i]) continue;
-        const T *kr = k + i * a.k_sn, *vr = v + i * a.v_sn;
-        const float s = md_wave_sum(q0 * (in0 ? (float)kr[t] : 0.f) + q1 * (in1 ? (float)kr[t + 64] : 0.f)) * c;
-        const float mn = fmaxf(m, s), r = exp2f(m - mn), p = exp2f(s - mn);
-        m = mn;
-        l = l * r + p;
-        o0 = o0 * r + p * (in0 ? (float)vr[t] : 0.f);
-        o1 = o1 * r + p * (in1 ? (float)vr[t + 64] : 0.f);
+using f32x16 = float __attribute__((ext_vector_type(16)));
+template <class E> struct Vec { using v8 = E __attribute__((ext_vector_type(8))); };
+template <class T> struct Frag { using E = T; static constexpr int NP = 1; };
+template <> struct Frag<float> { using E = bf16_t; static constexpr int NP = 3; };
+
+__device__ __forceinline__ f32x16 mfma(Vec<bf16_t>::v8 a, Vec<bf16_t>::v8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x16 mfma(Vec<f16_t>::v8 a, Vec<f16_t>::v8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+
+// c + a b for operands of NP pieces, the smallest products first
+template <class E, int NP>
+__device__ __forceinline__ f32x16 mfma_pieces(const typename Vec<E>::v8 (&a)[NP], const typename Vec<E>::v8 (&b)[NP], f32x16 c) {
+    if constexpr (NP == 3) {
+        c = mfma(a[2], b[0], c);
+        c = mfma(a[1], b[1], c);
+        c = mfma(a[0], b[2], c);
+        c = mfma(a[1], b[0], c);
+        c = mfma(a[0], b[1], c);
     }
-    const float inv = l > 0.f ? 1.f / l : 0.f;
-    T *o = (T *)a.o + (((long long)b * a.Nq + qi) * a.Hq + hq) * a.d;
-    if (in0) o[t] = (T)(o0 * inv);
-    if (in1) o[t + 64] = (T)(o1 * inv);
-    if (a.lse && t == 0) a.lse[((long long)b * a.Hq + hq) * a.Nq + qi] = l > 0.f ? m + log2f(l) : INFINITY;
+    return mfma(a[0], b[0], c);
 }
 
-template <class T>
-__global__ __launch_bounds__(64) void xa_dq_kernel(md_attn_desc a, float *__restrict__ delta) {
-    const int t = threadIdx.x, qi = blockIdx.x, hq = blockIdx.y, b = blockIdx.z, hk = hq / (a.Hq / a.Hk);
-    const T *q = (const T *)a.q + b * a.q_sb + qi * a.q_sn + hq * a.q_sh, *g = (const T *)a.g + b * a.g_sb + qi * a.g_sn + hq * a.g_sh;
-    const T *k = (const T *)a.k + b * a.k_sb + hk * a.k_sh, *v = (const T *)a.v + b * a.v_sb + hk * a.v_sh;
-    const long long at = (((long long)b * a.Nq + qi) * a.Hq + hq) * a.d;
-    const T *o = (const T *)a.o + at;
-    const unsigned char *mask = a.key_mask ? (const unsigned char *)a.key_mask + b * a.mask_sb : nullptr;
-    const bool in0 = t < a.d, in1 = t + 64 < a.d;
-    const float c = a.scale * LOG2E, q0 = in0 ? (float)q[t] : 0.f, q1 = in1 ? (float)q[t + 64] : 0.f;
-    const float g0 = in0 ? (float)g[t] : 0.f, g1 = in1 ? (float)g[t + 64] : 0.f;
-    const float D = md_wave_sum(g0 * (in0 ? (float)o[t] : 0.f) + g1 * (in1 ? (float)o[t + 64] : 0.f));
-    const float lse = a.lse[((long long)b * a.Hq + hq) * a.Nq + qi];
-    if (t == 0) delta[((long long)b * a.Hq + hq) * a.Nq + qi] = D;
-    float d0 = 0.f, d1 = 0.f;
-    for (int i = 0; i < a.Nk; ++i) {
-        if (mask && !mask[i]) continue;
-        const T *kr = k + i * a.k_sn, *vr = v + i * a.v_sn;
-        const float k0 = in0 ? (float)kr[t] : 0.f, k1 = in1 ? (float)kr[t + 64] : 0.f;
-        const float p = exp2f(md_wave_sum(q0 * k0 + q1 * k1) * c - lse);
-        const float ds = p * (md_wave_sum(g0 * (in0 ? (float)vr[t] : 0.f) + g1 * (in1 ? (float)vr[t + 64] : 0.f)) - D);
-        d0 = fmaf(ds, k0, d0);
-        d1 = fmaf(ds, k1, d1);
+template <class E, int NP> __device__ __forceinline__ void split8(const float (&v)[8], typename Vec<E>::v8 (&out)[NP]) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        float x = v[j];
+#pragma unroll
+        for (int p = 0; p < NP; ++p) {
+            out[p][j] = (E)x;
+            x -= (float)out[p][j];
+        }
     }
-    if (!a.dq) return;
-    T *dq = (T *)a.dq + at;
-    if (in0) dq[t] = (T)(d0 * a.scale);
-    if (in1) dq[t + 64] = (T)(d1 * a.scale);
 }
 
-// one wave per key row, over the queries of every head that shares it
+__device__ __forceinline__ float swap_halves_max(float v) {
+    auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float swap_halves_sum(float v) {
+    auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// 1 KB, 16 bytes per lane, from global memory straight to shared memory (lane order); complete after s_waitcnt vmcnt(0)
+__device__ __forceinline__ void load_chunk(const char *from, char *to, int lane) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(from + lane * 16),
+                                     (__attribute__((address_space(3))) void *)to, 16, 0, 0);
+}
+__device__ __forceinline__ void wait_loads_and_barrier() {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+}
+template <class E, int NP> __device__ __forceinline__ void read_frag(const char *at, int lane, typename Vec<E>::v8 (&out)[NP]) {
+#pragma unroll
+    for (int p = 0; p < NP; ++p) out[p] = *(const typename Vec<E>::v8 *)(at + p * 1024 + lane * 16);
+}
+
+// neighbouring workgroups of a launch go to the 8 dies in turn: give each die a contiguous share of the work, so that the tiles of one z share its cache
+__device__ __forceinline__ int die_order(int block, int blocks) {
+    const int per = (blocks + 7) / 8;
+    return (block % 8) * per + block / 8;
+}
+
+// ---------------------------------------------------------------- what the kernels are told
+struct Shape {
+    int B, Hk, G, Nq, N, M, Hq, d;
+    const int *idx, *cnt;          // valid keys of each sequence and their number, or null
+};
+__device__ __forceinline__ int keys_of(const Shape &s, int z) { return s.cnt ? s.cnt[z / s.Hk] : s.N; }
+__device__ __forceinline__ long long q_row(const Shape &s, int z, int r) {      // row r of z in (B, Nq, Hq)
+    const int b = z / s.Hk, g = r / s.Nq;
+    return ((long long)b * s.Nq + (r - g * s.Nq)) * s.Hq + (z - b * s.Hk) * s.G + g;
+}
+__device__ __forceinline__ long long k_row(const Shape &s, int z, int i) {      // i-th valid key of z in (B, N, Hk)
+    const int b = z / s.Hk;
+    return ((long long)b * s.N + (s.idx ? s.idx[(long long)b * s.N + i] : i)) * s.Hk + (z - b * s.Hk);
+}
+
+// ---------------------------------------------------------------- the valid keys of each sequence, in order
+__global__ __launch_bounds__(1024) void xa_compact_kernel(const unsigned char *__restrict__ mask, long long sb, int N, int *__restrict__ idx,
+                                                          int *__restrict__ cnt) {
+    __shared__ int wave_sum[16];
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    mask += blockIdx.x * sb;
+    idx += (long long)blockIdx.x * N;
+    const bool aligned = ((uintptr_t)mask & 15) == 0;
+    int base = 0;
+    for (long long at = 0; at < N; at += 16384) {
+        const long long first = at + t * 16;
+        unsigned bits = 0;
+        if (aligned && first + 16 <= N) {
+            const uint4 w = *(const uint4 *)(mask + first);
+            const unsigned word[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int j = 0; j < 16; ++j) bits |= ((word[j / 4] >> (8 * (j % 4))) & 0xFF ? 1u : 0u) << j;
+        } else {
+            for (int j = 0; j < 16; ++j)
+                if (first + j < N && mask[first + j]) bits |= 1u << j;
+        }
+        const int mine = __popc(bits);
+        int upto = mine;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int v = __shfl_up(upto, o);
+            if (lane >= o) upto += v;
+        }
+        if (lane == 63) wave_sum[wave] = upto;
+        __syncthreads();
+        int before = 0, all = 0;
+#pragma unroll
+        for (int w = 0; w < 16; ++w) {
+            before += w < wave ? wave_sum[w] : 0;
+            all += wave_sum[w];
+        }
+        int to = base + before + upto - mine;
+        for (; bits; bits &= bits - 1) idx[to++] = (int)(first + __ffs(bits) - 1);
+        base += all;
+        __syncthreads();
+    }
+    if (t == 0) cnt[blockIdx.x] = base;
+}
+
+// ---------------------------------------------------------------- operands into fragment order
+struct PackJob {
+    const void *x;
+    long long sb, sn, sh;
+    char *R, *T;                 // where to, either may be null
+    int tiles;                   // of 32 rows, per z; rows behind the last are written as zeros
+    int query;                   // rows are query rows (else valid keys)
+    int vec;                     // 16-byte loads: d and all strides are multiples of 8 elements, x is aligned
+    float sign;
+    unsigned *amax;              // largest |row|^2 as float bits, or null
+};
+struct PackArgs {
+    PackJob job[4];
+    int blocks[5];               // jobs' first workgroups; behind the last job: rows of masked keys to be zeroed in dk, dv
+    int jobs;
+    Shape s;
+    const void *o;               // with `stat`: of job 0 (the gradient g) also D = g . o and lse, per tile 32 + 32 floats in 1 KB
+    const float *lse;
+    char *stat;
+    const unsigned char *mask;
+    long long mask_sb;
+    void *dk, *dv;
+};
+
+template <class T, int KS>
+__global__ __launch_bounds__(64) void xa_pack_kernel(PackArgs a) {
+    using E = typename Frag<T>::E;
+    constexpr int NP = Frag<T>::NP, DP = 16 * KS, LD = DP + 16 / sizeof(T), DB = (KS + 1) / 2;
+    __shared__ __attribute__((aligned(16))) T rows[32 * LD];
+    const int lane = threadIdx.x, col = lane & 31, half = lane >> 5;
+    const Shape &s = a.s;
+    int j = 0;
+    while (j < a.jobs && (int)blockIdx.x >= a.blocks[j + 1]) ++j;
+    const int local = blockIdx.x - a.blocks[j];
+    if (j == a.jobs) {           // 32 rows of one sequence's dk, dv
+        const int per = (s.N + 31) / 32, b = local / per, n0 = (local % per) * 32;
+        const int len = s.Hk * s.d;
+        for (int n = n0; n < n0 + 32 && n < s.N; ++n)
+            if (!a.mask[b * a.mask_sb + n])
+                for (int i = lane; i < len; i += 64) {
+                    ((T *)a.dk)[((long long)b * s.N + n) * len + i] = (T)0.f;
+                    ((T *)a.dv)[((long long)b * s.N + n) * len + i] = (T)0.f;
+                }
+        return;
+    }
+    const PackJob &job = a.job[j];
+    const int z = local / job.tiles, tile = local % job.tiles, b = z / s.Hk, hk = z - b * s.Hk;
+    const int count = job.query ? s.M : keys_of(s, z);
+#pragma unroll
+    for (int c = 0; c < KS; ++c) {
+        const int chunk = c * 64 + lane, r = chunk / (2 * KS), off = chunk % (2 * KS) * 8, i = tile * 32 + r;
+        T v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = (T)0.f;
+        if (i < count) {
+            const T *x = (const T *)job.x;
+            if (job.query) {
+                const int g = i / s.Nq;
+                x += b * job.sb + (i - g * s.Nq) * job.sn + (hk * s.G + g) * job.sh;
+            } else
+                x += b * job.sb + (s.idx ? s.idx[(long long)b * s.N + i] : i) * job.sn + hk * job.sh;
+            if (job.vec) {
+                if (off < s.d)
+#pragma unroll
+                    for (int w = 0; w < (int)sizeof(T) / 2; ++w) ((uint4 *)v)[w] = ((const uint4 *)(x + off))[w];
+            } else {
+                for (int e = 0; e < 8; ++e)
+                    if (off + e < s.d) v[e] = x[off + e];
+            }
+        }
+#pragma unroll
+        for (int w = 0; w < (int)sizeof(T) / 2; ++w) ((uint4 *)(rows + r * LD + off))[w] = ((uint4 *)v)[w];
+    }
+    __syncthreads();
+    const long long at = (long long)z * job.tiles + tile;
+    if (job.R)
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+            float v[8];
+            typename Vec<E>::v8 p[NP];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = (float)rows[col * LD + 16 * k + 8 * half + e] * job.sign;
+            split8<E, NP>(v, p);
+#pragma unroll
+            for (int n = 0; n < NP; ++n) *(typename Vec<E>::v8 *)(job.R + ((at * KS + k) * NP + n) * 1024 + lane * 16) = p[n];
+        }
+    if (job.T)
+#pragma unroll
+        for (int f = 0; f < 2 * DB; ++f) {
+            const int dim = 32 * (f / 2) + col;
+            float v[8];
+            typename Vec<E>::v8 p[NP];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int r = 16 * (f % 2) + 8 * (e / 4) + 4 * half + e % 4;
+                v[e] = dim < DP ? (float)rows[r * LD + (dim < DP ? dim : 0)] * job.sign : 0.f;
+            }
+            split8<E, NP>(v, p);
+#pragma unroll
+            for (int n = 0; n < NP; ++n) *(typename Vec<E>::v8 *)(job.T + ((at * 2 * DB + f) * NP + n) * 1024 + lane * 16) = p[n];
+        }
+    if (j == 0 && a.stat) {
+        const int i = tile * 32 + col;
+        float D = 0.f;
+        if (i < s.M) {
+            const T *o = (const T *)a.o + q_row(s, z, i) * s.d;
+            for (int e = half * 8 * KS; e < (half + 1) * 8 * KS && e < s.d; ++e) D = fmaf((float)rows[col * LD + e], (float)o[e], D);
+        }
+        D = swap_halves_sum(D);
+        float *st = (float *)(a.stat + at * 1024);
+        if (half == 0) st[col] = i < s.M ? a.lse[(long long)z * s.M + i] : INFINITY;
+        else st[32 + col] = D;
+    }
+    if (job.amax) {
+        float q = 0.f;
+        for (int e = half * 8 * KS; e < (half + 1) * 8 * KS; ++e) q = fmaf((float)rows[col * LD + e], (float)rows[col * LD + e], q);
+        q = md_wave_max(swap_halves_sum(q));
+        if (lane == 0) atomicMax(job.amax, __float_as_uint(q));       // non-negative floats order as their bits; a maximum does not depend on the order
+    }
+}
+
+__global__ void xa_clear_kernel(unsigned *p) { p[threadIdx.x] = 0u; }
+
+// ---------------------------------------------------------------- forward, tiles of 32 queries per wave and step of TK keys
+struct TileArgs {
+    Shape s;
+    const char *Qr, *Kr, *Vt;                          // forward
+    const char *Qt, *Kt, *Vr, *Gr, *Gt, *stat;         // backward
+    int q_tiles, k_tiles, blocks, splits;
+    float c, scale;
+    void *o, *dq, *dk, *dv;
+    float *lse, *part, *part2, *ml;                      // partial results of a split launch: [split][z][row][d], [split][z][row][2]
+    const unsigned *amax;
+};
+
+template <class E> struct Shift { static constexpr float fwd = 0.f, bwd = 0.f; };
+template <> struct Shift<f16_t> { static constexpr float fwd = 7.f, bwd = 15.f; };
+
+template <class T, int KS, int QT, int TK>
+__global__ __launch_bounds__(256, 2) void xa_fwd_kernel(TileArgs a) {
+    using E = typename Frag<T>::E;
+    using v8 = typename Vec<E>::v8;
+    constexpr int NP = Frag<T>::NP, DB = (KS + 1) / 2, SUB = TK / 32;
+    constexpr int KC = SUB * KS * NP, VC = SUB * DB * 2 * NP;       // 1 KB chunks per step
+    __shared__ __attribute__((aligned(1024))) char lds[2][(KC + VC) * 1024];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, half = lane >> 5;
+    const int work = die_order(blockIdx.x, gridDim.x);
+    if (work >= a.blocks) return;
+    const int q_blocks = (a.q_tiles + 4 * QT - 1) / (4 * QT);
+    const int split = work % a.splits, qb = work / a.splits % q_blocks, z = work / a.splits / q_blocks;
+    const int n = keys_of(a.s, z), steps = (n + TK - 1) / TK;
+    const int first = (int)((long long)steps * split / a.splits), last = (int)((long long)steps * (split + 1) / a.splits);
+    const int q0 = (qb * 4 + wave) * QT;                // this wave's first query tile
+
+    v8 q[QT][KS][NP];
+    f32x16 o[QT][DB];
+    float m[QT], l[QT];
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+        const int tile = q0 + t < a.q_tiles ? q0 + t : a.q_tiles - 1;
+#pragma unroll
+        for (int k = 0; k < KS; ++k) read_frag<E, NP>(a.Qr + (((long long)z * a.q_tiles + tile) * KS + k) * NP * 1024, lane, q[t][k]);
+#pragma unroll
+        for (int b = 0; b < DB; ++b) o[t][b] = (f32x16)0.f;
+        m[t] = -INFINITY;
+        l[t] = 0.f;
+    }
+    const char *Kz = a.Kr + (long long)z * a.k_tiles * KS * NP * 1024, *Vz = a.Vt + (long long)z * a.k_tiles * DB * 2 * NP * 1024;
+    auto fetch = [&](int step) {
+        char *to = lds[step & 1];
+        for (int i = wave; i < KC + VC; i += 4)
+            load_chunk(i < KC ? Kz + ((long long)step * KC + i) * 1024 : Vz + ((long long)step * VC + i - KC) * 1024, to + i * 1024, lane);
+    };
+    if (first < last) fetch(first);
+    for (int step = first; step < last; ++step) {
+        wait_loads_and_barrier();
+        if (step + 1 < last) fetch(step + 1);
+        const char *K = lds[step & 1], *V = K + KC * 1024;
+#pragma unroll
+        for (int t = 0; t < QT; ++t) {
+            f32x16 s[SUB];
+#pragma unroll
+            for (int u = 0; u < SUB; ++u) {
+                s[u] = (f32x16)0.f;
+#pragma unroll
+                for (int k = 0; k < KS; ++k) {
+                    v8 f[NP];
+                    read_frag<E, NP>(K + (u * KS + k) * NP * 1024, lane, f);
+                    s[u] = mfma_pieces<E, NP>(f, q[t][k], s[u]);
+                }
+            }
+            if (step * TK + TK > n)                      // rows behind the last key
+#pragma unroll
+                for (int u = 0; u < SUB; ++u)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        if (step * TK + u * 32 + 8 * (r / 4) + 4 * half + r % 4 >= n) s[u][r] = -INFINITY;
+            float top = s[0][0];
+#pragma unroll
+            for (int u = 0; u < SUB; ++u)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) top = fmaxf(top, s[u][r]);
+            top = swap_halves_max(top) * a.c;
+            if (__any(top > m[t] + LAZY)) {
+                const float up = fmaxf(m[t], top), f = __builtin_amdgcn_exp2f(m[t] - up);
+                m[t] = up;
+                l[t] *= f;
+#pragma unroll
+                for (int b = 0; b < DB; ++b) o[t][b] *= f;
+            }
+            const float base = m[t] - Shift<E>::fwd;
+#pragma unroll
+            for (int u = 0; u < SUB; ++u)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    float p[8];
+                    v8 f[NP];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        p[e] = __builtin_amdgcn_exp2f(fmaf(s[u][8 * h + e], a.c, -base));
+                        l[t] += p[e];
+                    }
+                    split8<E, NP>(p, f);
+#pragma unroll
+                    for (int b = 0; b < DB; ++b) {
+                        v8 w[NP];
+                        read_frag<E, NP>(V + ((u * DB + b) * 2 + h) * NP * 1024, lane, w);
+                        o[t][b] = mfma_pieces<E, NP>(w, f, o[t][b]);
+                    }
+                }
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+        const int row = (q0 + t) * 32 + col;
+        const float sum = swap_halves_sum(l[t]), base = m[t] - Shift<E>::fwd;
+        if (row >= a.s.M) continue;
+        const long long zr = (long long)z * a.s.M + row;
+        if (a.splits > 1) {
+            const long long at = (long long)split * a.s.B * a.s.Hk * a.s.M + zr;
+            if (half == 0) {
+                a.ml[2 * at] = base;
+                a.ml[2 * at + 1] = sum;
+            }
+#pragma unroll
+            for (int b = 0; b < DB; ++b)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int dim = 32 * b + 8 * (r / 4) + 4 * half + r % 4;
+                    if (dim < a.s.d) a.part[at * a.s.d + dim] = o[t][b][r];
+                }
+        } else {
+            const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);     // (NaN stays NaN)
+            if (half == 0 && a.lse) a.lse[zr] = sum == 0.f ? INFINITY : base + __log2f(sum);
+            T *to = (T *)a.o + q_row(a.s, z, row) * a.s.d;
+#pragma unroll
+            for (int b = 0; b < DB; ++b)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int dim = 32 * b + 8 * (r / 4) + 4 * half + r % 4;
+                    if (dim < a.s.d) to[dim] = (T)(o[t][b][r] * inv);
+                }
+        }
+    }
+}
+
+// the splits of one row joined: O = sum 2^(m_i - m) O_i / sum 2^(m_i - m) l_i, m = max m_i
 template <class T>
-__global__ __launch_bounds__(64) void xa_dkv_kernel(md_attn_desc a, const float *__restrict__ delta) {
-    const int t = threadIdx.x, ki = blockIdx.x, hk = blockIdx.y, b = blockIdx.z, G = a.Hq / a.Hk;
-    const bool in0 = t < a.d, in1 = t + 64 < a.d;
-    const bool valid = !a.key_mask || ((const unsigned char *)a.key_mask)[b * a.mask_sb + ki];
-    float dk0 = 0.f, dk1 = 0.f, dv0 = 0.f, dv1 = 0.f;
-    if (valid) {
-        const T *k = (const T *)a.k + b * a.k_sb + ki * a.k_sn + hk * a.k_sh, *v = (const T *)a.v + b * a.v_sb + ki * a.v_sn + hk * a.v_sh;
-        const float c = a.scale * LOG2E, k0 = in0 ? (float)k[t] : 0.f, k1 = in1 ? (float)k[t + 64] : 0.f;
-        const float v0 = in0 ? (float)v[t] : 0.f, v1 = in1 ? (float)v[t + 64] : 0.f;
-        for (int h = hk * G; h < (hk + 1) * G; ++h)
-            for (int i = 0; i < a.Nq; ++i) {
-                const T *q = (const T *)a.q + b * a.q_sb + i * a.q_sn + h * a.q_sh, *g = (const T *)a.g + b * a.g_sb + i * a.g_sn + h * a.g_sh;
-                const float q0 = in0 ? (float)q[t] : 0.f, q1 = in1 ? (float)q[t + 64] : 0.f;
-                const float g0 = in0 ? (float)g[t] : 0.f, g1 = in1 ? (float)g[t + 64] : 0.f;
-                const long long r = ((long long)b * a.Hq + h) * a.Nq + i;
-                const float p = exp2f(md_wave_sum(q0 * k0 + q1 * k1) * c - a.lse[r]);
-                const float ds = p * (md_wave_sum(g0 * v0 + g1 * v1) - delta[r]);
-                dk0 = fmaf(ds, q0, dk0);
-                dk1 = fmaf(ds, q1, dk1);
-                dv0 = fmaf(p, g0, dv0);
-                dv1 = fmaf(p, g1, dv1);
+__global__ __launch_bounds__(64) void xa_join_kernel(TileArgs a) {
+    const int lane = threadIdx.x, z = blockIdx.x / a.s.M, row = blockIdx.x % a.s.M;
+    const long long rows = (long long)a.s.B * a.s.Hk * a.s.M, at = blockIdx.x;
+    float m = -INFINITY;
+    for (int i = 0; i < a.splits; ++i) m = fmaxf(m, a.ml[2 * (i * rows + at)]);
+    float sum = 0.f, o0 = 0.f, o1 = 0.f;
+    for (int i = 0; i < a.splits; ++i) {
+        const float mi = a.ml[2 * (i * rows + at)], li = a.ml[2 * (i * rows + at) + 1];
+        if (li == 0.f) continue;                       // no keys there
+        const float f = exp2f(mi - m);
+        sum = fmaf(f, li, sum);
+        const float *p = a.part + (i * rows + at) * a.s.d;
+        if (lane < a.s.d) o0 = fmaf(f, p[lane], o0);
+        if (lane + 64 < a.s.d) o1 = fmaf(f, p[lane + 64], o1);
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    T *to = (T *)a.o + q_row(a.s, z, row) * a.s.d;
+    if (lane < a.s.d) to[lane] = (T)(o0 * inv);
+    if (lane + 64 < a.s.d) to[lane + 64] = (T)(o1 * inv);
+    if (lane == 0 && a.lse) a.lse[at] = sum == 0.f ? INFINITY : m + log2f(sum);
+}
+
+// ---------------------------------------------------------------- backward
+// float16: dS times 2^k, |dS| 2^k < 2^15: |dS| <= |g v - D| <= 2 max|g| max|v|
+template <class E> __device__ __forceinline__ float ds_scale(const unsigned *amax) {
+    if constexpr (Shift<E>::bwd == 0.f) return 1.f;
+    const float sq = 4.f * __uint_as_float(amax[0]) * __uint_as_float(amax[1]);
+    if (!(sq > 0.f) || sq > 1e37f) return 1.f;
+    const int e2 = (int)(__float_as_uint(sq) >> 23) - 127;             // 2^e2 <= sq < 2^(e2 + 1)
+    int k = 14 - ((e2 + 2) >> 1);
+    k = k < -60 ? -60 : k > 60 ? 60 : k;
+    return __uint_as_float((unsigned)(127 + k) << 23);
+}
+
+template <class T, int KS, int QT, int TK>
+__global__ __launch_bounds__(256, Frag<T>::NP == 3 && KS > 4 ? 1 : 2) void xa_dq_kernel(TileArgs a) {
+    using E = typename Frag<T>::E;
+    using v8 = typename Vec<E>::v8;
+    constexpr int NP = Frag<T>::NP, DB = (KS + 1) / 2, SUB = TK / 32;
+    constexpr int RC = SUB * KS * NP, TC = SUB * DB * 2 * NP;
+    __shared__ __attribute__((aligned(1024))) char lds[2][(2 * RC + TC) * 1024];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, half = lane >> 5;
+    const int work = die_order(blockIdx.x, gridDim.x);
+    if (work >= a.blocks) return;
+    const int q_blocks = (a.q_tiles + 4 * QT - 1) / (4 * QT);
+    const int split = work % a.splits, qb = work / a.splits % q_blocks, z = work / a.splits / q_blocks;
+    const int n = keys_of(a.s, z), steps = (n + TK - 1) / TK;
+    const int first = (int)((long long)steps * split / a.splits), last = (int)((long long)steps * (split + 1) / a.splits);
+    const int q0 = (qb * 4 + wave) * QT;
+    const float up = ds_scale<E>(a.amax);
+
+    v8 q[QT][KS][NP], g[QT][KS][NP];
+    f32x16 dq[QT][DB];
+    float lse[QT], D[QT];
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+        const long long tile = (long long)z * a.q_tiles + (q0 + t < a.q_tiles ? q0 + t : a.q_tiles - 1);
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+            read_frag<E, NP>(a.Qr + (tile * KS + k) * NP * 1024, lane, q[t][k]);
+            read_frag<E, NP>(a.Gr + (tile * KS + k) * NP * 1024, lane, g[t][k]);
+        }
+#pragma unroll
+        for (int b = 0; b < DB; ++b) dq[t][b] = (f32x16)0.f;
+        lse[t] = ((const float *)(a.stat + tile * 1024))[col];
+        D[t] = ((const float *)(a.stat + tile * 1024))[32 + col];
+    }
+    const char *Kz = a.Kr + (long long)z * a.k_tiles * KS * NP * 1024, *Vz = a.Vr + (long long)z * a.k_tiles * KS * NP * 1024;
+    const char *Tz = a.Kt + (long long)z * a.k_tiles * DB * 2 * NP * 1024;
+    auto fetch = [&](int step) {
+        char *to = lds[step & 1];
+        for (int i = wave; i < 2 * RC + TC; i += 4)
+            load_chunk(i < RC ? Kz + ((long long)step * RC + i) * 1024 : i < 2 * RC ? Vz + ((long long)step * RC + i - RC) * 1024
+                                                                                     : Tz + ((long long)step * TC + i - 2 * RC) * 1024,
+                       to + i * 1024, lane);
+    };
+    if (first < last) fetch(first);
+    for (int step = first; step < last; ++step) {
+        wait_loads_and_barrier();
+        if (step + 1 < last) fetch(step + 1);
+        const char *K = lds[step & 1], *V = K + RC * 1024, *KT = V + RC * 1024;
+#pragma unroll
+        for (int u = 0; u < SUB; ++u)
+#pragma unroll
+            for (int t = 0; t < QT; ++t) {
+                f32x16 s = (f32x16)0.f, dp = (f32x16)(-D[t]);
+#pragma unroll
+                for (int k = 0; k < KS; ++k) {
+                    v8 f[NP];
+                    read_frag<E, NP>(K + (u * KS + k) * NP * 1024, lane, f);
+                    s = mfma_pieces<E, NP>(f, q[t][k], s);
+                    read_frag<E, NP>(V + (u * KS + k) * NP * 1024, lane, f);
+                    dp = mfma_pieces<E, NP>(f, g[t][k], dp);
+                }
+                if (step * TK + TK > n)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        if (step * TK + u * 32 + 8 * (r / 4) + 4 * half + r % 4 >= n) s[r] = -INFINITY, dp[r] = 0.f;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    float ds[8];
+                    v8 f[NP];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        ds[e] = __builtin_amdgcn_exp2f(fmaf(s[8 * h + e], a.c, -lse[t])) * dp[8 * h + e];
+                        if constexpr (Shift<E>::bwd != 0.f) ds[e] *= up;
+                    }
+                    split8<E, NP>(ds, f);
+#pragma unroll
+                    for (int b = 0; b < DB; ++b) {
+                        v8 w[NP];
+                        read_frag<E, NP>(KT + ((u * DB + b) * 2 + h) * NP * 1024, lane, w);
+                        dq[t][b] = mfma_pieces<E, NP>(w, f, dq[t][b]);
+                    }
+                }
             }
     }
-    const long long at = (((long long)b * a.Nk + ki) * a.Hk + hk) * a.d;
-    T *dk = (T *)a.dk + at, *dv = (T *)a.dv + at;
-    if (in0) dk[t] = (T)(dk0 * a.scale), dv[t] = (T)dv0;
-    if (in1) dk[t + 64] = (T)(dk1 * a.scale), dv[t + 64] = (T)dv1;
+    const float back = a.scale / up;
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+        const int row = (q0 + t) * 32 + col;
+        if (row >= a.s.M) continue;
+        float *part = a.part + ((long long)split * a.s.B * a.s.Hk * a.s.M + (long long)z * a.s.M + row) * a.s.d;
+        T *to = (T *)a.dq + q_row(a.s, z, row) * a.s.d;
+#pragma unroll
+        for (int b = 0; b < DB; ++b)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int dim = 32 * b + 8 * (r / 4) + 4 * half + r % 4;
+                if (dim < a.s.d) {
+                    if (a.splits > 1) part[dim] = dq[t][b][r] * back;
+                    else to[dim] = (T)(dq[t][b][r] * back);
+                }
+            }
+    }
 }
+
+// 32 KT keys per wave, steps of 32 queries
+template <class T, int KS, int KT>
+struct DkvLds {
+    static constexpr int NP = Frag<T>::NP, DB = (KS + 1) / 2, CHUNKS = 2 * KS * NP + 4 * DB * NP + 1;
+    static constexpr int BUFFERS = CHUNKS <= 80 ? 2 : 1;
+};
+
+template <class T, int KS, int KT>
+__global__ __launch_bounds__(256, (Frag<T>::NP == 3 && KS > 2) || KT * KS > 8 ? 1 : 2) void xa_dkv_kernel(TileArgs a) {
+    using E = typename Frag<T>::E;
+    using v8 = typename Vec<E>::v8;
+    using L = DkvLds<T, KS, KT>;
+    constexpr int NP = L::NP, DB = L::DB, RC = KS * NP, TC = DB * 2 * NP, NB = L::BUFFERS;
+    extern __shared__ __attribute__((aligned(1024))) char lds[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, half = lane >> 5;
+    const int work = die_order(blockIdx.x, gridDim.x);
+    if (work >= a.blocks) return;
+    const int k_blocks = (a.k_tiles + 4 * KT - 1) / (4 * KT);
+    const int split = work % a.splits, kb = work / a.splits % k_blocks, z = work / a.splits / k_blocks;
+    const int n = keys_of(a.s, z);
+    if (kb * 4 * KT * 32 >= n) return;
+    const int steps = a.q_tiles;
+    const int first = (int)((long long)steps * split / a.splits), last = (int)((long long)steps * (split + 1) / a.splits);
+    const int k0 = (kb * 4 + wave) * KT;
+    const float up = ds_scale<E>(a.amax);
+
+    v8 kf[KT][KS][NP], vf[KT][KS][NP];
+    f32x16 dk[KT][DB], dv[KT][DB];
+#pragma unroll
+    for (int t = 0; t < KT; ++t) {
+        const long long tile = (long long)z * a.k_tiles + (k0 + t < a.k_tiles ? k0 + t : a.k_tiles - 1);
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+            read_frag<E, NP>(a.Kr + (tile * KS + k) * NP * 1024, lane, kf[t][k]);
+            read_frag<E, NP>(a.Vr + (tile * KS + k) * NP * 1024, lane, vf[t][k]);
+        }
+#pragma unroll
+        for (int b = 0; b < DB; ++b) dk[t][b] = dv[t][b] = (f32x16)0.f;
+    }
+    const long long qz = (long long)z * a.q_tiles;
+    auto fetch = [&](int step) {
+        char *to = lds + (NB == 2 ? (step & 1) * L::CHUNKS * 1024 : 0);
+        const long long tile = qz + step;
+        for (int i = wave; i < L::CHUNKS; i += 4) {
+            const char *from = i < RC ? a.Qr + (tile * RC + i) * 1024 : i < 2 * RC ? a.Gr + (tile * RC + i - RC) * 1024
+                             : i < 2 * RC + TC ? a.Qt + (tile * TC + i - 2 * RC) * 1024
+                             : i < 2 * RC + 2 * TC ? a.Gt + (tile * TC + i - 2 * RC - TC) * 1024 : a.stat + tile * 1024;
+            load_chunk(from, to + i * 1024, lane);
+        }
+    };
+    if (first < last) fetch(first);
+    for (int step = first; step < last; ++step) {
+        wait_loads_and_barrier();
+        if (NB == 2 && step + 1 < last) fetch(step + 1);
+        const char *Q = lds + (NB == 2 ? (step & 1) * L::CHUNKS * 1024 : 0), *G = Q + RC * 1024, *QT = G + RC * 1024, *GT = QT + TC * 1024;
+        const float *st = (const float *)(GT + TC * 1024);
+#pragma unroll
+        for (int t = 0; t < KT; ++t) {
+            f32x16 s = (f32x16)0.f, dp;
+            float lse[16];
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                lse[r] = st[8 * (r / 4) + 4 * half + r % 4];
+                dp[r] = -st[32 + 8 * (r / 4) + 4 * half + r % 4];
+            }
+#pragma unroll
+            for (int k = 0; k < KS; ++k) {
+                v8 f[NP];
+                read_frag<E, NP>(Q + k * NP * 1024, lane, f);
+                s = mfma_pieces<E, NP>(f, kf[t][k], s);
+                read_frag<E, NP>(G + k * NP * 1024, lane, f);
+                dp = mfma_pieces<E, NP>(f, vf[t][k], dp);
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float p[8], ds[8];
+                v8 f[NP];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    p[e] = __builtin_amdgcn_exp2f(fmaf(s[8 * h + e], a.c, Shift<E>::bwd - lse[8 * h + e]));
+                    ds[e] = p[e] * dp[8 * h + e];
+                    if constexpr (Shift<E>::bwd != 0.f) ds[e] *= up * (1.f / 32768.f);
+                }
+                split8<E, NP>(p, f);
+#pragma unroll
+                for (int b = 0; b < DB; ++b) {
+                    v8 w[NP];
+                    read_frag<E, NP>(GT + (b * 2 + h) * NP * 1024, lane, w);
+                    dv[t][b] = mfma_pieces<E, NP>(w, f, dv[t][b]);
+                }
+                split8<E, NP>(ds, f);
+#pragma unroll
+                for (int b = 0; b < DB; ++b) {
+                    v8 w[NP];
+                    read_frag<E, NP>(QT + (b * 2 + h) * NP * 1024, lane, w);
+                    dk[t][b] = mfma_pieces<E, NP>(w, f, dk[t][b]);
+                }
+            }
+        }
+        if (NB == 1) {
+            __syncthreads();
+            if (step + 1 < last) fetch(step + 1);
+        }
+    }
+    const float back_k = a.scale / up, back_v = Shift<E>::bwd != 0.f ? 1.f / 32768.f : 1.f;
+#pragma unroll
+    for (int t = 0; t < KT; ++t) {
+        const int i = (k0 + t) * 32 + col;
+        if (i >= n) continue;
+        const long long at = ((long long)split * a.s.B * a.s.Hk + z) * a.s.N + i, to = k_row(a.s, z, i) * a.s.d;
+#pragma unroll
+        for (int b = 0; b < DB; ++b)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int dim = 32 * b + 8 * (r / 4) + 4 * half + r % 4;
+                if (dim < a.s.d) {
+                    const float x = dk[t][b][r] * back_k, y = dv[t][b][r] * back_v;
+                    if (a.splits > 1) {
+                        a.part[at * a.s.d + dim] = x;
+                        a.part2[at * a.s.d + dim] = y;
+                    } else {
+                        ((T *)a.dk)[to + dim] = (T)x;
+                        ((T *)a.dv)[to + dim] = (T)y;
+                    }
+                }
+            }
+    }
+}
+
+// the splits' sums in their order; one thread per element of dq, or of dk and dv
+template <class T>
+__global__ __launch_bounds__(256) void xa_sum_kernel(TileArgs a, int keys) {
+    const int rows = keys ? a.s.N : a.s.M;
+    const long long per = (long long)a.s.B * a.s.Hk * rows * a.s.d, e = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (e >= per) return;
+    const int dim = (int)(e % a.s.d), row = (int)(e / a.s.d % rows), z = (int)(e / a.s.d / rows);
+    if (keys && row >= keys_of(a.s, z)) return;
+    float x = 0.f, y = 0.f;
+    for (int i = 0; i < a.splits; ++i) {
+        x += a.part[i * per + e];
+        if (keys) y += a.part2[i * per + e];
+    }
+    if (keys) {
+        const long long to = k_row(a.s, z, row) * a.s.d + dim;
+        ((T *)a.dk)[to] = (T)x;
+        ((T *)a.dv)[to] = (T)y;
+    } else
+        ((T *)a.dq)[q_row(a.s, z, row) * a.s.d + dim] = (T)x;
+}
+
+// ---------------------------------------------------------------- a few query rows: K and V read once, in place
+// A key row is spread over LPR lanes (8 dims each), so 64 / LPR keys per wave and load; every lane group keeps its own m, l and O for all R query
+// rows and they are joined at the end: first within the workgroup, then, over the splits of the key axis, by xa_join.
+template <int LPR> __device__ __forceinline__ float group_sum(float v) {
+#define XA_DPP_ADD(ctrl) v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), ctrl, 0xF, 0xF, true))
+    if constexpr (LPR >= 2) XA_DPP_ADD(0xB1);
+    if constexpr (LPR >= 4) XA_DPP_ADD(0x4E);
+    if constexpr (LPR >= 8) XA_DPP_ADD(0x141);
+    if constexpr (LPR >= 16) XA_DPP_ADD(0x140);
+#undef XA_DPP_ADD
+    return v;
+}
+
+struct FewArgs {
+    Shape s;
+    const void *q, *k, *v;
+    long long q_sb, q_sn, q_sh, k_sb, k_sn, k_sh, v_sb, v_sn, v_sh, mask_sb;
+    const unsigned char *mask;
+    int splits;
+    float c;
+    void *o;
+    float *lse, *part, *ml;
+};
+
+template <class T, bool VEC> __device__ __forceinline__ void few_load(const T *x, int off, int d, float (&v)[8]) {
+    T raw[8];
+    if constexpr (VEC) {
+#pragma unroll
+        for (int w = 0; w < (int)sizeof(T) / 2; ++w) ((uint4 *)raw)[w] = off < d ? ((const uint4 *)(x + off))[w] : make_uint4(0, 0, 0, 0);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) raw[e] = off + e < d ? x[off + e] : (T)0.f;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = (float)raw[e];
+}
+
+template <class T, int R, int LPR, bool VEC>
+__global__ __launch_bounds__(256) void xa_few_kernel(FewArgs a) {
+    constexpr int GROUPS = 64 / LPR, U = 2;             // lane groups per wave, keys in flight per group
+    __shared__ float sm[4][R][2], so[4][R][LPR * 8];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, off = (lane % LPR) * 8, group = wave * GROUPS + lane / LPR;
+    const int split = blockIdx.x % a.splits, z = blockIdx.x / a.splits, b = z / a.s.Hk, hk = z - b * a.s.Hk;
+    const T *k = (const T *)a.k + b * a.k_sb + hk * a.k_sh, *v = (const T *)a.v + b * a.v_sb + hk * a.v_sh;
+    const unsigned char *mask = a.mask ? a.mask + b * a.mask_sb : nullptr;
+    const int n0 = (int)((long long)a.s.N * split / a.splits), n1 = (int)((long long)a.s.N * (split + 1) / a.splits);
+    float q[R][8], o[R][8], m[R], l[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const int g = r / a.s.Nq;
+        if (r < a.s.M) few_load<T, false>((const T *)a.q + b * a.q_sb + (r - g * a.s.Nq) * a.q_sn + (hk * a.s.G + g) * a.q_sh, off, a.s.d, q[r]);
+        else
+#pragma unroll
+            for (int e = 0; e < 8; ++e) q[r][e] = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            q[r][e] *= a.c;
+            o[r][e] = 0.f;
+        }
+        m[r] = -INFINITY;
+        l[r] = 0.f;
+    }
+    // every lane of a wave runs the same number of rounds: the row sums cross lanes
+    for (long long i0 = n0; i0 < n1; i0 += 4 * GROUPS * U) {
+        float kv[U][8], vv[U][8];
+        bool on[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const long long i = i0 + u * 4 * GROUPS + group;
+            on[u] = i < n1 && (!mask || mask[i < n1 ? i : n0]);
+            const long long at = i < n1 ? i : n0;
+            few_load<T, VEC>(k + at * a.k_sn, off, a.s.d, kv[u]);
+            few_load<T, VEC>(v + at * a.v_sn, off, a.s.d, vv[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (!on[u])
+#pragma unroll
+                for (int e = 0; e < 8; ++e) vv[u][e] = 0.f;         // what stands in a masked row may be NaN
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            float s[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                s[u] = 0.f;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) s[u] = fmaf(q[r][e], kv[u][e], s[u]);
+                s[u] = group_sum<LPR>(s[u]);
+                s[u] = on[u] ? s[u] : -INFINITY;
+            }
+            float top = s[0];
+#pragma unroll
+            for (int u = 1; u < U; ++u) top = fmaxf(top, s[u]);
+            if (__any(top > m[r] + LAZY)) {
+                const float up = fmaxf(m[r], top), f = up == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[r] - up);
+                m[r] = up;
+                l[r] *= f;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) o[r][e] *= f;
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const float p = on[u] ? __builtin_amdgcn_exp2f(s[u] - m[r]) : 0.f;
+                l[r] += p;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) o[r][e] = fmaf(p, vv[u][e], o[r][e]);
+            }
+        }
+    }
+    // join the lane groups of the wave, then the four waves
+#pragma unroll
+    for (int x = LPR; x < 64; x <<= 1)
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const float m2 = __shfl_xor(m[r], x), l2 = __shfl_xor(l[r], x), up = fmaxf(m[r], m2);
+            const float f = m[r] == -INFINITY ? 0.f : exp2f(m[r] - up), f2 = m2 == -INFINITY ? 0.f : exp2f(m2 - up);
+            m[r] = up;
+            l[r] = l[r] * f + l2 * f2;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) o[r][e] = o[r][e] * f + __shfl_xor(o[r][e], x) * f2;
+        }
+    if (lane < LPR)
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            if (lane == 0) {
+                sm[wave][r][0] = m[r];
+                sm[wave][r][1] = l[r];
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) so[wave][r][off + e] = o[r][e];
+        }
+    __syncthreads();
+    for (int i = threadIdx.x; i < R * LPR * 8; i += 256) {
+        const int r = i / (LPR * 8), dim = i % (LPR * 8);
+        if (r >= a.s.M || dim >= a.s.d) continue;
+        float up = sm[0][r][0], sum = 0.f, x = 0.f;
+#pragma unroll
+        for (int w = 1; w < 4; ++w) up = fmaxf(up, sm[w][r][0]);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float f = sm[w][r][0] == -INFINITY ? 0.f : exp2f(sm[w][r][0] - up);
+            sum = fmaf(f, sm[w][r][1], sum);
+            x = fmaf(f, so[w][r][dim], x);
+        }
+        const long long zr = (long long)z * a.s.M + r;
+        if (a.splits > 1) {
+            const long long at = (long long)split * a.s.B * a.s.Hk * a.s.M + zr;
+            a.part[at * a.s.d + dim] = x;
+            if (dim == 0) {
+                a.ml[2 * at] = up;
+                a.ml[2 * at + 1] = sum;
+            }
+        } else {
+            ((T *)a.o)[q_row(a.s, z, r) * a.s.d + dim] = (T)(sum == 0.f ? 0.f : x / sum);
+            if (dim == 0 && a.lse) a.lse[zr] = sum == 0.f ? INFINITY : up + log2f(sum);
+        }
+    }
+}
+
+// ---------------------------------------------------------------- host side
+constexpr int FEW_ROWS = 8;                  // query rows per key head up to which K and V are read in place
+constexpr int CUS = 256;
 
 int check(const md_attn_desc &a, const char *what) {
     MD_REQUIRE(a.dtype >= 0 && a.dtype <= 2, "%s: unknown dtype %d (0 f32, 1 bf16, 2 f16)", what, a.dtype);
@@ -103,16 +874,288 @@ int check(const md_attn_desc &a, const char *what) {
     MD_REQUIRE(a.d >= 1 && a.d <= MD_ATTN_MAX_D, "%s: head size %d (1 .. %d)", what, a.d, MD_ATTN_MAX_D);
     MD_REQUIRE(a.Hk >= 1 && a.Hq >= 1 && a.Hq % a.Hk == 0, "%s: %d query heads are not a multiple of %d key heads", what, a.Hq, a.Hk);
     MD_REQUIRE(a.Hq <= 65535 && a.B <= 65535, "%s: more than 65535 heads or sequences", what);
-    MD_REQUIRE(a.scale == a.scale, "%s: scale is NaN", what);
+    MD_REQUIRE((long long)a.B * a.Hq * a.Nq < (1LL << 31) - 65536 && (long long)a.B * a.Hk * a.Nk < (1LL << 31) - 65536 &&
+                   a.Nk < (1 << 30) && (long long)a.Hq / a.Hk * a.Nq < (1 << 30),
+               "%s: 2^31 rows or more", what);
+    MD_REQUIRE(a.scale - a.scale == 0.f, "%s: scale is not finite", what);
     return MD_OK;
 }
+
+int ks_of(int d) { return d <= 16 ? 1 : d <= 32 ? 2 : d <= 64 ? 4 : d <= 96 ? 6 : 8; }
+size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
+
+// How a call is run, and where its workspace's parts begin; the same for the size query and the launch.
+struct Plan {
+    int M, Z, KS, NP, DB, q_tiles, k_tiles;
+    bool few;
+    int qt, kt, tk;                               // query tiles and key tiles per wave, keys per step (forward, dq)
+    int splits, splits_q, splits_k;               // forward; dq over keys; dk, dv over queries
+    size_t idx, cnt, Qr, Kr, Vt, Qt, Kt, Vr, Gr, Gt, stat, amax, part, part2, ml, bytes;
+};
+
+// enough workgroups for the chip: split the long axis until there are about `want`, at least `least` steps each
+int split_for(long long blocks, long long steps, int want, int least) {
+    long long s = blocks ? (want + blocks - 1) / blocks : 1;
+    if (s > steps / least) s = steps / least;
+    return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
+}
+
+Plan make_plan(const md_attn_desc &a, bool backward) {
+    Plan p{};
+    p.M = a.Hq / a.Hk * a.Nq;
+    p.Z = a.B * a.Hk;
+    p.KS = ks_of(a.d);
+    p.NP = a.dtype == 0 ? 3 : 1;
+    p.DB = (p.KS + 1) / 2;
+    p.q_tiles = (p.M + 31) / 32;
+    p.k_tiles = (a.Nk + 63) / 64 * 2;
+    p.few = !backward && p.M <= FEW_ROWS;
+    size_t at = 0;
+    auto take = [&](size_t n) { const size_t r = at; at = align256(at + n); return r; };
+    const size_t rows = (size_t)p.Z * p.M, kb = 1024;
+    if (p.few) {
+        const int keys = a.Nk < 1 ? 1 : a.Nk;
+        p.splits = split_for(p.Z, keys, 4 * CUS, 128);
+        if (p.splits > 1) {
+            p.part = take(rows * p.splits * a.d * 4);
+            p.ml = take(rows * p.splits * 8);
+        }
+        p.bytes = at;
+        return p;
+    }
+    if (a.key_mask) {
+        p.idx = take((size_t)a.B * a.Nk * 4);
+        p.cnt = take((size_t)a.B * 4);
+    }
+    const size_t qR = (size_t)p.Z * p.q_tiles * p.KS * p.NP * kb, qT = (size_t)p.Z * p.q_tiles * p.DB * 2 * p.NP * kb;
+    const size_t kR = (size_t)p.Z * p.k_tiles * p.KS * p.NP * kb, kT = (size_t)p.Z * p.k_tiles * p.DB * 2 * p.NP * kb;
+    auto wgs = [&](int tiles, int per) { return (long long)p.Z * ((tiles + 4 * per - 1) / (4 * per)); };
+    // two query tiles per wave read every key fragment once for both; one where that leaves the chip short of workgroups, or registers
+    p.qt = p.NP == 1 && p.KS <= 4 && wgs(p.q_tiles, 2) >= 2 * CUS ? 2 : 1;
+    p.kt = 1;
+    p.tk = p.NP == 3 && p.KS > 2 ? 32 : 64;
+    p.Qr = take(qR);
+    p.Kr = take(kR);
+    if (!backward) {
+        p.Vt = take(kT);
+        p.splits = split_for(wgs(p.q_tiles, p.qt), (a.Nk + p.tk - 1) / p.tk, 2 * CUS, 4);
+        if (p.splits > 1) {
+            p.part = take(rows * p.splits * a.d * 4);
+            p.ml = take(rows * p.splits * 8);
+        }
+    } else {
+        p.tk = 32;
+        p.Vr = take(kR);
+        p.Kt = take(kT);
+        p.Qt = take(qT);
+        p.Gr = take(qR);
+        p.Gt = take(qT);
+        p.stat = take((size_t)p.Z * p.q_tiles * kb);
+        p.amax = take(256);
+        p.splits_q = split_for(wgs(p.q_tiles, p.qt), (a.Nk + p.tk - 1) / p.tk, 2 * CUS, 4);
+        p.splits_k = split_for(wgs(p.k_tiles, p.kt), p.q_tiles, 2 * CUS, 4);
+        const size_t nq = p.splits_q > 1 ? rows * p.splits_q * a.d * 4 : 0;
+        const size_t nk = p.splits_k > 1 ? (size_t)p.Z * a.Nk * p.splits_k * a.d * 4 : 0;
+        p.part = take(nq > nk ? nq : nk);            // dq's is summed before dk's is written
+        p.part2 = take(nk);
+    }
+    p.bytes = at;
+    return p;
+}
+
+bool aligned_rows(const void *x, size_t size, int d, long long sb, long long sn, long long sh) {
+    const long long e = 16 / (long long)size;
+    return d % 8 == 0 && ((uintptr_t)x & 15) == 0 && sb % e == 0 && sn % e == 0 && sh % e == 0;
+}
+
+template <class K> int set_lds(K kernel, int bytes) {
+    if (bytes > 64 * 1024) MD_CHECK_HIP(hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    return MD_OK;
+}
+
+unsigned grid8(long long blocks) { return (unsigned)((blocks + 7) / 8 * 8); }
+
+template <class T, int R> int launch_few(const FewArgs &f, int d, bool vec, hipStream_t s) {
+    const unsigned grid = (unsigned)f.s.B * f.s.Hk * f.splits;
+#define XA_FEW(LPR) \
+    if (vec) xa_few_kernel<T, R, LPR, true><<<grid, 256, 0, s>>>(f); else xa_few_kernel<T, R, LPR, false><<<grid, 256, 0, s>>>(f)
+    if (d <= 16) { XA_FEW(2); }
+    else if (d <= 32) { XA_FEW(4); }
+    else if (d <= 64) { XA_FEW(8); }
+    else { XA_FEW(16); }
+#undef XA_FEW
+    return MD_OK;
+}
+
+template <class T> int run_few(const md_attn_desc &a, const Plan &p, const Shape &sh, char *ws, hipStream_t s) {
+    FewArgs f{};
+    f.s = sh;
+    f.q = a.q, f.k = a.k, f.v = a.v;
+    f.q_sb = a.q_sb, f.q_sn = a.q_sn, f.q_sh = a.q_sh, f.k_sb = a.k_sb, f.k_sn = a.k_sn, f.k_sh = a.k_sh;
+    f.v_sb = a.v_sb, f.v_sn = a.v_sn, f.v_sh = a.v_sh, f.mask_sb = a.mask_sb;
+    f.mask = (const unsigned char *)a.key_mask;
+    f.splits = p.splits;
+    f.c = a.scale * LOG2E;
+    f.o = a.o, f.lse = a.lse;
+    f.part = (float *)(ws + p.part), f.ml = (float *)(ws + p.ml);
+    const bool vec = aligned_rows(a.k, sizeof(T), a.d, a.k_sb, a.k_sn, a.k_sh) && aligned_rows(a.v, sizeof(T), a.d, a.v_sb, a.v_sn, a.v_sh);
+    const int rc = p.M <= 1 ? launch_few<T, 1>(f, a.d, vec, s) : p.M <= 4 ? launch_few<T, 4>(f, a.d, vec, s) : launch_few<T, 8>(f, a.d, vec, s);
+    if (rc) return rc;
+    MD_CHECK_LAUNCH("md_cross_attn_fwd: few rows");
+    if (p.splits > 1) {
+        TileArgs t{};
+        t.s = sh, t.splits = p.splits, t.part = f.part, t.ml = f.ml, t.o = a.o, t.lse = a.lse;
+        xa_join_kernel<T><<<(unsigned)p.Z * p.M, 64, 0, s>>>(t);
+        MD_CHECK_LAUNCH("md_cross_attn_fwd: join");
+    }
+    return MD_OK;
+}
+
+// descriptor -> kernels' shape, and the list of valid keys where there is a mask
+int start(const md_attn_desc &a, const Plan &p, char *ws, hipStream_t s, Shape &sh) {
+    sh.B = a.B, sh.Hk = a.Hk, sh.G = a.Hq / a.Hk, sh.Nq = a.Nq, sh.N = a.Nk, sh.M = p.M, sh.Hq = a.Hq, sh.d = a.d;
+    if (a.key_mask && !p.few) {
+        sh.idx = (const int *)(ws + p.idx), sh.cnt = (const int *)(ws + p.cnt);
+        xa_compact_kernel<<<a.B, 1024, 0, s>>>((const unsigned char *)a.key_mask, a.mask_sb, a.Nk, (int *)(ws + p.idx), (int *)(ws + p.cnt));
+        MD_CHECK_LAUNCH("md_cross_attn: key list");
+    }
+    return MD_OK;
+}
+
+PackJob job_of(const void *x, long long sb, long long sn, long long sh, size_t size, int d, char *R, char *T, int tiles, int query, float sign) {
+    PackJob j{};
+    j.x = x, j.sb = sb, j.sn = sn, j.sh = sh, j.R = R, j.T = T, j.tiles = tiles, j.query = query, j.sign = sign;
+    j.vec = aligned_rows(x, size, d, sb, sn, sh);
+    return j;
+}
+
+template <class T, int KS> int launch_pack(PackArgs &k, const Plan &p, long long more, hipStream_t s) {
+    long long n = 0;
+    for (int i = 0; i < k.jobs; ++i) {
+        k.blocks[i] = (int)n;
+        n += (long long)p.Z * k.job[i].tiles;
+    }
+    k.blocks[k.jobs] = (int)n;
+    n += more;
+    MD_REQUIRE(n < (1LL << 31), "md_cross_attn: too many tiles");
+    if (n) xa_pack_kernel<T, KS><<<(unsigned)n, 64, 0, s>>>(k);
+    MD_CHECK_LAUNCH("md_cross_attn: pack");
+    return MD_OK;
+}
+
+template <class T, int KS> int run_fwd(const md_attn_desc &a, const Plan &p, const Shape &sh, char *ws, hipStream_t s) {
+    constexpr int NP = Frag<T>::NP, TK = NP == 3 && KS > 2 ? 32 : 64;
+    const float sign = a.scale < 0.f ? -1.f : 1.f;          // c > 0 in the kernels: a negative scale goes into q's sign
+    PackArgs k{};
+    k.s = sh, k.jobs = 3;
+    k.job[0] = job_of(a.q, a.q_sb, a.q_sn, a.q_sh, sizeof(T), a.d, ws + p.Qr, nullptr, p.q_tiles, 1, sign);
+    k.job[1] = job_of(a.k, a.k_sb, a.k_sn, a.k_sh, sizeof(T), a.d, ws + p.Kr, nullptr, p.k_tiles, 0, 1.f);
+    k.job[2] = job_of(a.v, a.v_sb, a.v_sn, a.v_sh, sizeof(T), a.d, nullptr, ws + p.Vt, p.k_tiles, 0, 1.f);
+    if (int rc = launch_pack<T, KS>(k, p, 0, s)) return rc;
+    TileArgs t{};
+    t.s = sh;
+    t.Qr = ws + p.Qr, t.Kr = ws + p.Kr, t.Vt = ws + p.Vt;
+    t.q_tiles = p.q_tiles, t.k_tiles = p.k_tiles, t.splits = p.splits;
+    t.c = fmaxf(fabsf(a.scale) * LOG2E, 1.2e-38f);         // not 0: the scores of rows behind the last key are -inf
+    t.o = a.o, t.lse = a.lse, t.part = (float *)(ws + p.part), t.ml = (float *)(ws + p.ml);
+    const long long blocks = (long long)p.Z * ((p.q_tiles + 4 * p.qt - 1) / (4 * p.qt)) * p.splits;
+    MD_REQUIRE(blocks < (1LL << 31) - 8, "md_cross_attn_fwd: too many tiles");
+    t.blocks = (int)blocks;
+    if constexpr (NP == 1 && KS <= 4) {
+        if (p.qt == 2) xa_fwd_kernel<T, KS, 2, TK><<<grid8(blocks), 256, 0, s>>>(t);
+        else xa_fwd_kernel<T, KS, 1, TK><<<grid8(blocks), 256, 0, s>>>(t);
+    } else
+        xa_fwd_kernel<T, KS, 1, TK><<<grid8(blocks), 256, 0, s>>>(t);
+    MD_CHECK_LAUNCH("md_cross_attn_fwd");
+    if (p.splits > 1) {
+        xa_join_kernel<T><<<(unsigned)p.Z * p.M, 64, 0, s>>>(t);
+        MD_CHECK_LAUNCH("md_cross_attn_fwd: join");
+    }
+    return MD_OK;
+}
+
+template <class T, int KS> int run_bwd(const md_attn_desc &a, const Plan &p, const Shape &sh, char *ws, hipStream_t s) {
+    constexpr int NP = Frag<T>::NP;
+    const float sign = a.scale < 0.f ? -1.f : 1.f;
+    PackArgs k{};
+    k.s = sh;
+    k.jobs = 4;
+    k.job[0] = job_of(a.g, a.g_sb, a.g_sn, a.g_sh, sizeof(T), a.d, ws + p.Gr, ws + p.Gt, p.q_tiles, 1, 1.f);
+    k.job[1] = job_of(a.q, a.q_sb, a.q_sn, a.q_sh, sizeof(T), a.d, ws + p.Qr, ws + p.Qt, p.q_tiles, 1, sign);
+    k.job[2] = job_of(a.k, a.k_sb, a.k_sn, a.k_sh, sizeof(T), a.d, ws + p.Kr, ws + p.Kt, p.k_tiles, 0, 1.f);
+    k.job[3] = job_of(a.v, a.v_sb, a.v_sn, a.v_sh, sizeof(T), a.d, ws + p.Vr, nullptr, p.k_tiles, 0, 1.f);
+    k.o = a.o, k.lse = a.lse, k.stat = ws + p.stat;
+    if (a.dtype == 2) {
+        unsigned *amax = (unsigned *)(ws + p.amax);
+        xa_clear_kernel<<<1, 2, 0, s>>>(amax);
+        MD_CHECK_LAUNCH("md_cross_attn_bwd: clear");
+        k.job[0].amax = amax, k.job[3].amax = amax + 1;
+    }
+    long long zero = 0;
+    if (a.key_mask && a.dk) {
+        k.mask = (const unsigned char *)a.key_mask, k.mask_sb = a.mask_sb, k.dk = a.dk, k.dv = a.dv;
+        zero = (long long)a.B * ((a.Nk + 31) / 32);
+    }
+    if (int rc = launch_pack<T, KS>(k, p, zero, s)) return rc;
+    TileArgs t{};
+    t.s = sh;
+    t.Qr = ws + p.Qr, t.Kr = ws + p.Kr, t.Vr = ws + p.Vr, t.Qt = ws + p.Qt, t.Kt = ws + p.Kt, t.Gr = ws + p.Gr, t.Gt = ws + p.Gt, t.stat = ws + p.stat;
+    t.q_tiles = p.q_tiles, t.k_tiles = p.k_tiles;
+    t.c = fmaxf(fabsf(a.scale) * LOG2E, 1.2e-38f);
+    t.dq = a.dq, t.dk = a.dk, t.dv = a.dv, t.part = (float *)(ws + p.part), t.part2 = (float *)(ws + p.part2);
+    t.amax = (const unsigned *)(ws + p.amax);
+    if (a.dq && p.M) {
+        t.scale = a.scale;
+        t.splits = p.splits_q;
+        const long long blocks = (long long)p.Z * ((p.q_tiles + 4 * p.qt - 1) / (4 * p.qt)) * t.splits;
+        MD_REQUIRE(blocks < (1LL << 31) - 8, "md_cross_attn_bwd: too many tiles");
+        t.blocks = (int)blocks;
+        if constexpr (NP == 1 && KS <= 4) {
+            if (p.qt == 2) xa_dq_kernel<T, KS, 2, 32><<<grid8(blocks), 256, 0, s>>>(t);
+            else xa_dq_kernel<T, KS, 1, 32><<<grid8(blocks), 256, 0, s>>>(t);
+        } else
+            xa_dq_kernel<T, KS, 1, 32><<<grid8(blocks), 256, 0, s>>>(t);
+        MD_CHECK_LAUNCH("md_cross_attn_bwd: dq");
+        if (t.splits > 1) {
+            xa_sum_kernel<T><<<md_cdiv((long long)p.Z * p.M * a.d, 256), 256, 0, s>>>(t, 0);
+            MD_CHECK_LAUNCH("md_cross_attn_bwd: dq sums");
+        }
+    }
+    if (a.dk && a.Nk) {
+        t.scale = fabsf(a.scale);                          // Q's fragments carry the sign
+        t.splits = p.splits_k;
+        const long long blocks = (long long)p.Z * ((p.k_tiles + 3) / 4) * t.splits;
+        MD_REQUIRE(blocks < (1LL << 31) - 8, "md_cross_attn_bwd: too many tiles");
+        t.blocks = (int)blocks;
+        using L = DkvLds<T, KS, 1>;
+        const int lds = L::BUFFERS * L::CHUNKS * 1024;
+        if (int rc = set_lds(xa_dkv_kernel<T, KS, 1>, lds)) return rc;
+        xa_dkv_kernel<T, KS, 1><<<grid8(blocks), 256, lds, s>>>(t);
+        MD_CHECK_LAUNCH("md_cross_attn_bwd: dk, dv");
+        if (t.splits > 1) {
+            xa_sum_kernel<T><<<md_cdiv((long long)p.Z * a.Nk * a.d, 256), 256, 0, s>>>(t, 1);
+            MD_CHECK_LAUNCH("md_cross_attn_bwd: dk, dv sums");
+        }
+    }
+    return MD_OK;
+}
+
+#define XA_DISPATCH(what, KSV, CALL)                                     \
+    MD_DISPATCH_DTYPE(a->dtype, what, switch (KSV) {                     \
+        case 1: rc = CALL<T, 1>(*a, p, sh, w, s); break;                 \
+        case 2: rc = CALL<T, 2>(*a, p, sh, w, s); break;                 \
+        case 4: rc = CALL<T, 4>(*a, p, sh, w, s); break;                 \
+        case 6: rc = CALL<T, 6>(*a, p, sh, w, s); break;                 \
+        default: rc = CALL<T, 8>(*a, p, sh, w, s); break;                \
+    })
 
 }  // namespace
 
 extern "C" size_t md_attn_desc_bytes(void) { return sizeof(md_attn_desc); }
 
 extern "C" size_t md_cross_attn_ws_bytes(const md_attn_desc *a, int backward) {
-    return a && backward && a->B > 0 && a->Nq > 0 && a->Hq > 0 ? (size_t)a->B * a->Hq * a->Nq * sizeof(float) : 0;
+    if (!a || check(*a, "md_cross_attn_ws_bytes") || a->B == 0) return 0;
+    return make_plan(*a, backward != 0).bytes;
 }
 
 extern "C" int md_cross_attn_fwd(const md_attn_desc *a, void *ws, size_t ws_bytes, md_stream_t stream) {
@@ -120,10 +1163,17 @@ extern "C" int md_cross_attn_fwd(const md_attn_desc *a, void *ws, size_t ws_byte
     if (int rc = check(*a, "md_cross_attn_fwd")) return rc;
     if (a->B == 0 || a->Nq == 0) return MD_OK;
     MD_REQUIRE(a->q && a->o && (a->Nk == 0 || (a->k && a->v)), "md_cross_attn_fwd: null pointer");
+    const Plan p = make_plan(*a, false);
+    MD_REQUIRE(ws_bytes >= p.bytes && (ws || p.bytes == 0), "md_cross_attn_fwd: workspace of %zu bytes, %zu needed", ws ? ws_bytes : (size_t)0, p.bytes);
+    MD_REQUIRE(((uintptr_t)ws & 255) == 0, "md_cross_attn_fwd: workspace is not aligned to 256 bytes");
     hipStream_t s = (hipStream_t)stream;
-    MD_DISPATCH_DTYPE(a->dtype, "md_cross_attn_fwd", xa_fwd_kernel<T><<<dim3(a->Nq, a->Hq, a->B), 64, 0, s>>>(*a));
-    MD_CHECK_LAUNCH("md_cross_attn_fwd");
-    return MD_OK;
+    char *w = (char *)ws;
+    Shape sh{};
+    int rc = start(*a, p, w, s, sh);
+    if (rc) return rc;
+    if (p.few) MD_DISPATCH_DTYPE(a->dtype, "md_cross_attn_fwd", rc = run_few<T>(*a, p, sh, w, s));
+    else XA_DISPATCH("md_cross_attn_fwd", p.KS, run_fwd);
+    return rc;
 }
 
 extern "C" int md_cross_attn_bwd(const md_attn_desc *a, void *ws, size_t ws_bytes, md_stream_t stream) {
@@ -133,17 +1183,14 @@ extern "C" int md_cross_attn_bwd(const md_attn_desc *a, void *ws, size_t ws_byte
     MD_REQUIRE((a->dk == nullptr) == (a->dv == nullptr), "md_cross_attn_bwd: dk and dv come together");
     MD_REQUIRE(a->Nq == 0 || (a->q && a->o && a->g && a->lse), "md_cross_attn_bwd: null pointer");
     MD_REQUIRE(a->Nk == 0 || (a->k && a->v), "md_cross_attn_bwd: null pointer");
-    MD_REQUIRE(ws_bytes >= md_cross_attn_ws_bytes(a, 1) && (ws || ws_bytes == 0), "md_cross_attn_bwd: workspace of %zu bytes, %zu needed", ws_bytes,
-               md_cross_attn_ws_bytes(a, 1));
+    const Plan p = make_plan(*a, true);
+    MD_REQUIRE(ws_bytes >= p.bytes && (ws || p.bytes == 0), "md_cross_attn_bwd: workspace of %zu bytes, %zu needed", ws ? ws_bytes : (size_t)0, p.bytes);
+    MD_REQUIRE(((uintptr_t)ws & 255) == 0, "md_cross_attn_bwd: workspace is not aligned to 256 bytes");
     hipStream_t s = (hipStream_t)stream;
-    float *delta = (float *)ws;
-    if (a->Nq) {
-        MD_DISPATCH_DTYPE(a->dtype, "md_cross_attn_bwd", xa_dq_kernel<T><<<dim3(a->Nq, a->Hq, a->B), 64, 0, s>>>(*a, delta));
-        MD_CHECK_LAUNCH("md_cross_attn_bwd: dq");
-    }
-    if (a->Nk && a->dk) {
-        MD_DISPATCH_DTYPE(a->dtype, "md_cross_attn_bwd", xa_dkv_kernel<T><<<dim3(a->Nk, a->Hk, a->B), 64, 0, s>>>(*a, delta));
-        MD_CHECK_LAUNCH("md_cross_attn_bwd: dk, dv");
-    }
-    return MD_OK;
+    char *w = (char *)ws;
+    Shape sh{};
+    int rc = start(*a, p, w, s, sh);
+    if (rc) return rc;
+    XA_DISPATCH("md_cross_attn_bwd", p.KS, run_bwd);
+    return rc;
 }
