@@ -2,48 +2,250 @@
 // h = g w:  dx = r (h - mean h - n mean(h n)),  dw = sum_rows g n,  db = sum_rows g.
 // Every sum is held in 32 bits; the mean is taken off before squaring, so a large common offset costs no digits of the variance.
 // With 8-bit codes (md_types.hpp) in place of x the backward's n is (x8 - m) r, with m and r those of x itself.
+//
+// Bound by memory: each row is read once into registers (16 bytes per lane and access at any alignment, so odd row lengths run like the others), and a
+// workgroup goes over many rows, so w and b are read, and the columns' sums kept, in registers.  A row takes TPR lanes with NV accesses
+// each; the few lanes of a short row leave a wave several rows at once.
+#include <algorithm>
+
 #include "md_types.hpp"
 
 namespace {
 
-template <class T>
-__global__ __launch_bounds__(64) void ln_fwd_kernel(const T *__restrict__ x, long long ldx, const float *__restrict__ w,
-                                                    const float *__restrict__ b, int C, float eps, T *__restrict__ y,
-                                                    float *__restrict__ stat, signed char *__restrict__ codes,
-                                                    signed char *__restrict__ scales) {
-    const long long row = blockIdx.x;
-    const int t = threadIdx.x;
-    x += row * ldx;
-    y += row * C;
+// sum over the TPR lanes of a row (TPR 256: over the workgroup, through shared memory; `slot` alternates so that one barrier is enough)
+template <int TPR> __device__ __forceinline__ float row_sum(float v, float *shared, int slot) {
+#define LN_DPP_ADD(ctrl) v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), ctrl, 0xF, 0xF, true))
+    LN_DPP_ADD(0xB1);
+    LN_DPP_ADD(0x4E);
+    LN_DPP_ADD(0x141);
+    if constexpr (TPR >= 16) LN_DPP_ADD(0x140);
+#undef LN_DPP_ADD
+    if constexpr (TPR >= 32) v += __shfl_xor(v, 16);
+    if constexpr (TPR >= 64) v += __shfl_xor(v, 32);
+    if constexpr (TPR == 256) {
+        if ((threadIdx.x & 63) == 0) shared[slot * 4 + (threadIdx.x >> 6)] = v;
+        __syncthreads();
+        v = (shared[slot * 4] + shared[slot * 4 + 1]) + (shared[slot * 4 + 2] + shared[slot * 4 + 3]);
+    }
+    return v;
+}
+
+template <class T, int TPR, int NV, bool ACT8>
+__global__ __launch_bounds__(256) void ln_fwd_kernel(const T *__restrict__ x, long long ldx, const float *__restrict__ w, const float *__restrict__ b,
+                                                     int rows, int C, float eps, T *__restrict__ y, float *__restrict__ stat,
+                                                     signed char *__restrict__ codes, signed char *__restrict__ scales) {
+    constexpr int W = Wide<T>::n, RPB = 256 / TPR;
+    __shared__ float shared[8];
+    const int sub = threadIdx.x % TPR;
+    float wv[NV][W], bv[NV][W];
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int j = 0; j < W; ++j) {
+            const int c = (i * TPR + sub) * W + j;
+            wv[i][j] = w && c < C ? w[c] : 1.f;
+            bv[i][j] = b && c < C ? b[c] : 0.f;
+        }
+    const float inv = 1.f / (float)C;
+    const int groups = (C + MD_ACT8_GROUP - 1) / MD_ACT8_GROUP;
+    // every lane runs the same rounds: sums cross lanes
+    for (long long at = (long long)blockIdx.x * RPB; at < rows; at += (long long)gridDim.x * RPB) {
+        const long long row = at + threadIdx.x / TPR;
+        const bool live = row < rows;
+        const T *xr = x + (live ? row : 0) * ldx;
+        float v[NV][W];
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) md_load_wide<T>(xr, (i * TPR + sub) * W, C, v[i]);
+        if constexpr (ACT8)
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const int c = (i * TPR + sub) * W;
+                const int code = md_act8_code<T>(md_act8_group_max(v[i]));
+                unsigned q[W / 4];
+                md_act8_encode(v[i], code, q);
+                if (live) {
+                    md_store_codes<T>(codes + row * C, c, C, q);
+                    if (c % MD_ACT8_GROUP == 0 && c < C) scales[row * groups + c / MD_ACT8_GROUP] = (signed char)code;
+                }
+            }
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int j = 0; j < W; ++j) s += v[i][j];
+        const float mean = row_sum<TPR>(s, shared, 0) * inv;
+        s = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int j = 0; j < W; ++j) {
+                v[i][j] = (i * TPR + sub) * W + j < C ? v[i][j] - mean : 0.f;
+                s = fmaf(v[i][j], v[i][j], s);
+            }
+        const float rstd = 1.f / sqrtf(row_sum<TPR>(s, shared, 1) * inv + eps);
+        if (!live) continue;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+#pragma unroll
+            for (int j = 0; j < W; ++j) v[i][j] = fmaf(v[i][j] * rstd, wv[i][j], bv[i][j]);
+            md_store_wide<T>(y + row * C, (i * TPR + sub) * W, C, v[i]);
+        }
+        if (stat && sub == 0) {
+            stat[2 * row] = mean;
+            stat[2 * row + 1] = rstd;
+        }
+    }
+}
+
+// dx and, with `part`, this workgroup's column sums [workgroup][2][C]
+template <class T, int TPR, int NV, bool ACT8>
+__global__ __launch_bounds__(256) void ln_bwd_kernel(const T *__restrict__ g, long long ldg, const T *__restrict__ x, long long ldx,
+                                                     const signed char *__restrict__ codes, const signed char *__restrict__ scales,
+                                                     const float *__restrict__ stat, const float *__restrict__ w, int rows, int C, T *__restrict__ dx,
+                                                     float *__restrict__ part) {
+    constexpr int W = Wide<T>::n, RPB = 256 / TPR;
+    __shared__ float shared[RPB > 1 ? 256 * W : 8];
+    const int sub = threadIdx.x % TPR;
+    float wv[NV][W], dw[NV][W], db[NV][W];
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int j = 0; j < W; ++j) {
+            const int c = (i * TPR + sub) * W + j;
+            wv[i][j] = w && c < C ? w[c] : 1.f;
+            dw[i][j] = db[i][j] = 0.f;
+        }
+    const float inv = 1.f / (float)C;
+    const int groups = (C + MD_ACT8_GROUP - 1) / MD_ACT8_GROUP;
+    for (long long at = (long long)blockIdx.x * RPB; at < rows; at += (long long)gridDim.x * RPB) {
+        const long long row = at + threadIdx.x / TPR;
+        const bool live = row < rows;
+        const long long from = live ? row : 0;
+        const float mean = stat[2 * from], rstd = stat[2 * from + 1];
+        float gv[NV][W], n[NV][W];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (i * TPR + sub) * W;
+            md_load_wide<T>(g + from * ldg, c, C, gv[i]);
+            if constexpr (ACT8) md_load_codes<T>(codes + from * C, c, C, c < C ? md_act8_scale(scales[from * groups + c / MD_ACT8_GROUP]) : 0.f, n[i]);
+            else md_load_wide<T>(x + from * ldx, c, C, n[i]);
+        }
+        float sh = 0.f, shn = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int j = 0; j < W; ++j) {
+                n[i][j] = (n[i][j] - mean) * rstd;           // (behind the row's end g is 0: no sum sees it)
+                const float h = gv[i][j] * wv[i][j];
+                sh += h;
+                shn = fmaf(h, n[i][j], shn);
+            }
+        sh = row_sum<TPR>(sh, shared, 0) * inv;
+        shn = row_sum<TPR>(shn, shared, 1) * inv;
+        if (live) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+#pragma unroll
+                for (int j = 0; j < W; ++j) {
+                    dw[i][j] = fmaf(gv[i][j], n[i][j], dw[i][j]);
+                    db[i][j] += gv[i][j];
+                }
+            if (dx)
+#pragma unroll
+                for (int i = 0; i < NV; ++i) {
+#pragma unroll
+                    for (int j = 0; j < W; ++j) gv[i][j] = rstd * (fmaf(gv[i][j], wv[i][j], -sh) - n[i][j] * shn);
+                    md_store_wide<T>(dx + row * C, (i * TPR + sub) * W, C, gv[i]);
+                }
+        }
+    }
+    if (!part) return;
+    part += (size_t)blockIdx.x * 2 * C;
+    if constexpr (RPB == 1) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int j = 0; j < W; ++j) {
+                const int c = (i * TPR + sub) * W + j;
+                if (c < C) part[c] = dw[i][j], part[C + c] = db[i][j];
+            }
+    } else {
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                __syncthreads();
+#pragma unroll
+                for (int j = 0; j < W; ++j) shared[threadIdx.x * W + j] = k ? db[i][j] : dw[i][j];
+                __syncthreads();
+                for (int e = threadIdx.x; e < TPR * W; e += 256) {
+                    const int c = i * TPR * W + e;
+                    float s = 0.f;
+                    for (int r = 0; r < RPB; ++r) s += shared[r * TPR * W + e];
+                    if (c < C) part[k * C + c] = s;
+                }
+            }
+    }
+}
+
+// ---------------------------------------------------------------- rows too long for a workgroup's registers: read again for each sum
+constexpr int LONG = 1024;
+
+__device__ __forceinline__ float block_sum(float v, float *shared) {
+    v = md_wave_sum(v);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) shared[threadIdx.x >> 6] = v;
+    __syncthreads();
     float s = 0.f;
-    for (int c = t; c < C; c += 64) s += (float)x[c];
-    const float mean = md_wave_sum(s) / (float)C;
+#pragma unroll
+    for (int i = 0; i < LONG / 64; ++i) s += shared[i];
+    return s;
+}
+
+template <class T>
+__global__ __launch_bounds__(LONG) void ln_long_fwd_kernel(const T *__restrict__ x, long long ldx, const float *__restrict__ w, const float *__restrict__ b,
+                                                           int C, float eps, T *__restrict__ y, float *__restrict__ stat,
+                                                           signed char *__restrict__ codes, signed char *__restrict__ scales) {
+    constexpr int W = Wide<T>::n;
+    __shared__ float shared[LONG / 64];
+    const long long row = blockIdx.x;
+    x += row * ldx;
+    float v[W], s = 0.f;
+    for (int c = threadIdx.x * W; c < C; c += LONG * W) {
+        md_load_wide<T>(x, c, C, v);
+#pragma unroll
+        for (int j = 0; j < W; ++j) s += v[j];
+    }
+    const float mean = block_sum(s, shared) / (float)C;
     s = 0.f;
-    for (int c = t; c < C; c += 64) {
-        const float d = (float)x[c] - mean;
-        s = fmaf(d, d, s);
+    for (int c = threadIdx.x * W; c < C; c += LONG * W) {
+        md_load_wide<T>(x, c, C, v);
+#pragma unroll
+        for (int j = 0; j < W; ++j) {
+            const float d = c + j < C ? v[j] - mean : 0.f;
+            s = fmaf(d, d, s);
+        }
     }
-    const float rstd = 1.f / sqrtf(md_wave_sum(s) / (float)C + eps);
-    for (int c = t; c < C; c += 64) {
-        const float v = ((float)x[c] - mean) * rstd;
-        y[c] = (T)fmaf(v, w ? w[c] : 1.f, b ? b[c] : 0.f);
+    const float rstd = 1.f / sqrtf(block_sum(s, shared) / (float)C + eps);
+    const int groups = (C + MD_ACT8_GROUP - 1) / MD_ACT8_GROUP, rounds = (C + LONG * W - 1) / (LONG * W);
+    for (int i = 0; i < rounds; ++i) {                    // whole rounds: a group's lanes exchange its maximum
+        const int c = (i * LONG + threadIdx.x) * W;
+        md_load_wide<T>(x, c, C, v);
+        if (codes) {
+            const int code = md_act8_code<T>(md_act8_group_max(v));
+            unsigned q[W / 4];
+            md_act8_encode(v, code, q);
+            md_store_codes<T>(codes + row * C, c, C, q);
+            if (c % MD_ACT8_GROUP == 0 && c < C) scales[row * groups + c / MD_ACT8_GROUP] = (signed char)code;
+        }
+#pragma unroll
+        for (int j = 0; j < W; ++j)
+            if (c + j < C) v[j] = fmaf((v[j] - mean) * rstd, w ? w[c + j] : 1.f, b ? b[c + j] : 0.f);
+        md_store_wide<T>(y + row * C, c, C, v);
     }
-    if (stat && t == 0) {
+    if (stat && threadIdx.x == 0) {
         stat[2 * row] = mean;
         stat[2 * row + 1] = rstd;
-    }
-    if (codes) {
-        const int groups = (C + MD_ACT8_GROUP - 1) / MD_ACT8_GROUP;
-        for (int g = t; g < groups; g += 64) {
-            const int hi = min(C, (g + 1) * MD_ACT8_GROUP);
-            unsigned amax = 0;
-            for (int c = g * MD_ACT8_GROUP; c < hi; ++c) amax = max(amax, __float_as_uint((float)x[c]) & 0x7FFFFFFFu);
-            const int code = md_act8_code<T>(amax);
-            const float inv = md_act8_inv(code);
-            for (int c = g * MD_ACT8_GROUP; c < hi; ++c)
-                codes[row * C + c] = code == MD_ACT8_NAN ? 0 : (signed char)md_act8_round((float)x[c], inv);
-            scales[row * groups + g] = (signed char)code;
-        }
     }
 }
 
@@ -55,34 +257,31 @@ __device__ __forceinline__ float ln_value(const T *x, long long ldx, const signe
 }
 
 template <class T>
-__global__ __launch_bounds__(64) void ln_dx_kernel(const T *__restrict__ g, long long ldg, const T *__restrict__ x, long long ldx,
-                                                   const signed char *__restrict__ codes, const signed char *__restrict__ scales,
-                                                   const float *__restrict__ stat, const float *__restrict__ w, int C, T *__restrict__ dx) {
+__global__ __launch_bounds__(LONG) void ln_long_dx_kernel(const T *__restrict__ g, long long ldg, const T *__restrict__ x, long long ldx,
+                                                          const signed char *__restrict__ codes, const signed char *__restrict__ scales,
+                                                          const float *__restrict__ stat, const float *__restrict__ w, int C, T *__restrict__ dx) {
+    __shared__ float shared[LONG / 64];
     const long long row = blockIdx.x;
-    const int t = threadIdx.x;
     const float mean = stat[2 * row], rstd = stat[2 * row + 1];
     float sh = 0.f, shn = 0.f;
-    for (int c = t; c < C; c += 64) {
+    for (int c = threadIdx.x; c < C; c += LONG) {
         const float h = (float)g[row * ldg + c] * (w ? w[c] : 1.f);
-        const float n = (ln_value(x, ldx, codes, scales, row, C, c) - mean) * rstd;
         sh += h;
-        shn = fmaf(h, n, shn);
+        shn = fmaf(h, (ln_value(x, ldx, codes, scales, row, C, c) - mean) * rstd, shn);
     }
-    sh = md_wave_sum(sh) / (float)C;
-    shn = md_wave_sum(shn) / (float)C;
-    for (int c = t; c < C; c += 64) {
+    sh = block_sum(sh, shared) / (float)C;
+    shn = block_sum(shn, shared) / (float)C;
+    for (int c = threadIdx.x; c < C; c += LONG) {
         const float h = (float)g[row * ldg + c] * (w ? w[c] : 1.f);
-        const float n = (ln_value(x, ldx, codes, scales, row, C, c) - mean) * rstd;
-        dx[row * C + c] = (T)(rstd * (h - sh - n * shn));
+        dx[row * C + c] = (T)(rstd * (h - sh - (ln_value(x, ldx, codes, scales, row, C, c) - mean) * rstd * shn));
     }
 }
 
-// one thread per column and slice of rows: partial sums [slice][2][C]
 template <class T>
-__global__ __launch_bounds__(64) void ln_dwdb_kernel(const T *__restrict__ g, long long ldg, const T *__restrict__ x, long long ldx,
-                                                     const signed char *__restrict__ codes, const signed char *__restrict__ scales,
-                                                     const float *__restrict__ stat, long long rows, int C, float *__restrict__ part) {
-    const int c = blockIdx.x * 64 + threadIdx.x;
+__global__ __launch_bounds__(256) void ln_long_columns_kernel(const T *__restrict__ g, long long ldg, const T *__restrict__ x, long long ldx,
+                                                              const signed char *__restrict__ codes, const signed char *__restrict__ scales,
+                                                              const float *__restrict__ stat, long long rows, int C, float *__restrict__ part) {
+    const int c = blockIdx.x * 256 + threadIdx.x;
     if (c >= C) return;
     float dw = 0.f, db = 0.f;
     for (long long row = blockIdx.y; row < rows; row += gridDim.y) {
@@ -94,24 +293,66 @@ __global__ __launch_bounds__(64) void ln_dwdb_kernel(const T *__restrict__ g, lo
     part[(size_t)blockIdx.y * 2 * C + C + c] = db;
 }
 
-__global__ __launch_bounds__(64) void ln_dwdb_sum_kernel(const float *__restrict__ part, int slices, int C, float *__restrict__ dw,
-                                                         float *__restrict__ db) {
-    const int c = blockIdx.x * 64 + threadIdx.x;
-    if (c >= 2 * C) return;
-    double s = 0.;
-    for (int i = 0; i < slices; ++i) s += part[(size_t)i * 2 * C + c];
-    if (c < C) {
-        if (dw) dw[c] = (float)s;
-    } else if (db) db[c - C] = (float)s;
+// ---------------------------------------------------------------- the workgroups' column sums in a fixed order: 32 columns x 32 shares of the workgroups
+__global__ __launch_bounds__(1024) void ln_sum_kernel(const float *__restrict__ part, int slices, int C, float *__restrict__ dw, float *__restrict__ db) {
+    __shared__ float shared[32][33];
+    const int col = threadIdx.x & 31, share = threadIdx.x >> 5, c = blockIdx.x * 32 + col;
+    float s = 0.f;
+    if (c < 2 * C)
+        for (int i = share; i < slices; i += 32) s += part[(size_t)i * 2 * C + c];
+    shared[share][col] = s;
+    __syncthreads();
+    if (share == 0 && c < 2 * C) {
+        s = 0.f;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) s += shared[i][col];
+        if (c < C) {
+            if (dw) dw[c] = s;
+        } else if (db)
+            db[c - C] = s;
+    }
 }
 
-constexpr int LN_SLICES = 512;
+// ---------------------------------------------------------------- host side
+constexpr int CUS = 256;
+
+// lanes per row and accesses per lane for a row of `wide` 16-byte pieces: up to 4 accesses a lane before a row takes more lanes
+struct Split { int tpr, nv; };
+Split split_of(int wide) {
+    if (wide <= 8) return {8, 1};
+    if (wide <= 16) return {16, 1};
+    if (wide <= 32) return {32, 1};
+    if (wide <= 64) return {64, 1};
+    if (wide <= 128) return {64, 2};
+    if (wide <= 256) return {64, 4};
+    if (wide <= 512) return {256, 2};
+    if (wide <= 1024) return {256, 4};
+    return {0, 0};                                 // too long for registers
+}
+int pieces(int dtype, int C) { return md_cdiv(C, 16 / (int)md_dtype_bytes(dtype)); }
+int fwd_blocks(long long rows, int tpr) { return (int)std::min<long long>(md_cdiv(rows, 256 / tpr), 8 * CUS); }
+// workgroups of the backward pass: each leaves 2 C partial sums, so no more than the chip needs to stream
+int bwd_blocks(long long rows, int tpr) { return (int)std::min<long long>(md_cdiv(rows, 256 / tpr), 2 * CUS); }
+int column_slices(long long rows) { return (int)std::min<long long>(rows, 64); }
+
+#define LN_CONFIG(S, ...)                                                                      \
+    switch ((S).tpr * 10 + (S).nv) {                                                           \
+        case 81: { constexpr int TPR = 8, NV = 1; __VA_ARGS__; } break;                        \
+        case 161: { constexpr int TPR = 16, NV = 1; __VA_ARGS__; } break;                      \
+        case 321: { constexpr int TPR = 32, NV = 1; __VA_ARGS__; } break;                      \
+        case 641: { constexpr int TPR = 64, NV = 1; __VA_ARGS__; } break;                      \
+        case 642: { constexpr int TPR = 64, NV = 2; __VA_ARGS__; } break;                      \
+        case 644: { constexpr int TPR = 64, NV = 4; __VA_ARGS__; } break;                      \
+        case 2562: { constexpr int TPR = 256, NV = 2; __VA_ARGS__; } break;                    \
+        default: { constexpr int TPR = 256, NV = 4; __VA_ARGS__; } break;                      \
+    }
 
 }  // namespace
 
 #define LN_CHECK(what)                                                                                                        \
     MD_REQUIRE(rows >= 0 && C >= 1 && C <= (1 << 20), "%s: %lld rows of %d columns (1 .. 2^20 columns)", what, rows, C);      \
     MD_REQUIRE(rows <= 0x7FFFFFFF, "%s: more than 2^31 - 1 rows", what);                                                      \
+    MD_REQUIRE(dtype >= 0 && dtype <= 2, "%s: unknown dtype %d (0 f32, 1 bf16, 2 f16)", what, dtype);                         \
     MD_REQUIRE((codes == nullptr) == (scales == nullptr), "%s: codes and scales come together", what)
 
 extern "C" int md_layer_norm_fwd(const void *x, int dtype, long long rows, int C, long long ldx, const float *w, const float *b, float eps,
@@ -122,16 +363,26 @@ extern "C" int md_layer_norm_fwd(const void *x, int dtype, long long rows, int C
     MD_REQUIRE(x && y, "md_layer_norm_fwd: null pointer");
     MD_REQUIRE(ldx >= C || rows == 1, "md_layer_norm_fwd: row stride %lld below %d columns", ldx, C);
     hipStream_t s = (hipStream_t)stream;
-    MD_DISPATCH_DTYPE(dtype, "md_layer_norm_fwd",
-                      ln_fwd_kernel<T><<<(unsigned)rows, 64, 0, s>>>((const T *)x, ldx, w, b, C, eps, (T *)y, stat, (signed char *)codes,
-                                                                     (signed char *)scales));
+    signed char *cd = (signed char *)codes, *sc = (signed char *)scales;
+    const Split sp = split_of(pieces(dtype, C));
+    if (!sp.tpr) {
+        MD_DISPATCH_DTYPE(dtype, "md_layer_norm_fwd",
+                          ln_long_fwd_kernel<T><<<(unsigned)rows, LONG, 0, s>>>((const T *)x, ldx, w, b, C, eps, (T *)y, stat, cd, sc));
+    } else {
+        const int grid = fwd_blocks(rows, sp.tpr);
+        MD_DISPATCH_DTYPE(dtype, "md_layer_norm_fwd", LN_CONFIG(sp, {
+            if (codes) ln_fwd_kernel<T, TPR, NV, true><<<grid, 256, 0, s>>>((const T *)x, ldx, w, b, (int)rows, C, eps, (T *)y, stat, cd, sc);
+            else ln_fwd_kernel<T, TPR, NV, false><<<grid, 256, 0, s>>>((const T *)x, ldx, w, b, (int)rows, C, eps, (T *)y, stat, cd, sc);
+        }));
+    }
     MD_CHECK_LAUNCH("md_layer_norm_fwd");
     return MD_OK;
 }
 
 extern "C" size_t md_layer_norm_bwd_ws_bytes(long long rows, int C) {
     if (rows < 1 || C < 1) return 0;
-    return (size_t)(rows < LN_SLICES ? rows : LN_SLICES) * 2 * C * sizeof(float);
+    // a workgroup per row at the most, and never more than bwd_blocks or column_slices give
+    return (size_t)std::min<long long>(rows, 2 * CUS) * 2 * C * sizeof(float);
 }
 
 extern "C" int md_layer_norm_bwd(const void *g, long long ldg, const void *x, long long ldx, const void *codes, const void *scales, int dtype,
@@ -139,27 +390,34 @@ extern "C" int md_layer_norm_bwd(const void *g, long long ldg, const void *x, lo
                                  size_t ws_bytes, md_stream_t stream) {
     LN_CHECK("md_layer_norm_bwd");
     hipStream_t s = (hipStream_t)stream;
+    const bool sums = dw || db;
+    int slices = 0;
     if (rows > 0) {
         MD_REQUIRE(g && stat && (x || codes), "md_layer_norm_bwd: null pointer");
         MD_REQUIRE((ldg >= C || rows == 1) && (codes || ldx >= C || rows == 1), "md_layer_norm_bwd: row stride below %d columns", C);
-        MD_REQUIRE(!(dw || db) || (ws && ws_bytes >= md_layer_norm_bwd_ws_bytes(rows, C)), "md_layer_norm_bwd: workspace of %zu bytes, %zu needed",
+        MD_REQUIRE(!sums || (ws && ws_bytes >= md_layer_norm_bwd_ws_bytes(rows, C)), "md_layer_norm_bwd: workspace of %zu bytes, %zu needed",
                    ws_bytes, md_layer_norm_bwd_ws_bytes(rows, C));
-    }
-    const signed char *cd = (const signed char *)codes, *sc = (const signed char *)scales;
-    if (rows > 0 && dx) {
-        MD_DISPATCH_DTYPE(dtype, "md_layer_norm_bwd",
-                          ln_dx_kernel<T><<<(unsigned)rows, 64, 0, s>>>((const T *)g, ldg, (const T *)x, ldx, cd, sc, stat, w, C, (T *)dx));
-        MD_CHECK_LAUNCH("md_layer_norm_bwd: dx");
-    }
-    if (dw || db) {
-        const int slices = (int)(rows < LN_SLICES ? rows : LN_SLICES);
-        if (slices > 0) {
-            MD_DISPATCH_DTYPE(dtype, "md_layer_norm_bwd",
-                              ln_dwdb_kernel<T><<<dim3(md_cdiv(C, 64), slices), 64, 0, s>>>((const T *)g, ldg, (const T *)x, ldx, cd, sc, stat,
-                                                                                            rows, C, (float *)ws));
-            MD_CHECK_LAUNCH("md_layer_norm_bwd: partial sums");
+        const signed char *cd = (const signed char *)codes, *sc = (const signed char *)scales;
+        const Split sp = split_of(pieces(dtype, C));
+        if (!sp.tpr) {
+            slices = column_slices(rows);
+            MD_DISPATCH_DTYPE(dtype, "md_layer_norm_bwd", {
+                if (dx) ln_long_dx_kernel<T><<<(unsigned)rows, LONG, 0, s>>>((const T *)g, ldg, (const T *)x, ldx, cd, sc, stat, w, C, (T *)dx);
+                if (sums) ln_long_columns_kernel<T><<<dim3(md_cdiv(C, 256), slices), 256, 0, s>>>((const T *)g, ldg, (const T *)x, ldx, cd, sc, stat, rows,
+                                                                                                   C, (float *)ws);
+            });
+        } else {
+            slices = bwd_blocks(rows, sp.tpr);
+            float *part = sums ? (float *)ws : nullptr;
+            MD_DISPATCH_DTYPE(dtype, "md_layer_norm_bwd", LN_CONFIG(sp, {
+                if (codes) ln_bwd_kernel<T, TPR, NV, true><<<slices, 256, 0, s>>>((const T *)g, ldg, (const T *)x, ldx, cd, sc, stat, w, (int)rows, C, (T *)dx, part);
+                else ln_bwd_kernel<T, TPR, NV, false><<<slices, 256, 0, s>>>((const T *)g, ldg, (const T *)x, ldx, cd, sc, stat, w, (int)rows, C, (T *)dx, part);
+            }));
         }
-        ln_dwdb_sum_kernel<<<md_cdiv(2 * C, 64), 64, 0, s>>>((const float *)ws, slices, C, dw, db);
+        MD_CHECK_LAUNCH("md_layer_norm_bwd");
+    }
+    if (sums) {
+        ln_sum_kernel<<<md_cdiv(2 * C, 32), 1024, 0, s>>>((const float *)ws, slices, C, dw, db);
         MD_CHECK_LAUNCH("md_layer_norm_bwd: sums");
     }
     return MD_OK;

@@ -53,3 +53,90 @@ __device__ __forceinline__ int md_act8_round(float x, float inv) {
     const float r = rintf(x * inv);
     return (int)fminf(fmaxf(r, -127.f), 127.f);
 }
+
+// ---------------------------------------------------------------- 16 bytes of T, or as many 8-bit codes, at any element's address
+// (global memory takes 16-byte accesses at every alignment; rows of odd length then run like the others)
+using md_u32x4 = unsigned __attribute__((ext_vector_type(4)));
+template <class T> struct Wide {
+    static constexpr int n = 16 / (int)sizeof(T);
+    struct __attribute__((packed, aligned(sizeof(T)))) Mem { md_u32x4 v; };
+    struct __attribute__((packed, aligned(1))) Codes { unsigned char b[n]; };
+};
+
+// elements at .. at + n - 1 of a row of `len`, zeros behind its end
+template <class T> __device__ __forceinline__ void md_load_wide(const T *row, int at, int len, float (&v)[Wide<T>::n]) {
+    constexpr int n = Wide<T>::n;
+    T raw[n];
+    if (at + n <= len) {
+        const md_u32x4 w = ((const typename Wide<T>::Mem *)(row + at))->v;
+        __builtin_memcpy(raw, &w, 16);
+    } else {
+#pragma unroll
+        for (int j = 0; j < n; ++j) raw[j] = at + j < len ? row[at + j] : (T)0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < n; ++j) v[j] = (float)raw[j];
+}
+template <class T> __device__ __forceinline__ void md_store_wide(T *row, int at, int len, const float (&v)[Wide<T>::n]) {
+    constexpr int n = Wide<T>::n;
+    T raw[n];
+#pragma unroll
+    for (int j = 0; j < n; ++j) raw[j] = (T)v[j];
+    if (at + n <= len) {
+        md_u32x4 w;
+        __builtin_memcpy(&w, raw, 16);
+        ((typename Wide<T>::Mem *)(row + at))->v = w;
+    } else {
+#pragma unroll
+        for (int j = 0; j < n; ++j)
+            if (at + j < len) row[at + j] = raw[j];
+    }
+}
+
+// largest bit pattern of a group's magnitudes, over the 32 / n lanes that hold it
+template <int n> __device__ __forceinline__ unsigned md_act8_group_max(const float (&v)[n]) {
+    int m = 0;
+#pragma unroll
+    for (int j = 0; j < n; ++j) m = max(m, (int)(__float_as_uint(v[j]) & 0x7FFFFFFFu));
+    m = max(m, __builtin_amdgcn_update_dpp(m, m, 0xB1, 0xF, 0xF, false));           // lane ^ 1
+    m = max(m, __builtin_amdgcn_update_dpp(m, m, 0x4E, 0xF, 0xF, false));           // lane ^ 2
+    if (n == 4) m = max(m, __builtin_amdgcn_update_dpp(m, m, 0x141, 0xF, 0xF, false));   // the other half of 8
+    return (unsigned)m;
+}
+// n codes into a register pair, lowest byte first
+template <int n> __device__ __forceinline__ void md_act8_encode(const float (&v)[n], int code, unsigned (&w)[n / 4]) {
+    const float inv = md_act8_inv(code);
+#pragma unroll
+    for (int j = 0; j < n; ++j) {
+        const unsigned q = code == MD_ACT8_NAN ? 0u : (unsigned)md_act8_round(v[j], inv) & 0xFFu;
+        w[j / 4] = j % 4 ? w[j / 4] | q << (8 * (j % 4)) : q;
+    }
+}
+template <class T> __device__ __forceinline__ void md_store_codes(signed char *row, int at, int len, const unsigned (&w)[Wide<T>::n / 4]) {
+    constexpr int n = Wide<T>::n;
+    if (at + n <= len) {
+        typename Wide<T>::Codes c;
+        __builtin_memcpy(&c, w, n);
+        *(typename Wide<T>::Codes *)(row + at) = c;
+    } else {
+#pragma unroll
+        for (int j = 0; j < n; ++j)
+            if (at + j < len) row[at + j] = (signed char)(w[j / 4] >> (8 * (j % 4)));
+    }
+}
+template <class T> __device__ __forceinline__ void md_load_codes(const signed char *row, int at, int len, float scale, float (&v)[Wide<T>::n]) {
+    constexpr int n = Wide<T>::n;
+    unsigned w[n / 4];
+    if (at + n <= len) {
+        const typename Wide<T>::Codes c = *(const typename Wide<T>::Codes *)(row + at);
+        __builtin_memcpy(w, &c, n);
+    } else {
+#pragma unroll
+        for (int j = 0; j < n; ++j) {
+            const unsigned q = at + j < len ? (unsigned)(unsigned char)row[at + j] : 0u;
+            w[j / 4] = j % 4 ? w[j / 4] | q << (8 * (j % 4)) : q;
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < n; ++j) v[j] = (float)(signed char)(w[j / 4] >> (8 * (j % 4))) * scale;
+}

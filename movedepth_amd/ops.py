@@ -4,6 +4,7 @@ PyTorch is plumbing here: it owns device memory, the current HIP stream and auto
 forward/backward below is one or two launches of a hand-written gfx950 kernel.  No CPU fallback exists:
 tensors must live on the GPU and the HIP library must load, otherwise these raise.
 """
+import contextlib
 import ctypes
 
 import torch
@@ -1478,9 +1479,21 @@ def _wants_grad(*tensors):
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
+_NO_GUARD = contextlib.nullcontext()
+
+
+def _on(device):
+    """context in which launches go to `device`; nothing to enter (and nothing to pay for) where it is current already"""
+    return _NO_GUARD if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
 def _stream_of(device):
-    """raw current stream of the tensors' own device (which need not be the current device: callers hold torch.cuda.device(device))"""
-    return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+    """raw current stream of the tensors' own device"""
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+def _at(t):
+    return None if t is None else t.data_ptr()
 
 
 # --------------------------------------------------------------------------- 8-bit activation checkpoints
@@ -1513,23 +1526,23 @@ def act8_pack(x):
     step: 2^-7 of the group's largest magnitude (at the far end of the type's range, where that power would overflow, up to one part in
     128 of the value).  32 neighbours that hold an infinity or a NaN come back as NaN.  No gradient."""
     _token_check(x, "x", "act8_pack")
-    with torch.no_grad(), torch.cuda.device(x.device):
+    with torch.no_grad(), _on(x.device):
         x = x.detach()
         if not _is_dense(x):
             x = x.contiguous()
         n = x.numel()
         codes = torch.empty(n, device=x.device, dtype=torch.int8)
         scales = torch.empty((n + 31) // 32, device=x.device, dtype=torch.int8)
-        _timed_call("md_act8_pack", _p(x), _TOKEN_DTYPE[x.dtype], n, _p(codes), _p(scales), _stream_of(x.device))
+        _timed_call("md_act8_pack", _at(x), _TOKEN_DTYPE[x.dtype], n, _at(codes), _at(scales), _stream_of(x.device))
     return Act8(codes, scales, x.shape, x.stride(), x.dtype)
 
 
 def act8_unpack(packed):
     """Act8 -> tensor of the packed one's shape, strides and type (exact: the stored values are representable in it)."""
     dev = packed.codes.device
-    with torch.cuda.device(dev):
+    with _on(dev):
         x = torch.empty_strided(packed.shape, packed.stride, device=dev, dtype=packed.dtype)
-        _timed_call("md_act8_unpack", _p(packed.codes), _p(packed.scales), _TOKEN_DTYPE[packed.dtype], x.numel(), _p(x), _stream_of(dev))
+        _timed_call("md_act8_unpack", _at(packed.codes), _at(packed.scales), _TOKEN_DTYPE[packed.dtype], x.numel(), _at(x), _stream_of(dev))
     return x
 
 
@@ -1559,26 +1572,32 @@ def _rows(t, C):
     return t, (t.stride(0) if t.shape[0] > 1 else C)
 
 
+def _layer_norm_fwd(x, weight, bias, eps, act_bits, keep):
+    """-> y and, with `keep`, what the backward pass reads: (x as rows or None, codes, scales, statistics, weight in float32)"""
+    C, dev = x.shape[-1], x.device
+    w = None if weight is None else _f32c(weight)
+    b = None if bias is None else _f32c(bias)
+    with _on(dev):
+        x2, ldx = _rows(x, C)
+        rows = x2.shape[0]
+        y = torch.empty(x.shape, device=dev, dtype=x.dtype)
+        stat = codes = scales = None
+        if keep:
+            stat = torch.empty(rows, 2, device=dev, dtype=torch.float32)
+            if act_bits:
+                codes = torch.empty(rows, C, device=dev, dtype=torch.int8)
+                scales = torch.empty(rows, (C + 31) // 32, device=dev, dtype=torch.int8)
+        _timed_call("md_layer_norm_fwd", x2.data_ptr(), _TOKEN_DTYPE[x.dtype], rows, C, ldx, _at(w), _at(b), eps, y.data_ptr(), _at(stat), _at(codes),
+                    _at(scales), _stream_of(dev))
+    return y, (None if codes is not None else x2, codes, scales, stat, w)
+
+
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, eps, act_bits, keep):
-        C = x.shape[-1]
-        w = None if weight is None else _f32c(weight)
-        b = None if bias is None else _f32c(bias)
-        with torch.cuda.device(x.device):
-            x2, ldx = _rows(x, C)
-            rows = x2.shape[0]
-            y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
-            stat = torch.empty(rows, 2, device=x.device, dtype=torch.float32) if keep else None
-            codes = scales = None
-            if keep and act_bits:
-                codes = torch.empty(rows, C, device=x.device, dtype=torch.int8)
-                scales = torch.empty(rows, (C + 31) // 32, device=x.device, dtype=torch.int8)
-            _timed_call("md_layer_norm_fwd", _p(x2), _TOKEN_DTYPE[x.dtype], rows, C, ldx, _p(w), _p(b), eps, _p(y), _p(stat), _p(codes),
-                        _p(scales), _stream_of(x.device))
-        if keep:
-            ctx.save_for_backward(None if codes is not None else x2, codes, scales, stat, w)
-            ctx.dtype, ctx.wdtype, ctx.bdtype = x.dtype, None if weight is None else weight.dtype, None if bias is None else bias.dtype
+    def forward(ctx, x, weight, bias, eps, act_bits):
+        y, kept = _layer_norm_fwd(x, weight, bias, eps, act_bits, True)
+        ctx.save_for_backward(*kept)
+        ctx.dtype, ctx.wdtype, ctx.bdtype = x.dtype, None if weight is None else weight.dtype, None if bias is None else bias.dtype
         return y
 
     @staticmethod
@@ -1586,7 +1605,7 @@ class _LayerNorm(torch.autograd.Function):
     def backward(ctx, gy):
         x2, codes, scales, stat, w = ctx.saved_tensors
         C, dev = gy.shape[-1], gy.device
-        with torch.cuda.device(dev):
+        with _on(dev):
             g, ldg = _rows(gy.to(ctx.dtype), C)
             rows = g.shape[0]
             ldx = C if x2 is None or rows <= 1 else x2.stride(0)
@@ -1595,9 +1614,9 @@ class _LayerNorm(torch.autograd.Function):
             dwb = torch.empty(2, C, device=dev, dtype=torch.float32) if need_w or need_b else None
             nbytes = 0 if dwb is None else _lib.load().md_layer_norm_bwd_ws_bytes(rows, C)
             ws = _ws(nbytes, dev) if nbytes else None
-            _timed_call("md_layer_norm_bwd", _p(g), ldg, _p(x2), ldx, _p(codes), _p(scales), _TOKEN_DTYPE[ctx.dtype], _p(stat), _p(w), rows, C,
-                        _p(dx), _p(dwb[0]) if need_w else None, _p(dwb[1]) if need_b else None, _p(ws), nbytes, _stream_of(dev))
-        return dx, dwb[0].to(ctx.wdtype) if need_w else None, dwb[1].to(ctx.bdtype) if need_b else None, None, None, None
+            _timed_call("md_layer_norm_bwd", _at(g), ldg, _at(x2), ldx, _at(codes), _at(scales), _TOKEN_DTYPE[ctx.dtype], _at(stat), _at(w), rows, C,
+                        _at(dx), _at(dwb[0]) if need_w else None, _at(dwb[1]) if need_b else None, _at(ws), nbytes, _stream_of(dev))
+        return dx, dwb[0].to(ctx.wdtype) if need_w else None, dwb[1].to(ctx.bdtype) if need_b else None, None, None
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5, act_bits=0):
@@ -1615,7 +1634,9 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, act_bits=0):
         raise _lib.MovedepthHipError("layer_norm: act_bits = %r (0 or 8)" % (act_bits,))
     if not eps >= 0:
         raise _lib.MovedepthHipError("layer_norm: eps = %r" % (eps,))
-    return _LayerNorm.apply(x, weight, bias, float(eps), int(act_bits), _wants_grad(x, weight, bias))
+    if not _wants_grad(x, weight, bias):
+        return _layer_norm_fwd(x, weight, bias, float(eps), 0, False)[0]
+    return _LayerNorm.apply(x, weight, bias, float(eps), int(act_bits))
 
 
 # --------------------------------------------------------------------------- attention to another sequence's tokens
@@ -1638,24 +1659,29 @@ def _attn_desc(q, k, v, key_mask, scale):
     return a
 
 
+def _cross_attention_fwd(q, k, v, key_mask, scale, keep):
+    """-> o and, with `keep`, what the backward pass reads"""
+    dev = q.device
+    with _on(dev):
+        (q, _), (k, _), (v, _) = _attn_strides(q), _attn_strides(k), _attn_strides(v)
+        if key_mask is not None and key_mask.shape[1] > 1 and key_mask.stride(1) != 1:
+            key_mask = key_mask.contiguous()
+        a = _attn_desc(q, k, v, key_mask, scale)
+        o = torch.empty(q.shape, device=dev, dtype=q.dtype)
+        lse = torch.empty(a.B, a.Hq, a.Nq, device=dev, dtype=torch.float32) if keep else None
+        a.o, a.lse = o.data_ptr(), _at(lse)
+        nbytes = _lib.load().md_cross_attn_ws_bytes(ctypes.byref(a), 0)
+        ws = _ws(nbytes, dev) if nbytes else None
+        _timed_call("md_cross_attn_fwd", ctypes.byref(a), _at(ws), nbytes, _stream_of(dev))
+    return o, (q, k, v, key_mask, o, lse)
+
+
 class _CrossAttention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, key_mask, scale, keep):
-        dev = q.device
-        with torch.cuda.device(dev):
-            (q, _), (k, _), (v, _) = _attn_strides(q), _attn_strides(k), _attn_strides(v)
-            if key_mask is not None and key_mask.shape[1] > 1 and key_mask.stride(1) != 1:
-                key_mask = key_mask.contiguous()
-            a = _attn_desc(q, k, v, key_mask, scale)
-            o = torch.empty(q.shape, device=dev, dtype=q.dtype)
-            lse = torch.empty(a.B, a.Hq, a.Nq, device=dev, dtype=torch.float32) if keep else None
-            a.o, a.lse = o.data_ptr(), None if lse is None else lse.data_ptr()
-            nbytes = _lib.load().md_cross_attn_ws_bytes(ctypes.byref(a), 0)
-            ws = _ws(nbytes, dev) if nbytes else None
-            _timed_call("md_cross_attn_fwd", ctypes.byref(a), _p(ws), nbytes, _stream_of(dev))
-        if keep:
-            ctx.save_for_backward(q, k, v, key_mask, o, lse)
-            ctx.scale = scale
+    def forward(ctx, q, k, v, key_mask, scale):
+        o, kept = _cross_attention_fwd(q, k, v, key_mask, scale, True)
+        ctx.save_for_backward(*kept)
+        ctx.scale = scale
         return o
 
     @staticmethod
@@ -1663,7 +1689,7 @@ class _CrossAttention(torch.autograd.Function):
     def backward(ctx, g):
         q, k, v, key_mask, o, lse = ctx.saved_tensors
         dev = q.device
-        with torch.cuda.device(dev):
+        with _on(dev):
             g, gs = _attn_strides(g.to(q.dtype))
             o = o.contiguous()
             a = _attn_desc(q, k, v, key_mask, ctx.scale)
@@ -1673,11 +1699,11 @@ class _CrossAttention(torch.autograd.Function):
             both = ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
             dk = torch.empty(k.shape, device=dev, dtype=k.dtype) if both else None
             dv = torch.empty(v.shape, device=dev, dtype=v.dtype) if both else None
-            a.dq, a.dk, a.dv = (None if t is None else t.data_ptr() for t in (dq, dk, dv))
+            a.dq, a.dk, a.dv = _at(dq), _at(dk), _at(dv)
             nbytes = _lib.load().md_cross_attn_ws_bytes(ctypes.byref(a), 1)
             ws = _ws(nbytes, dev) if nbytes else None
-            _timed_call("md_cross_attn_bwd", ctypes.byref(a), _p(ws), nbytes, _stream_of(dev))
-        return dq, dk if ctx.needs_input_grad[1] else None, dv if ctx.needs_input_grad[2] else None, None, None, None
+            _timed_call("md_cross_attn_bwd", ctypes.byref(a), _at(ws), nbytes, _stream_of(dev))
+        return dq, dk if ctx.needs_input_grad[1] else None, dv if ctx.needs_input_grad[2] else None, None, None
 
 
 def cross_attention(q, k, v, key_mask=None, scale=None):
@@ -1701,4 +1727,7 @@ def cross_attention(q, k, v, key_mask=None, scale=None):
     if key_mask is not None and (key_mask.dtype != torch.bool or key_mask.device != q.device or tuple(key_mask.shape) != (B, k.shape[1])):
         raise _lib.MovedepthHipError("cross_attention: key_mask %s %s on %s (bool (%d, %d) on %s: True where a key takes part)"
                                      % (key_mask.dtype, tuple(key_mask.shape), key_mask.device, B, k.shape[1], q.device))
-    return _CrossAttention.apply(q, k, v, key_mask, float(d ** -0.5 if scale is None else scale), _wants_grad(q, k, v))
+    scale = float(d ** -0.5 if scale is None else scale)
+    if not _wants_grad(q, k, v):
+        return _cross_attention_fwd(q, k, v, key_mask, scale, False)[0]
+    return _CrossAttention.apply(q, k, v, key_mask, scale)
