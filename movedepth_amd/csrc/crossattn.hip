@@ -22,6 +22,8 @@
 // magnitudes matter to 2^-24, which is 6 / 16 of what the float32 matrix instruction costs.  2-byte types: P and dS are rounded to
 // the type before their products (half a step relative).  float16 holds P times 2^7 (forward) or 2^15 (backward) and dS times a power
 // of two from the largest |g| |v|, so that the small weights of long rows do not fall below its range.
+#include <algorithm>
+
 #include "md_types.hpp"
 
 namespace {
@@ -90,6 +92,14 @@ __device__ __forceinline__ int die_order(int block, int blocks) {
     const int per = (blocks + 7) / 8;
     return (block % 8) * per + block / 8;
 }
+
+// Workgroups of 4 waves that a CU holds at once (registers, and shared memory where it is short), per kernel; also what the compiler is asked to keep to.
+template <int NP, int KS, int QT> constexpr int fwd_per_cu() { return NP == 3 ? (KS <= 4 ? 3 : KS == 6 ? 2 : 1) : QT == 2 ? 2 : KS <= 2 ? 4 : KS == 4 ? 3 : 2; }
+template <int NP, int KS, int QT> constexpr int dq_per_cu() { return NP == 3 ? (KS <= 2 ? 3 : KS == 4 ? 2 : 1) : QT == 2 ? 2 : KS <= 2 ? 4 : KS == 4 ? 3 : 2; }
+template <int NP, int KS> constexpr int dkv_per_cu() { return NP == 3 ? (KS == 1 ? 4 : KS == 2 ? 3 : 1) : KS <= 2 ? 4 : KS == 4 ? 3 : 2; }
+// query tiles per wave: two read every key fragment once for both (heads of 64: 371 us against 386 in the forward pass of 2 x 16 heads x 4096 x 8192), but
+// hold the registers of two, which the smaller heads use better for more waves (heads of 32, 2 x 2 x 20480 x 20480: 430 us against 406)
+template <int NP, int KS> constexpr int query_tiles() { return NP == 1 && KS == 4 ? 2 : 1; }
 
 // ---------------------------------------------------------------- what the kernels are told
 struct Shape {
@@ -273,36 +283,196 @@ __global__ __launch_bounds__(64) void xa_pack_kernel(PackArgs a) {
 
 __global__ void xa_clear_kernel(unsigned *p) { p[threadIdx.x] = 0u; }
 
-// ---------------------------------------------------------------- forward, tiles of 32 queries per wave and step of TK keys
+// ---------------------------------------------------------------- accumulators to memory
+// A lane holds 4 neighbouring dims of its row in each 4 registers: one 8- or 16-byte store where the rows allow it.
+template <class T, int DB> __device__ __forceinline__ void store_row(T *row, int d, int half, const f32x16 (&x)[DB], float f) {
+#pragma unroll
+    for (int b = 0; b < DB; ++b)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int dim = 32 * b + 8 * g + 4 * half;
+            T v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = (T)(x[b][4 * g + e] * f);
+            if (d % 4 == 0) {
+                if (dim < d) __builtin_memcpy(__builtin_assume_aligned(row + dim, 4 * sizeof(T)), v, 4 * sizeof(T));
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (dim + e < d) row[dim + e] = v[e];
+            }
+        }
+}
+// a part of 32 rows, as it stands in the registers: [b][g][lane][4 floats], 1 KB each
+using f32x4 = float __attribute__((ext_vector_type(4)));
+template <int DB> __device__ __forceinline__ void store_part(float *to, int lane, const f32x16 (&x)[DB], float f) {
+#pragma unroll
+    for (int b = 0; b < DB; ++b)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            f32x4 v;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = x[b][4 * g + e] * f;
+            *(f32x4 *)(to + ((b * 4 + g) * 64 + lane) * 4) = v;
+        }
+}
+template <int DB> __device__ __forceinline__ void add_part(const float *from, int lane, f32x16 (&x)[DB], float f) {
+#pragma unroll
+    for (int b = 0; b < DB; ++b)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const f32x4 v = *(const f32x4 *)(from + ((b * 4 + g) * 64 + lane) * 4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[b][4 * g + e] = fmaf(f, v[e], x[b][4 * g + e]);
+        }
+}
+
+// ---------------------------------------------------------------- the tile kernels' share of the work
+// The work of a launch is a line of units: blocks of rows (`rows` query rows, or keys in the dk / dv kernel) of each z, one behind the other, and of each
+// block the steps over the other axis.  Every worker (workgroup) takes an equal stretch of it, so the chip is filled evenly whatever the
+// sizes.  A block that lies within one stretch is written at once; of the others each worker leaves its part in a slot (at most two: its
+// first block and its last) and xa_join / xa_sum put the parts together in the order of the line: the same bits every time.
 struct TileArgs {
     Shape s;
     const char *Qr, *Kr, *Vt;                          // forward
     const char *Qt, *Kt, *Vr, *Gr, *Gt, *stat;         // backward
-    int q_tiles, k_tiles, blocks, splits;
+    int q_tiles, k_tiles, workers, rows, step;          // `step`: keys per step; 0: blocks are of keys, a step is a tile of 32 queries
+    long long units;                                    // all of them; with a mask the device counts
     float c, scale;
     void *o, *dq, *dk, *dv;
-    float *lse, *part, *part2, *ml;                      // partial results of a split launch: [split][z][row][d], [split][z][row][2]
+    int4 *first;                                         // each worker's first piece: z (-1: idle), block, step -- for who joins the parts
+    float *lse, *part, *part2, *ml;                      // parts: [slot][tile of the block][store_part], [slot][row of the block][2]
     const unsigned *amax;
+};
+
+struct Line {                                          // of one sequence: blocks of a z, steps of a block
+    int blocks, steps;
+    __device__ long long units(int Hk) const { return (long long)Hk * blocks * steps; }
+};
+__device__ __forceinline__ Line line_of(const TileArgs &a, int b) {
+    const int n = a.s.cnt ? a.s.cnt[b] : a.s.N;
+    Line l;
+    l.blocks = ((a.step ? a.s.M : n) + a.rows - 1) / a.rows;
+    l.steps = max(1, a.step ? (n + a.step - 1) / a.step : a.q_tiles);     // (a block without steps is still written)
+    return l;
+}
+__device__ __forceinline__ long long uniform(long long v) {
+    return (long long)((unsigned long long)(unsigned)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32 | (unsigned)__builtin_amdgcn_readfirstlane((int)v));
+}
+// all units, and those ahead of sequence `b`; every lane of a wave calls it
+__device__ __forceinline__ long long units_before(const TileArgs &a, int b, long long &all) {
+    if (!a.s.cnt) {
+        all = a.units;
+        return line_of(a, 0).units(a.s.Hk) * b;
+    }
+    const int lane = threadIdx.x & 63;
+    long long before = 0, sum = 0;
+    for (int b0 = 0; b0 < a.s.B; b0 += 64) {
+        const long long mine = b0 + lane < a.s.B ? line_of(a, b0 + lane).units(a.s.Hk) : 0;
+        long long x = mine, y = b0 + lane < b ? mine : 0;
+#pragma unroll
+        for (int o = 32; o; o >>= 1) {
+            x += __shfl_xor(x, o);
+            y += __shfl_xor(y, o);
+        }
+        sum += x;
+        before += y;
+    }
+    all = uniform(sum);
+    return uniform(before);
+}
+// a / b of non-negative numbers, in 32 bits where they fit (64-bit division is ~100 instructions)
+__device__ __forceinline__ long long quotient(long long a, long long b) {
+    return ((a | b) >> 32) == 0 ? (long long)((unsigned)a / (unsigned)b) : a / b;
+}
+__device__ __forceinline__ long long stretch_start(long long all, int worker, int workers) {     // all * worker / workers
+    const long long q = quotient(all, workers);
+    return q * worker + quotient((all - q * workers) * worker, workers);
+}
+
+struct Piece { int z, block, first, last, slot; bool whole; };
+struct Walk {
+    long long left;
+    int b, hk, block, first, slot, part;
+    Line line;
+    __device__ __forceinline__ Walk(const TileArgs &a, int worker) {
+        long long all;
+        units_before(a, 0, all);
+        const int workers = (int)min((long long)a.workers, all);      // (a mask may leave fewer units than workers: the others are idle)
+        long long at = 0;
+        left = 0;
+        if (worker < workers) {
+            at = stretch_start(all, worker, workers);
+            left = stretch_start(all, worker + 1, workers) - at;
+        }
+        b = hk = block = first = 0;
+        line = {};
+        if (left > 0) {
+            if (!a.s.cnt) {
+                line = line_of(a, 0);
+                const long long per = line.units(a.s.Hk);
+                b = (int)quotient(at, per);
+                at -= per * b;
+            } else
+                for (line = line_of(a, 0); at >= line.units(a.s.Hk); line = line_of(a, b)) {
+                    at -= line.units(a.s.Hk);
+                    ++b;
+                }
+            const long long per = (long long)line.blocks * line.steps;
+            hk = (int)quotient(at, per);
+            at -= hk * per;
+            block = (int)quotient(at, line.steps);
+            first = (int)(at - (long long)block * line.steps);
+        }
+        // the same in every lane: scalar registers
+        left = uniform(left);
+        b = __builtin_amdgcn_readfirstlane(b), hk = __builtin_amdgcn_readfirstlane(hk), block = __builtin_amdgcn_readfirstlane(block);
+        first = __builtin_amdgcn_readfirstlane(first);
+        line.blocks = __builtin_amdgcn_readfirstlane(line.blocks), line.steps = __builtin_amdgcn_readfirstlane(line.steps);
+        slot = 2 * worker;
+        part = 0;
+        if (a.first && threadIdx.x == 0) a.first[worker] = make_int4(left > 0 ? b * a.s.Hk + hk : -1, block, first, 0);
+    }
+    __device__ __forceinline__ bool next(const TileArgs &a, Piece &p) {
+        if (left <= 0) return false;
+        p.z = b * a.s.Hk + hk, p.block = block, p.first = first;
+        p.last = (int)min((long long)line.steps, first + left);
+        p.whole = p.last - p.first == line.steps;
+        p.slot = slot + (part ? 1 : 0);
+        part = 1;
+        left -= p.last - p.first;
+        first = 0;
+        if (++block == line.blocks) {
+            block = 0;
+            if (++hk == a.s.Hk) {
+                hk = 0;
+                if (left > 0)
+                    do line = line_of(a, ++b);
+                    while (!line.blocks);
+            }
+        }
+        return true;
+    }
 };
 
 template <class E> struct Shift { static constexpr float fwd = 0.f, bwd = 0.f; };
 template <> struct Shift<f16_t> { static constexpr float fwd = 7.f, bwd = 15.f; };
 
-template <class T, int KS, int QT, int TK>
-__global__ __launch_bounds__(256, 2) void xa_fwd_kernel(TileArgs a) {
+// ---------------------------------------------------------------- forward: 32 QT queries per wave, NW waves, steps of TK keys
+template <class T, int KS, int QT, int TK, int NW>
+__global__ __launch_bounds__(64 * NW, (NW == 4 ? fwd_per_cu<Frag<T>::NP, KS, QT>() : 1)) void xa_fwd_kernel(TileArgs a) {
     using E = typename Frag<T>::E;
     using v8 = typename Vec<E>::v8;
     constexpr int NP = Frag<T>::NP, DB = (KS + 1) / 2, SUB = TK / 32;
     constexpr int KC = SUB * KS * NP, VC = SUB * DB * 2 * NP;       // 1 KB chunks per step
     __shared__ __attribute__((aligned(1024))) char lds[2][(KC + VC) * 1024];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, half = lane >> 5;
-    const int work = die_order(blockIdx.x, gridDim.x);
-    if (work >= a.blocks) return;
-    const int q_blocks = (a.q_tiles + 4 * QT - 1) / (4 * QT);
-    const int split = work % a.splits, qb = work / a.splits % q_blocks, z = work / a.splits / q_blocks;
-    const int n = keys_of(a.s, z), steps = (n + TK - 1) / TK;
-    const int first = (int)((long long)steps * split / a.splits), last = (int)((long long)steps * (split + 1) / a.splits);
-    const int q0 = (qb * 4 + wave) * QT;                // this wave's first query tile
+    const int worker = die_order(blockIdx.x, gridDim.x);
+    if (worker >= a.workers) return;
+    Piece w;
+    for (Walk walk(a, worker); walk.next(a, w);) {
+    const int z = w.z, n = keys_of(a.s, z), last = min(w.last, (n + TK - 1) / TK);
+    const int q0 = (w.block * NW + wave) * QT;          // this wave's first query tile
 
     v8 q[QT][KS][NP];
     f32x16 o[QT][DB];
@@ -320,11 +490,12 @@ __global__ __launch_bounds__(256, 2) void xa_fwd_kernel(TileArgs a) {
     const char *Kz = a.Kr + (long long)z * a.k_tiles * KS * NP * 1024, *Vz = a.Vt + (long long)z * a.k_tiles * DB * 2 * NP * 1024;
     auto fetch = [&](int step) {
         char *to = lds[step & 1];
-        for (int i = wave; i < KC + VC; i += 4)
+        for (int i = wave; i < KC + VC; i += NW)
             load_chunk(i < KC ? Kz + ((long long)step * KC + i) * 1024 : Vz + ((long long)step * VC + i - KC) * 1024, to + i * 1024, lane);
     };
-    if (first < last) fetch(first);
-    for (int step = first; step < last; ++step) {
+    __syncthreads();                                   // the last piece's tiles have been read
+    if (w.first < last) fetch(w.first);
+    for (int step = w.first; step < last; ++step) {
         wait_loads_and_barrier();
         if (step + 1 < last) fetch(step + 1);
         const char *K = lds[step & 1], *V = K + KC * 1024;
@@ -386,52 +557,178 @@ __global__ __launch_bounds__(256, 2) void xa_fwd_kernel(TileArgs a) {
     for (int t = 0; t < QT; ++t) {
         const int row = (q0 + t) * 32 + col;
         const float sum = swap_halves_sum(l[t]), base = m[t] - Shift<E>::fwd;
-        if (row >= a.s.M) continue;
-        const long long zr = (long long)z * a.s.M + row;
-        if (a.splits > 1) {
-            const long long at = (long long)split * a.s.B * a.s.Hk * a.s.M + zr;
+        if (!w.whole) {
+            const long long tile = (long long)w.slot * (NW * QT) + wave * QT + t;
             if (half == 0) {
-                a.ml[2 * at] = base;
-                a.ml[2 * at + 1] = sum;
+                a.ml[2 * (tile * 32 + col)] = base;
+                a.ml[2 * (tile * 32 + col) + 1] = sum;
             }
-#pragma unroll
-            for (int b = 0; b < DB; ++b)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int dim = 32 * b + 8 * (r / 4) + 4 * half + r % 4;
-                    if (dim < a.s.d) a.part[at * a.s.d + dim] = o[t][b][r];
-                }
-        } else {
+            store_part<DB>(a.part + tile * DB * 1024, lane, o[t], 1.f);
+        } else if (row < a.s.M) {
             const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);     // (NaN stays NaN)
-            if (half == 0 && a.lse) a.lse[zr] = sum == 0.f ? INFINITY : base + __log2f(sum);
-            T *to = (T *)a.o + q_row(a.s, z, row) * a.s.d;
+            if (half == 0 && a.lse) a.lse[(long long)z * a.s.M + row] = sum == 0.f ? INFINITY : base + __log2f(sum);
+            store_row<T, DB>((T *)a.o + q_row(a.s, z, row) * a.s.d, a.s.d, half, o[t], inv);
+        }
+    }
+    }
+}
+
+// The block that the start of stretch `worker` falls into, and who has parts of it: workers `from` .. `to` - 1, from what each worker noted of its first piece.
+// Found once, by the first worker that starts inside the block: for the others find() is false.
+struct Joint {
+    int z, block, from, to;
+    bool tail;                   // `from` has a piece ahead of this one: its part is in its second slot
+    __device__ __forceinline__ bool find(const TileArgs &a, int worker) {
+        const int4 me = a.first[worker];
+        if (worker == 0 || me.x < 0 || me.z == 0) return false;        // idle, or it starts with a block of its own
+        const int4 last = a.first[worker - 1];
+        const bool same = last.x == me.x && last.y == me.y;
+        if (same && last.z > 0) return false;
+        z = me.x, block = me.y, from = worker - 1, tail = !same;
+        for (to = worker + 1; to < a.workers; ++to) {
+            const int4 next = a.first[to];
+            if (next.x != z || next.y != block || next.z == 0) break;
+        }
+        return true;
+    }
+    __device__ __forceinline__ int slot(int i) const { return 2 * i + (tail && i == from ? 1 : 0); }
+};
+
+// The four waves of a workgroup add up one tile's parts, each every fourth of them, in their order; then wave g holds registers 4 g .. 4 g + 3 of each b.
+template <int DB> __device__ __forceinline__ void sum_waves(float *shared, int wave, int lane, const f32x16 (&x)[DB], const float (&f)[4], f32x4 (&out)[DB]) {
 #pragma unroll
-            for (int b = 0; b < DB; ++b)
+    for (int b = 0; b < DB; ++b) {
+        __syncthreads();
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int dim = 32 * b + 8 * (r / 4) + 4 * half + r % 4;
-                    if (dim < a.s.d) to[dim] = (T)(o[t][b][r] * inv);
-                }
+        for (int g = 0; g < 4; ++g) {
+            f32x4 v;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = x[b][4 * g + e];
+            *(f32x4 *)(shared + ((wave * 4 + g) * 64 + lane) * 4) = v;
+        }
+        __syncthreads();
+        out[b] = (f32x4)0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) out[b] += *(const f32x4 *)(shared + ((i * 4 + wave) * 64 + lane) * 4) * f[i];
+    }
+}
+template <class T, int DB> __device__ __forceinline__ void store_quarter(T *row, int d, int half, int g, const f32x4 (&x)[DB], float f) {
+#pragma unroll
+    for (int b = 0; b < DB; ++b) {
+        const int dim = 32 * b + 8 * g + 4 * half;
+        T v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = (T)(x[b][e] * f);
+        if (d % 4 == 0) {
+            if (dim < d) __builtin_memcpy(__builtin_assume_aligned(row + dim, 4 * sizeof(T)), v, 4 * sizeof(T));
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (dim + e < d) row[dim + e] = v[e];
         }
     }
 }
 
-// the splits of one row joined: O = sum 2^(m_i - m) O_i / sum 2^(m_i - m) l_i, m = max m_i
+// O = sum 2^(m_i - m) O_i / sum 2^(m_i - m) l_i, m = max m_i; a workgroup per tile of 32 rows
+template <class T, int DB>
+__global__ __launch_bounds__(256) void xa_join_kernel(TileArgs a) {
+    __shared__ float shared[4096], sm[4][2][32];
+    Joint j;
+    if (!j.find(a, blockIdx.x)) return;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, half = lane >> 5;
+    const int tiles = a.rows / 32, row = j.block * a.rows + blockIdx.y * 32 + col;
+    f32x16 o[DB];
+#pragma unroll
+    for (int b = 0; b < DB; ++b) o[b] = (f32x16)0.f;
+    float m = -INFINITY, sum = 0.f;
+    for (int i = j.from + wave; i < j.to; i += 4) {
+        const long long tile = (long long)j.slot(i) * tiles + blockIdx.y;
+        const float mi = a.ml[2 * (tile * 32 + col)], li = a.ml[2 * (tile * 32 + col) + 1];
+        const float up = fmaxf(m, mi), f = m == -INFINITY ? 0.f : exp2f(m - up), fi = li == 0.f ? 0.f : exp2f(mi - up);     // (0: no keys there)
+        m = up;
+        sum = sum * f + li * fi;
+        if (__any(f != 1.f))
+#pragma unroll
+            for (int b = 0; b < DB; ++b) o[b] *= f;
+        add_part<DB>(a.part + tile * DB * 1024, lane, o, fi);
+    }
+    if (half == 0) sm[wave][0][col] = m, sm[wave][1][col] = sum;
+    __syncthreads();
+    float f[4], top = -INFINITY, total = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) top = fmaxf(top, sm[i][0][col]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        f[i] = sm[i][1][col] == 0.f ? 0.f : exp2f(sm[i][0][col] - top);
+        total = fmaf(f[i], sm[i][1][col], total);
+    }
+    f32x4 out[DB];
+    sum_waves<DB>(shared, wave, lane, o, f, out);
+    if (row >= a.s.M) return;
+    store_quarter<T, DB>((T *)a.o + q_row(a.s, j.z, row) * a.s.d, a.s.d, half, wave, out, total == 0.f ? 0.f : 1.f / total);
+    if (threadIdx.x < 32 && a.lse) a.lse[(long long)j.z * a.s.M + row] = total == 0.f ? INFINITY : top + log2f(total);
+}
+
+// dq, or dk and dv: the parts' sums
+template <class T, int DB>
+__global__ __launch_bounds__(256) void xa_sum_kernel(TileArgs a) {
+    __shared__ float shared[4096];
+    Joint j;
+    if (!j.find(a, blockIdx.x)) return;
+    const bool keys = a.step == 0;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, half = lane >> 5;
+    const int tiles = a.rows / 32, row = j.block * a.rows + blockIdx.y * 32 + col;
+    const bool live = row < (keys ? keys_of(a.s, j.z) : a.s.M);
+    const long long to = live ? (keys ? k_row(a.s, j.z, row) : q_row(a.s, j.z, row)) * a.s.d : 0;
+    const float one[4] = {1.f, 1.f, 1.f, 1.f};
+    for (int which = 0; which < (keys ? 2 : 1); ++which) {
+        f32x16 x[DB];
+#pragma unroll
+        for (int b = 0; b < DB; ++b) x[b] = (f32x16)0.f;
+        for (int i = j.from + wave; i < j.to; i += 4)
+            add_part<DB>((which ? a.part2 : a.part) + ((long long)j.slot(i) * tiles + blockIdx.y) * DB * 1024, lane, x, 1.f);
+        f32x4 out[DB];
+        sum_waves<DB>(shared, wave, lane, x, one, out);
+        if (live) store_quarter<T, DB>((T *)(which ? a.dv : keys ? a.dk : a.dq) + to, a.s.d, half, wave, out, 1.f);
+    }
+}
+
+// the splits of a few rows (xa_few): [split][z][row][d]
+struct FewArgs {
+    Shape s;
+    const void *q, *k, *v;
+    long long q_sb, q_sn, q_sh, k_sb, k_sn, k_sh, v_sb, v_sn, v_sh, mask_sb;
+    const unsigned char *mask;
+    int splits;
+    float c;
+    void *o;
+    float *lse, *part, *ml;
+};
 template <class T>
-__global__ __launch_bounds__(64) void xa_join_kernel(TileArgs a) {
+__global__ __launch_bounds__(64) void xa_few_join_kernel(FewArgs a) {
     const int lane = threadIdx.x, z = blockIdx.x / a.s.M, row = blockIdx.x % a.s.M;
     const long long rows = (long long)a.s.B * a.s.Hk * a.s.M, at = blockIdx.x;
-    float m = -INFINITY;
-    for (int i = 0; i < a.splits; ++i) m = fmaxf(m, a.ml[2 * (i * rows + at)]);
-    float sum = 0.f, o0 = 0.f, o1 = 0.f;
-    for (int i = 0; i < a.splits; ++i) {
-        const float mi = a.ml[2 * (i * rows + at)], li = a.ml[2 * (i * rows + at) + 1];
-        if (li == 0.f) continue;                       // no keys there
-        const float f = exp2f(mi - m);
-        sum = fmaf(f, li, sum);
-        const float *p = a.part + (i * rows + at) * a.s.d;
-        if (lane < a.s.d) o0 = fmaf(f, p[lane], o0);
-        if (lane + 64 < a.s.d) o1 = fmaf(f, p[lane + 64], o1);
+    // a lane holds one split's m and l (there are at most 64), then the weights go round
+    const bool on = lane < a.splits;
+    const float mi = on ? a.ml[2 * (lane * rows + at)] : -INFINITY, li = on ? a.ml[2 * (lane * rows + at) + 1] : 0.f;
+    const float m = md_wave_max(mi), f = li == 0.f ? 0.f : exp2f(mi - m);
+    const float sum = md_wave_sum(f * li);
+    float o0 = 0.f, o1 = 0.f;
+    constexpr int U = 8;           // parts in flight
+    for (int i0 = 0; i0 < a.splits; i0 += U) {
+        float x0[U], x1[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = i0 + u < a.splits ? i0 + u : i0;
+            const float *p = a.part + (i * rows + at) * a.s.d;
+            x0[u] = lane < a.s.d ? p[lane] : 0.f;
+            x1[u] = lane + 64 < a.s.d ? p[lane + 64] : 0.f;
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const float fi = i0 + u < a.splits ? __shfl(f, i0 + u) : 0.f;
+            if (fi != 0.f) o0 = fmaf(fi, x0[u], o0), o1 = fmaf(fi, x1[u], o1);
+        }
     }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
     T *to = (T *)a.o + q_row(a.s, z, row) * a.s.d;
@@ -452,22 +749,21 @@ template <class E> __device__ __forceinline__ float ds_scale(const unsigned *ama
     return __uint_as_float((unsigned)(127 + k) << 23);
 }
 
-template <class T, int KS, int QT, int TK>
-__global__ __launch_bounds__(256, Frag<T>::NP == 3 && KS > 4 ? 1 : 2) void xa_dq_kernel(TileArgs a) {
+template <class T, int KS, int QT, int TK, int NW>
+__global__ __launch_bounds__(64 * NW, (NW == 4 ? dq_per_cu<Frag<T>::NP, KS, QT>() : 1)) void xa_dq_kernel(TileArgs a) {
     using E = typename Frag<T>::E;
     using v8 = typename Vec<E>::v8;
     constexpr int NP = Frag<T>::NP, DB = (KS + 1) / 2, SUB = TK / 32;
     constexpr int RC = SUB * KS * NP, TC = SUB * DB * 2 * NP;
     __shared__ __attribute__((aligned(1024))) char lds[2][(2 * RC + TC) * 1024];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, half = lane >> 5;
-    const int work = die_order(blockIdx.x, gridDim.x);
-    if (work >= a.blocks) return;
-    const int q_blocks = (a.q_tiles + 4 * QT - 1) / (4 * QT);
-    const int split = work % a.splits, qb = work / a.splits % q_blocks, z = work / a.splits / q_blocks;
-    const int n = keys_of(a.s, z), steps = (n + TK - 1) / TK;
-    const int first = (int)((long long)steps * split / a.splits), last = (int)((long long)steps * (split + 1) / a.splits);
-    const int q0 = (qb * 4 + wave) * QT;
+    const int worker = die_order(blockIdx.x, gridDim.x);
+    if (worker >= a.workers) return;
     const float up = ds_scale<E>(a.amax);
+    Piece w;
+    for (Walk walk(a, worker); walk.next(a, w);) {
+    const int z = w.z, n = keys_of(a.s, z), first = w.first, last = min(w.last, (n + TK - 1) / TK);
+    const int q0 = (w.block * NW + wave) * QT;
 
     v8 q[QT][KS][NP], g[QT][KS][NP];
     f32x16 dq[QT][DB];
@@ -489,11 +785,12 @@ __global__ __launch_bounds__(256, Frag<T>::NP == 3 && KS > 4 ? 1 : 2) void xa_dq
     const char *Tz = a.Kt + (long long)z * a.k_tiles * DB * 2 * NP * 1024;
     auto fetch = [&](int step) {
         char *to = lds[step & 1];
-        for (int i = wave; i < 2 * RC + TC; i += 4)
+        for (int i = wave; i < 2 * RC + TC; i += NW)
             load_chunk(i < RC ? Kz + ((long long)step * RC + i) * 1024 : i < 2 * RC ? Vz + ((long long)step * RC + i - RC) * 1024
                                                                                      : Tz + ((long long)step * TC + i - 2 * RC) * 1024,
                        to + i * 1024, lane);
     };
+    __syncthreads();                                   // the last piece's tiles have been read
     if (first < last) fetch(first);
     for (int step = first; step < last; ++step) {
         wait_loads_and_barrier();
@@ -539,19 +836,9 @@ __global__ __launch_bounds__(256, Frag<T>::NP == 3 && KS > 4 ? 1 : 2) void xa_dq
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
         const int row = (q0 + t) * 32 + col;
-        if (row >= a.s.M) continue;
-        float *part = a.part + ((long long)split * a.s.B * a.s.Hk * a.s.M + (long long)z * a.s.M + row) * a.s.d;
-        T *to = (T *)a.dq + q_row(a.s, z, row) * a.s.d;
-#pragma unroll
-        for (int b = 0; b < DB; ++b)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int dim = 32 * b + 8 * (r / 4) + 4 * half + r % 4;
-                if (dim < a.s.d) {
-                    if (a.splits > 1) part[dim] = dq[t][b][r] * back;
-                    else to[dim] = (T)(dq[t][b][r] * back);
-                }
-            }
+        if (!w.whole) store_part<DB>(a.part + ((long long)w.slot * (NW * QT) + wave * QT + t) * DB * 1024, lane, dq[t], back);
+        else if (row < a.s.M) store_row<T, DB>((T *)a.dq + q_row(a.s, z, row) * a.s.d, a.s.d, half, dq[t], back);
+    }
     }
 }
 
@@ -562,24 +849,21 @@ struct DkvLds {
     static constexpr int BUFFERS = CHUNKS <= 80 ? 2 : 1;
 };
 
-template <class T, int KS, int KT>
-__global__ __launch_bounds__(256, (Frag<T>::NP == 3 && KS > 2) || KT * KS > 8 ? 1 : 2) void xa_dkv_kernel(TileArgs a) {
+template <class T, int KS, int KT, int NW>
+__global__ __launch_bounds__(64 * NW, (NW == 4 ? dkv_per_cu<Frag<T>::NP, KS>() : 1)) void xa_dkv_kernel(TileArgs a) {
     using E = typename Frag<T>::E;
     using v8 = typename Vec<E>::v8;
     using L = DkvLds<T, KS, KT>;
     constexpr int NP = L::NP, DB = L::DB, RC = KS * NP, TC = DB * 2 * NP, NB = L::BUFFERS;
     extern __shared__ __attribute__((aligned(1024))) char lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, half = lane >> 5;
-    const int work = die_order(blockIdx.x, gridDim.x);
-    if (work >= a.blocks) return;
-    const int k_blocks = (a.k_tiles + 4 * KT - 1) / (4 * KT);
-    const int split = work % a.splits, kb = work / a.splits % k_blocks, z = work / a.splits / k_blocks;
-    const int n = keys_of(a.s, z);
-    if (kb * 4 * KT * 32 >= n) return;
-    const int steps = a.q_tiles;
-    const int first = (int)((long long)steps * split / a.splits), last = (int)((long long)steps * (split + 1) / a.splits);
-    const int k0 = (kb * 4 + wave) * KT;
+    const int worker = die_order(blockIdx.x, gridDim.x);
+    if (worker >= a.workers) return;
     const float up = ds_scale<E>(a.amax);
+    Piece w;
+    for (Walk walk(a, worker); walk.next(a, w);) {
+    const int z = w.z, n = keys_of(a.s, z), first = w.first, last = min(w.last, a.q_tiles);
+    const int k0 = (w.block * NW + wave) * KT;
 
     v8 kf[KT][KS][NP], vf[KT][KS][NP];
     f32x16 dk[KT][DB], dv[KT][DB];
@@ -598,13 +882,14 @@ __global__ __launch_bounds__(256, (Frag<T>::NP == 3 && KS > 2) || KT * KS > 8 ? 
     auto fetch = [&](int step) {
         char *to = lds + (NB == 2 ? (step & 1) * L::CHUNKS * 1024 : 0);
         const long long tile = qz + step;
-        for (int i = wave; i < L::CHUNKS; i += 4) {
+        for (int i = wave; i < L::CHUNKS; i += NW) {
             const char *from = i < RC ? a.Qr + (tile * RC + i) * 1024 : i < 2 * RC ? a.Gr + (tile * RC + i - RC) * 1024
                              : i < 2 * RC + TC ? a.Qt + (tile * TC + i - 2 * RC) * 1024
                              : i < 2 * RC + 2 * TC ? a.Gt + (tile * TC + i - 2 * RC - TC) * 1024 : a.stat + tile * 1024;
             load_chunk(from, to + i * 1024, lane);
         }
     };
+    __syncthreads();                                   // the last piece's tiles have been read
     if (first < last) fetch(first);
     for (int step = first; step < last; ++step) {
         wait_loads_and_barrier();
@@ -663,46 +948,17 @@ __global__ __launch_bounds__(256, (Frag<T>::NP == 3 && KS > 2) || KT * KS > 8 ? 
 #pragma unroll
     for (int t = 0; t < KT; ++t) {
         const int i = (k0 + t) * 32 + col;
-        if (i >= n) continue;
-        const long long at = ((long long)split * a.s.B * a.s.Hk + z) * a.s.N + i, to = k_row(a.s, z, i) * a.s.d;
-#pragma unroll
-        for (int b = 0; b < DB; ++b)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int dim = 32 * b + 8 * (r / 4) + 4 * half + r % 4;
-                if (dim < a.s.d) {
-                    const float x = dk[t][b][r] * back_k, y = dv[t][b][r] * back_v;
-                    if (a.splits > 1) {
-                        a.part[at * a.s.d + dim] = x;
-                        a.part2[at * a.s.d + dim] = y;
-                    } else {
-                        ((T *)a.dk)[to + dim] = (T)x;
-                        ((T *)a.dv)[to + dim] = (T)y;
-                    }
-                }
-            }
+        if (!w.whole) {
+            const long long tile = (long long)w.slot * (NW * KT) + wave * KT + t;
+            store_part<DB>(a.part + tile * DB * 1024, lane, dk[t], back_k);
+            store_part<DB>(a.part2 + tile * DB * 1024, lane, dv[t], back_v);
+        } else if (i < n) {
+            const long long to = k_row(a.s, z, i) * a.s.d;
+            store_row<T, DB>((T *)a.dk + to, a.s.d, half, dk[t], back_k);
+            store_row<T, DB>((T *)a.dv + to, a.s.d, half, dv[t], back_v);
+        }
     }
-}
-
-// the splits' sums in their order; one thread per element of dq, or of dk and dv
-template <class T>
-__global__ __launch_bounds__(256) void xa_sum_kernel(TileArgs a, int keys) {
-    const int rows = keys ? a.s.N : a.s.M;
-    const long long per = (long long)a.s.B * a.s.Hk * rows * a.s.d, e = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (e >= per) return;
-    const int dim = (int)(e % a.s.d), row = (int)(e / a.s.d % rows), z = (int)(e / a.s.d / rows);
-    if (keys && row >= keys_of(a.s, z)) return;
-    float x = 0.f, y = 0.f;
-    for (int i = 0; i < a.splits; ++i) {
-        x += a.part[i * per + e];
-        if (keys) y += a.part2[i * per + e];
     }
-    if (keys) {
-        const long long to = k_row(a.s, z, row) * a.s.d + dim;
-        ((T *)a.dk)[to] = (T)x;
-        ((T *)a.dv)[to] = (T)y;
-    } else
-        ((T *)a.dq)[q_row(a.s, z, row) * a.s.d + dim] = (T)x;
 }
 
 // ---------------------------------------------------------------- a few query rows: K and V read once, in place
@@ -717,17 +973,6 @@ template <int LPR> __device__ __forceinline__ float group_sum(float v) {
 #undef XA_DPP_ADD
     return v;
 }
-
-struct FewArgs {
-    Shape s;
-    const void *q, *k, *v;
-    long long q_sb, q_sn, q_sh, k_sb, k_sn, k_sh, v_sb, v_sn, v_sh, mask_sb;
-    const unsigned char *mask;
-    int splits;
-    float c;
-    void *o;
-    float *lse, *part, *ml;
-};
 
 template <class T, bool VEC> __device__ __forceinline__ void few_load(const T *x, int off, int d, float (&v)[8]) {
     T raw[8];
@@ -884,67 +1129,82 @@ int check(const md_attn_desc &a, const char *what) {
 int ks_of(int d) { return d <= 16 ? 1 : d <= 32 ? 2 : d <= 64 ? 4 : d <= 96 ? 6 : 8; }
 size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 
+// One launch of a tile kernel: `nw` waves of `t` tiles of 32 rows each in a workgroup, `workers` workgroups, and where their parts go.
+struct Tiles {
+    int nw, t, rows, step, workers;
+    long long units;
+    bool join;
+    size_t part, part2, ml, first;
+};
 // How a call is run, and where its workspace's parts begin; the same for the size query and the launch.
 struct Plan {
     int M, Z, KS, NP, DB, q_tiles, k_tiles;
     bool few;
-    int qt, kt, tk;                               // query tiles and key tiles per wave, keys per step (forward, dq)
-    int splits, splits_q, splits_k;               // forward; dq over keys; dk, dv over queries
-    size_t idx, cnt, Qr, Kr, Vt, Qt, Kt, Vr, Gr, Gt, stat, amax, part, part2, ml, bytes;
+    int splits;                                   // few rows: of the keys
+    Tiles fwd, dq, dkv;
+    size_t idx, cnt, Qr, Kr, Vt, Qt, Kt, Vr, Gr, Gt, stat, amax, part, ml, bytes;
 };
 
-// enough workgroups for the chip: split the long axis until there are about `want`, at least `least` steps each
-int split_for(long long blocks, long long steps, int want, int least) {
-    long long s = blocks ? (want + blocks - 1) / blocks : 1;
-    if (s > steps / least) s = steps / least;
-    return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
+// Workgroups that the chip holds at once, so that they all run to the end together -- unless that left them fewer than `least` steps: then one block of rows
+// each at the least.  `step` as in TileArgs; the number of keys is what it is without a mask.
+Tiles tiles_for(int Z, int tiles, int t, int step, long long steps, int least, int per_cu, bool masked) {
+    Tiles r{};
+    r.nw = tiles <= 1 ? 1 : 4;
+    r.t = r.nw == 1 ? 1 : t;
+    r.rows = 32 * r.t * r.nw;
+    r.step = step;
+    const long long blocks = (long long)Z * ((tiles + r.t * r.nw - 1) / (r.t * r.nw)), units = blocks * (steps < 1 ? 1 : steps);
+    const long long most = (r.nw == 1 ? 8 : per_cu) * CUS, want = std::max(blocks, units / least);
+    r.workers = (int)std::max<long long>(1, std::min(most, want));
+    r.units = units;
+    r.join = blocks && (masked || units % r.workers || units / r.workers % (steps < 1 ? 1 : steps));
+    return r;
 }
 
-Plan make_plan(const md_attn_desc &a, bool backward) {
+template <int NP, int KS> Plan plan_of(const md_attn_desc &a, bool backward) {
     Plan p{};
     p.M = a.Hq / a.Hk * a.Nq;
     p.Z = a.B * a.Hk;
-    p.KS = ks_of(a.d);
-    p.NP = a.dtype == 0 ? 3 : 1;
-    p.DB = (p.KS + 1) / 2;
+    p.KS = KS;
+    p.NP = NP;
+    p.DB = (KS + 1) / 2;
     p.q_tiles = (p.M + 31) / 32;
     p.k_tiles = (a.Nk + 63) / 64 * 2;
     p.few = !backward && p.M <= FEW_ROWS;
     size_t at = 0;
     auto take = [&](size_t n) { const size_t r = at; at = align256(at + n); return r; };
-    const size_t rows = (size_t)p.Z * p.M, kb = 1024;
+    const size_t kb = 1024;
     if (p.few) {
-        const int keys = a.Nk < 1 ? 1 : a.Nk;
-        p.splits = split_for(p.Z, keys, 4 * CUS, 128);
+        // as many workgroups as the chip holds at once (registers: 7, 3, 2 a CU for 1, 4, 8 rows), 128 keys each at the least
+        const long long want = (p.M <= 1 ? 7 : p.M <= 4 ? 3 : 2) * CUS / std::max(1, p.Z), most = a.Nk / 128;
+        p.splits = (int)std::max<long long>(1, std::min<long long>(std::min(want, most), 64));
         if (p.splits > 1) {
-            p.part = take(rows * p.splits * a.d * 4);
-            p.ml = take(rows * p.splits * 8);
+            p.part = take((size_t)p.Z * p.M * p.splits * a.d * 4);
+            p.ml = take((size_t)p.Z * p.M * p.splits * 8);
         }
         p.bytes = at;
         return p;
     }
-    if (a.key_mask) {
+    const bool masked = a.key_mask != nullptr;
+    if (masked) {
         p.idx = take((size_t)a.B * a.Nk * 4);
         p.cnt = take((size_t)a.B * 4);
     }
     const size_t qR = (size_t)p.Z * p.q_tiles * p.KS * p.NP * kb, qT = (size_t)p.Z * p.q_tiles * p.DB * 2 * p.NP * kb;
     const size_t kR = (size_t)p.Z * p.k_tiles * p.KS * p.NP * kb, kT = (size_t)p.Z * p.k_tiles * p.DB * 2 * p.NP * kb;
-    auto wgs = [&](int tiles, int per) { return (long long)p.Z * ((tiles + 4 * per - 1) / (4 * per)); };
-    // two query tiles per wave read every key fragment once for both; one where that leaves the chip short of workgroups, or registers
-    p.qt = p.NP == 1 && p.KS <= 4 && wgs(p.q_tiles, 2) >= 2 * CUS ? 2 : 1;
-    p.kt = 1;
-    p.tk = p.NP == 3 && p.KS > 2 ? 32 : 64;
+    const int qt = p.q_tiles >= 8 ? query_tiles<NP, KS>() : 1;
     p.Qr = take(qR);
     p.Kr = take(kR);
     if (!backward) {
+        const int tk = p.NP == 3 && p.KS > 2 ? 32 : 64;
         p.Vt = take(kT);
-        p.splits = split_for(wgs(p.q_tiles, p.qt), (a.Nk + p.tk - 1) / p.tk, 2 * CUS, 4);
-        if (p.splits > 1) {
-            p.part = take(rows * p.splits * a.d * 4);
-            p.ml = take(rows * p.splits * 8);
+        p.fwd = tiles_for(p.Z, p.q_tiles, qt, tk, (a.Nk + tk - 1) / tk, 4, qt == 2 ? fwd_per_cu<NP, KS, 2>() : fwd_per_cu<NP, KS, 1>(), masked);
+        if (p.fwd.join) {
+            p.fwd.part = take((size_t)2 * p.fwd.workers * p.fwd.rows * p.DB * 32 * 4);
+            p.fwd.ml = take((size_t)2 * p.fwd.workers * p.fwd.rows * 8);
+            p.fwd.first = take((size_t)p.fwd.workers * 16);
         }
     } else {
-        p.tk = 32;
         p.Vr = take(kR);
         p.Kt = take(kT);
         p.Qt = take(qT);
@@ -952,15 +1212,24 @@ Plan make_plan(const md_attn_desc &a, bool backward) {
         p.Gt = take(qT);
         p.stat = take((size_t)p.Z * p.q_tiles * kb);
         p.amax = take(256);
-        p.splits_q = split_for(wgs(p.q_tiles, p.qt), (a.Nk + p.tk - 1) / p.tk, 2 * CUS, 4);
-        p.splits_k = split_for(wgs(p.k_tiles, p.kt), p.q_tiles, 2 * CUS, 4);
-        const size_t nq = p.splits_q > 1 ? rows * p.splits_q * a.d * 4 : 0;
-        const size_t nk = p.splits_k > 1 ? (size_t)p.Z * a.Nk * p.splits_k * a.d * 4 : 0;
-        p.part = take(nq > nk ? nq : nk);            // dq's is summed before dk's is written
-        p.part2 = take(nk);
+        p.dq = tiles_for(p.Z, p.q_tiles, qt, 32, (a.Nk + 31) / 32, 8, qt == 2 ? dq_per_cu<NP, KS, 2>() : dq_per_cu<NP, KS, 1>(), masked);
+        p.dkv = tiles_for(p.Z, (a.Nk + 31) / 32, 1, 0, p.q_tiles, 8, dkv_per_cu<NP, KS>(), masked);
+        const size_t nq = p.dq.join ? (size_t)2 * p.dq.workers * p.dq.rows * p.DB * 32 * 4 : 0, nk = p.dkv.join ? (size_t)2 * p.dkv.workers * p.dkv.rows * p.DB * 32 * 4 : 0;
+        p.dq.part = p.dkv.part = take(std::max(nq, nk));            // dq's are summed before dk's are written (and `first` likewise)
+        p.dkv.part2 = take(nk);
+        p.dq.first = p.dkv.first = take((size_t)std::max(p.dq.workers, p.dkv.workers) * 16);
     }
     p.bytes = at;
     return p;
+}
+
+Plan make_plan(const md_attn_desc &a, bool backward) {
+    const int ks = ks_of(a.d);
+    if (a.dtype == 0)
+        return ks == 1 ? plan_of<3, 1>(a, backward) : ks == 2 ? plan_of<3, 2>(a, backward) : ks == 4 ? plan_of<3, 4>(a, backward)
+             : ks == 6 ? plan_of<3, 6>(a, backward) : plan_of<3, 8>(a, backward);
+    return ks == 1 ? plan_of<1, 1>(a, backward) : ks == 2 ? plan_of<1, 2>(a, backward) : ks == 4 ? plan_of<1, 4>(a, backward)
+         : ks == 6 ? plan_of<1, 6>(a, backward) : plan_of<1, 8>(a, backward);
 }
 
 bool aligned_rows(const void *x, size_t size, int d, long long sb, long long sn, long long sh) {
@@ -1003,9 +1272,7 @@ template <class T> int run_few(const md_attn_desc &a, const Plan &p, const Shape
     if (rc) return rc;
     MD_CHECK_LAUNCH("md_cross_attn_fwd: few rows");
     if (p.splits > 1) {
-        TileArgs t{};
-        t.s = sh, t.splits = p.splits, t.part = f.part, t.ml = f.ml, t.o = a.o, t.lse = a.lse;
-        xa_join_kernel<T><<<(unsigned)p.Z * p.M, 64, 0, s>>>(t);
+        xa_few_join_kernel<T><<<(unsigned)p.Z * p.M, 64, 0, s>>>(f);
         MD_CHECK_LAUNCH("md_cross_attn_fwd: join");
     }
     return MD_OK;
@@ -1043,6 +1310,15 @@ template <class T, int KS> int launch_pack(PackArgs &k, const Plan &p, long long
     return MD_OK;
 }
 
+TileArgs tile_args(const Shape &sh, const Plan &p, const Tiles &w, char *ws) {
+    TileArgs t{};
+    t.s = sh;
+    t.q_tiles = p.q_tiles, t.k_tiles = p.k_tiles, t.workers = w.workers, t.rows = w.rows, t.step = w.step, t.units = w.units;
+    t.part = (float *)(ws + w.part), t.part2 = (float *)(ws + w.part2), t.ml = (float *)(ws + w.ml);
+    t.first = w.join ? (int4 *)(ws + w.first) : nullptr;
+    return t;
+}
+
 template <class T, int KS> int run_fwd(const md_attn_desc &a, const Plan &p, const Shape &sh, char *ws, hipStream_t s) {
     constexpr int NP = Frag<T>::NP, TK = NP == 3 && KS > 2 ? 32 : 64;
     const float sign = a.scale < 0.f ? -1.f : 1.f;          // c > 0 in the kernels: a negative scale goes into q's sign
@@ -1052,23 +1328,20 @@ template <class T, int KS> int run_fwd(const md_attn_desc &a, const Plan &p, con
     k.job[1] = job_of(a.k, a.k_sb, a.k_sn, a.k_sh, sizeof(T), a.d, ws + p.Kr, nullptr, p.k_tiles, 0, 1.f);
     k.job[2] = job_of(a.v, a.v_sb, a.v_sn, a.v_sh, sizeof(T), a.d, nullptr, ws + p.Vt, p.k_tiles, 0, 1.f);
     if (int rc = launch_pack<T, KS>(k, p, 0, s)) return rc;
-    TileArgs t{};
-    t.s = sh;
+    TileArgs t = tile_args(sh, p, p.fwd, ws);
     t.Qr = ws + p.Qr, t.Kr = ws + p.Kr, t.Vt = ws + p.Vt;
-    t.q_tiles = p.q_tiles, t.k_tiles = p.k_tiles, t.splits = p.splits;
     t.c = fmaxf(fabsf(a.scale) * LOG2E, 1.2e-38f);         // not 0: the scores of rows behind the last key are -inf
-    t.o = a.o, t.lse = a.lse, t.part = (float *)(ws + p.part), t.ml = (float *)(ws + p.ml);
-    const long long blocks = (long long)p.Z * ((p.q_tiles + 4 * p.qt - 1) / (4 * p.qt)) * p.splits;
-    MD_REQUIRE(blocks < (1LL << 31) - 8, "md_cross_attn_fwd: too many tiles");
-    t.blocks = (int)blocks;
-    if constexpr (NP == 1 && KS <= 4) {
-        if (p.qt == 2) xa_fwd_kernel<T, KS, 2, TK><<<grid8(blocks), 256, 0, s>>>(t);
-        else xa_fwd_kernel<T, KS, 1, TK><<<grid8(blocks), 256, 0, s>>>(t);
+    t.o = a.o, t.lse = a.lse;
+    const unsigned grid = grid8(t.workers);
+    if (p.fwd.nw == 1) xa_fwd_kernel<T, KS, 1, TK, 1><<<grid, 64, 0, s>>>(t);
+    else if constexpr (query_tiles<NP, KS>() == 2) {
+        if (p.fwd.t == 2) xa_fwd_kernel<T, KS, 2, TK, 4><<<grid, 256, 0, s>>>(t);
+        else xa_fwd_kernel<T, KS, 1, TK, 4><<<grid, 256, 0, s>>>(t);
     } else
-        xa_fwd_kernel<T, KS, 1, TK><<<grid8(blocks), 256, 0, s>>>(t);
+        xa_fwd_kernel<T, KS, 1, TK, 4><<<grid, 256, 0, s>>>(t);
     MD_CHECK_LAUNCH("md_cross_attn_fwd");
-    if (p.splits > 1) {
-        xa_join_kernel<T><<<(unsigned)p.Z * p.M, 64, 0, s>>>(t);
+    if (p.fwd.join) {
+        xa_join_kernel<T, (KS + 1) / 2><<<dim3(t.workers, t.rows / 32), 256, 0, s>>>(t);
         MD_CHECK_LAUNCH("md_cross_attn_fwd: join");
     }
     return MD_OK;
@@ -1097,43 +1370,46 @@ template <class T, int KS> int run_bwd(const md_attn_desc &a, const Plan &p, con
         zero = (long long)a.B * ((a.Nk + 31) / 32);
     }
     if (int rc = launch_pack<T, KS>(k, p, zero, s)) return rc;
-    TileArgs t{};
-    t.s = sh;
-    t.Qr = ws + p.Qr, t.Kr = ws + p.Kr, t.Vr = ws + p.Vr, t.Qt = ws + p.Qt, t.Kt = ws + p.Kt, t.Gr = ws + p.Gr, t.Gt = ws + p.Gt, t.stat = ws + p.stat;
-    t.q_tiles = p.q_tiles, t.k_tiles = p.k_tiles;
-    t.c = fmaxf(fabsf(a.scale) * LOG2E, 1.2e-38f);
-    t.dq = a.dq, t.dk = a.dk, t.dv = a.dv, t.part = (float *)(ws + p.part), t.part2 = (float *)(ws + p.part2);
-    t.amax = (const unsigned *)(ws + p.amax);
+    auto args = [&](const Tiles &w) {
+        TileArgs t = tile_args(sh, p, w, ws);
+        t.Qr = ws + p.Qr, t.Kr = ws + p.Kr, t.Vr = ws + p.Vr, t.Qt = ws + p.Qt, t.Kt = ws + p.Kt, t.Gr = ws + p.Gr, t.Gt = ws + p.Gt, t.stat = ws + p.stat;
+        t.c = fmaxf(fabsf(a.scale) * LOG2E, 1.2e-38f);
+        t.dq = a.dq, t.dk = a.dk, t.dv = a.dv;
+        t.amax = (const unsigned *)(ws + p.amax);
+        return t;
+    };
     if (a.dq && p.M) {
+        TileArgs t = args(p.dq);
         t.scale = a.scale;
-        t.splits = p.splits_q;
-        const long long blocks = (long long)p.Z * ((p.q_tiles + 4 * p.qt - 1) / (4 * p.qt)) * t.splits;
-        MD_REQUIRE(blocks < (1LL << 31) - 8, "md_cross_attn_bwd: too many tiles");
-        t.blocks = (int)blocks;
-        if constexpr (NP == 1 && KS <= 4) {
-            if (p.qt == 2) xa_dq_kernel<T, KS, 2, 32><<<grid8(blocks), 256, 0, s>>>(t);
-            else xa_dq_kernel<T, KS, 1, 32><<<grid8(blocks), 256, 0, s>>>(t);
+        const unsigned grid = grid8(t.workers);
+        if (p.dq.nw == 1) xa_dq_kernel<T, KS, 1, 32, 1><<<grid, 64, 0, s>>>(t);
+        else if constexpr (query_tiles<NP, KS>() == 2) {
+            if (p.dq.t == 2) xa_dq_kernel<T, KS, 2, 32, 4><<<grid, 256, 0, s>>>(t);
+            else xa_dq_kernel<T, KS, 1, 32, 4><<<grid, 256, 0, s>>>(t);
         } else
-            xa_dq_kernel<T, KS, 1, 32><<<grid8(blocks), 256, 0, s>>>(t);
+            xa_dq_kernel<T, KS, 1, 32, 4><<<grid, 256, 0, s>>>(t);
         MD_CHECK_LAUNCH("md_cross_attn_bwd: dq");
-        if (t.splits > 1) {
-            xa_sum_kernel<T><<<md_cdiv((long long)p.Z * p.M * a.d, 256), 256, 0, s>>>(t, 0);
+        if (p.dq.join) {
+            xa_sum_kernel<T, (KS + 1) / 2><<<dim3(t.workers, t.rows / 32), 256, 0, s>>>(t);
             MD_CHECK_LAUNCH("md_cross_attn_bwd: dq sums");
         }
     }
     if (a.dk && a.Nk) {
+        TileArgs t = args(p.dkv);
         t.scale = fabsf(a.scale);                          // Q's fragments carry the sign
-        t.splits = p.splits_k;
-        const long long blocks = (long long)p.Z * ((p.k_tiles + 3) / 4) * t.splits;
-        MD_REQUIRE(blocks < (1LL << 31) - 8, "md_cross_attn_bwd: too many tiles");
-        t.blocks = (int)blocks;
+        const unsigned grid = grid8(t.workers);
         using L = DkvLds<T, KS, 1>;
         const int lds = L::BUFFERS * L::CHUNKS * 1024;
-        if (int rc = set_lds(xa_dkv_kernel<T, KS, 1>, lds)) return rc;
-        xa_dkv_kernel<T, KS, 1><<<grid8(blocks), 256, lds, s>>>(t);
+        if (p.dkv.nw == 1) {
+            if (int rc = set_lds(xa_dkv_kernel<T, KS, 1, 1>, lds)) return rc;
+            xa_dkv_kernel<T, KS, 1, 1><<<grid, 64, lds, s>>>(t);
+        } else {
+            if (int rc = set_lds(xa_dkv_kernel<T, KS, 1, 4>, lds)) return rc;
+            xa_dkv_kernel<T, KS, 1, 4><<<grid, 256, lds, s>>>(t);
+        }
         MD_CHECK_LAUNCH("md_cross_attn_bwd: dk, dv");
-        if (t.splits > 1) {
-            xa_sum_kernel<T><<<md_cdiv((long long)p.Z * a.Nk * a.d, 256), 256, 0, s>>>(t, 1);
+        if (p.dkv.join) {
+            xa_sum_kernel<T, (KS + 1) / 2><<<dim3(t.workers, t.rows / 32), 256, 0, s>>>(t);
             MD_CHECK_LAUNCH("md_cross_attn_bwd: dk, dv sums");
         }
     }

@@ -1601,22 +1601,37 @@ class _LayerNorm(torch.autograd.Function):
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, gy):
+    def _backward(ctx, gy):
         x2, codes, scales, stat, w = ctx.saved_tensors
-        C, dev = gy.shape[-1], gy.device
+        C, dev, dtype = gy.shape[-1], gy.device, ctx.dtype
         with _on(dev):
-            g, ldg = _rows(gy.to(ctx.dtype), C)
-            rows = g.shape[0]
+            if gy.dtype is not dtype:
+                gy = gy.to(dtype)
+            if gy.is_contiguous():
+                g, ldg = gy, C
+            else:
+                g, ldg = _rows(gy, C)
+            rows = gy.numel() // C
             ldx = C if x2 is None or rows <= 1 else x2.stride(0)
             need_x, need_w, need_b = ctx.needs_input_grad[:3]
-            dx = torch.empty(gy.shape, device=dev, dtype=ctx.dtype) if need_x else None
-            dwb = torch.empty(2, C, device=dev, dtype=torch.float32) if need_w or need_b else None
-            nbytes = 0 if dwb is None else _lib.load().md_layer_norm_bwd_ws_bytes(rows, C)
-            ws = _ws(nbytes, dev) if nbytes else None
-            _timed_call("md_layer_norm_bwd", _at(g), ldg, _at(x2), ldx, _at(codes), _at(scales), _TOKEN_DTYPE[ctx.dtype], _at(stat), _at(w), rows, C,
-                        _at(dx), _at(dwb[0]) if need_w else None, _at(dwb[1]) if need_b else None, _at(ws), nbytes, _stream_of(dev))
-        return dx, dwb[0].to(ctx.wdtype) if need_w else None, dwb[1].to(ctx.bdtype) if need_b else None, None, None
+            dx = torch.empty(gy.shape, device=dev, dtype=dtype) if need_x else None
+            dw = torch.empty(C, device=dev, dtype=torch.float32) if need_w else None
+            db = torch.empty(C, device=dev, dtype=torch.float32) if need_b else None
+            nbytes = _lib.load().md_layer_norm_bwd_ws_bytes(rows, C) if need_w or need_b else 0
+            ws = torch.empty(nbytes, device=dev, dtype=torch.uint8) if nbytes else None
+            _timed_call("md_layer_norm_bwd", g.data_ptr(), ldg, _at(x2), ldx, _at(codes), _at(scales), _TOKEN_DTYPE[dtype], stat.data_ptr(), _at(w), rows, C,
+                        _at(dx), _at(dw), _at(db), _at(ws), nbytes, _stream_of(dev))
+        if need_w and ctx.wdtype is not torch.float32:
+            dw = dw.to(ctx.wdtype)
+        if need_b and ctx.bdtype is not torch.float32:
+            db = db.to(ctx.bdtype)
+        return dx, dw, db, None, None
+
+    _backward_once = staticmethod(torch.autograd.function.once_differentiable(_backward.__func__))
+
+    @staticmethod
+    def backward(ctx, gy):
+        return (_LayerNorm._backward_once if torch.is_grad_enabled() else _LayerNorm._backward)(ctx, gy)
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5, act_bits=0):
@@ -1685,13 +1700,13 @@ class _CrossAttention(torch.autograd.Function):
         return o
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, g):
+    def _backward(ctx, g):
         q, k, v, key_mask, o, lse = ctx.saved_tensors
         dev = q.device
         with _on(dev):
-            g, gs = _attn_strides(g.to(q.dtype))
-            o = o.contiguous()
+            g, gs = _attn_strides(g if g.dtype is q.dtype else g.to(q.dtype))
+            if not o.is_contiguous():
+                o = o.contiguous()
             a = _attn_desc(q, k, v, key_mask, ctx.scale)
             a.o, a.lse, a.g = o.data_ptr(), lse.data_ptr(), g.data_ptr()
             a.g_sb, a.g_sn, a.g_sh = gs
@@ -1704,6 +1719,12 @@ class _CrossAttention(torch.autograd.Function):
             ws = _ws(nbytes, dev) if nbytes else None
             _timed_call("md_cross_attn_bwd", ctypes.byref(a), _at(ws), nbytes, _stream_of(dev))
         return dq, dk if ctx.needs_input_grad[1] else None, dv if ctx.needs_input_grad[2] else None, None, None
+
+    _backward_once = staticmethod(torch.autograd.function.once_differentiable(_backward.__func__))
+
+    @staticmethod
+    def backward(ctx, g):
+        return (_CrossAttention._backward_once if torch.is_grad_enabled() else _CrossAttention._backward)(ctx, g)
 
 
 def cross_attention(q, k, v, key_mask=None, scale=None):
