@@ -23,6 +23,7 @@
 // the type before their products (half a step relative).  float16 holds P times 2^7 (forward) or 2^15 (backward) and dS times a power
 // of two from the largest |g| |v|, so that the small weights of long rows do not fall below its range.
 #include <algorithm>
+#include <type_traits>
 
 #include "md_types.hpp"
 
@@ -52,14 +53,22 @@ __device__ __forceinline__ f32x16 mfma_pieces(const typename Vec<E>::v8 (&a)[NP]
     return mfma(a[0], b[0], c);
 }
 
+// 8 values as NP pieces each.  Pairs are rounded together (one instruction), and the pair's halves are its values' bits: what is left over is exact
 template <class E, int NP> __device__ __forceinline__ void split8(const float (&v)[8], typename Vec<E>::v8 (&out)[NP]) {
+    using v2 = E __attribute__((ext_vector_type(2)));
+    using f2 = float __attribute__((ext_vector_type(2)));
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        float x = v[j];
+    for (int j = 0; j < 8; j += 2) {
+        float x = v[j], y = v[j + 1];
 #pragma unroll
         for (int p = 0; p < NP; ++p) {
-            out[p][j] = (E)x;
-            x -= (float)out[p][j];
+            const v2 r = __builtin_convertvector((f2){x, y}, v2);
+            out[p][j] = r[0], out[p][j + 1] = r[1];
+            if (p + 1 < NP) {
+                const unsigned w = __builtin_bit_cast(unsigned, r);        // (bf16: the upper halves of two floats)
+                x -= __uint_as_float(w << 16);
+                y -= __uint_as_float(w & 0xFFFF0000u);
+            }
         }
     }
 }
@@ -96,10 +105,19 @@ __device__ __forceinline__ int die_order(int block, int blocks) {
 // Workgroups of 4 waves that a CU holds at once (registers, and shared memory where it is short), per kernel; also what the compiler is asked to keep to.
 template <int NP, int KS, int QT> constexpr int fwd_per_cu() { return NP == 3 ? (KS <= 4 ? 3 : KS == 6 ? 2 : 1) : QT == 2 ? 2 : KS <= 2 ? 4 : KS == 4 ? 3 : 2; }
 template <int NP, int KS, int QT> constexpr int dq_per_cu() { return NP == 3 ? (KS <= 2 ? 3 : KS == 4 ? 2 : 1) : QT == 2 ? 2 : KS <= 2 ? 4 : KS == 4 ? 3 : 2; }
-template <int NP, int KS> constexpr int dkv_per_cu() { return NP == 3 ? (KS == 1 ? 4 : KS == 2 ? 3 : 1) : KS <= 2 ? 4 : KS == 4 ? 3 : 2; }
+template <int NP, int KS> constexpr int dkv_per_cu() { return NP == 3 ? (KS == 1 ? 4 : KS == 2 ? 3 : 1) : KS == 4 ? 3 : 2; }
 // query tiles per wave: two read every key fragment once for both (heads of 64: 371 us against 386 in the forward pass of 2 x 16 heads x 4096 x 8192), but
 // hold the registers of two, which the smaller heads use better for more waves (heads of 32, 2 x 2 x 20480 x 20480: 430 us against 406)
 template <int NP, int KS> constexpr int query_tiles() { return NP == 1 && KS == 4 ? 2 : 1; }
+// key tiles per wave of the dk / dv kernel: two halve the fragments read from shared memory, which are what bounds it for small heads (heads of 32: 652 us
+// against 602); from 64 on the accumulators of two do not fit
+template <int NP, int KS> constexpr int key_tiles() { return NP == 1 && KS <= 2 ? 2 : 1; }
+
+// keys per step of the forward kernel: as many as shared memory has room for beside the other workgroups (two buffers each) -- a step is a barrier, and of its
+// parts of 32 keys all but the first have their products under way when their turn comes.  The backward kernels take 32 a step: they need the registers
+// that this costs for more waves (dq, heads of 32: 451 us at 4 waves per SIMD, 485 at 2 with the products ahead)
+constexpr int DQ_KEYS = 32;
+template <int NP, int KS> constexpr int fwd_keys() { return NP == 3 ? (KS <= 2 ? 64 : 32) : KS <= 2 ? 128 : 64; }
 
 // ---------------------------------------------------------------- what the kernels are told
 struct Shape {
@@ -168,7 +186,8 @@ struct PackJob {
     int tiles;                   // of 32 rows, per z; rows behind the last are written as zeros
     int query;                   // rows are query rows (else valid keys)
     int vec;                     // 16-byte loads: d and all strides are multiples of 8 elements, x is aligned
-    float sign;
+    float factor;
+    float *norm;                 // largest |row| (after `factor`) of each tile, or null
     unsigned *amax;              // largest |row|^2 as float bits, or null
 };
 struct PackArgs {
@@ -176,7 +195,7 @@ struct PackArgs {
     int blocks[5];               // jobs' first workgroups; behind the last job: rows of masked keys to be zeroed in dk, dv
     int jobs;
     Shape s;
-    const void *o;               // with `stat`: of job 0 (the gradient g) also D = g . o and lse, per tile 32 + 32 floats in 1 KB
+    const void *o;               // with `stat`: of job 0 (the gradient g) also -lse and -D = -g . o, per tile 32 + 32 floats in 1 KB
     const float *lse;
     char *stat;
     const unsigned char *mask;
@@ -241,7 +260,7 @@ __global__ __launch_bounds__(64) void xa_pack_kernel(PackArgs a) {
             float v[8];
             typename Vec<E>::v8 p[NP];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = (float)rows[col * LD + 16 * k + 8 * half + e] * job.sign;
+            for (int e = 0; e < 8; ++e) v[e] = (float)rows[col * LD + 16 * k + 8 * half + e] * job.factor;
             split8<E, NP>(v, p);
 #pragma unroll
             for (int n = 0; n < NP; ++n) *(typename Vec<E>::v8 *)(job.R + ((at * KS + k) * NP + n) * 1024 + lane * 16) = p[n];
@@ -255,7 +274,7 @@ __global__ __launch_bounds__(64) void xa_pack_kernel(PackArgs a) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 const int r = 16 * (f % 2) + 8 * (e / 4) + 4 * half + e % 4;
-                v[e] = dim < DP ? (float)rows[r * LD + (dim < DP ? dim : 0)] * job.sign : 0.f;
+                v[e] = dim < DP ? (float)rows[r * LD + (dim < DP ? dim : 0)] * job.factor : 0.f;
             }
             split8<E, NP>(v, p);
 #pragma unroll
@@ -270,14 +289,17 @@ __global__ __launch_bounds__(64) void xa_pack_kernel(PackArgs a) {
         }
         D = swap_halves_sum(D);
         float *st = (float *)(a.stat + at * 1024);
-        if (half == 0) st[col] = i < s.M ? a.lse[(long long)z * s.M + i] : INFINITY;
-        else st[32 + col] = D;
+        if (half == 0) st[col] = i < s.M ? -a.lse[(long long)z * s.M + i] : -INFINITY;
+        else st[32 + col] = -D;
     }
-    if (job.amax) {
+    if (job.amax || job.norm) {
         float q = 0.f;
         for (int e = half * 8 * KS; e < (half + 1) * 8 * KS; ++e) q = fmaf((float)rows[col * LD + e], (float)rows[col * LD + e], q);
-        q = md_wave_max(swap_halves_sum(q));
-        if (lane == 0) atomicMax(job.amax, __float_as_uint(q));       // non-negative floats order as their bits; a maximum does not depend on the order
+        q = swap_halves_sum(q);
+        const bool nan = __any(q != q);
+        q = nan ? NAN : md_wave_max(q);
+        if (lane == 0 && job.norm) job.norm[at] = sqrtf(q) * fabsf(job.factor);
+        if (lane == 0 && job.amax) atomicMax(job.amax, __float_as_uint(q));       // non-negative floats order as their bits; a maximum does not depend on the order
     }
 }
 
@@ -335,6 +357,7 @@ template <int DB> __device__ __forceinline__ void add_part(const float *from, in
 struct TileArgs {
     Shape s;
     const char *Qr, *Kr, *Vt;                          // forward
+    const float *qn, *kn;                              // largest row norm of each tile of 32
     const char *Qt, *Kt, *Vr, *Gr, *Gt, *stat;         // backward
     int q_tiles, k_tiles, workers, rows, step;          // `step`: keys per step; 0: blocks are of keys, a step is a tile of 32 queries
     long long units;                                    // all of them; with a mask the device counts
@@ -458,7 +481,21 @@ struct Walk {
 template <class E> struct Shift { static constexpr float fwd = 0.f, bwd = 0.f; };
 template <> struct Shift<f16_t> { static constexpr float fwd = 7.f, bwd = 15.f; };
 
+// largest of the norms of tiles `from` .. `to` - 1 (a NaN stays): every lane of a wave calls it
+__device__ __forceinline__ float row_norm(const float *norm, int from, int to) {
+    float x = 0.f;
+    bool nan = false;
+    for (int i = from + (threadIdx.x & 63); i < to; i += 64) {
+        x = fmaxf(x, norm[i]);
+        nan |= norm[i] != norm[i];
+    }
+    return __any(nan) ? NAN : __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(md_wave_max(x))));
+}
+
 // ---------------------------------------------------------------- forward: 32 QT queries per wave, NW waves, steps of TK keys
+// Where |q| |k| scale of a piece's rows bounds its scores by 2^48 either way, m is 0 throughout: no maximum, no rescaling, and the step is straight-line code in
+// which the products of one half run beside the exponentials of the other.  P and its sums stay within 2^+-48 times the row length then (bf16 has
+// float32's exponents; float16 has not and always takes the running maximum).
 template <class T, int KS, int QT, int TK, int NW>
 __global__ __launch_bounds__(64 * NW, (NW == 4 ? fwd_per_cu<Frag<T>::NP, KS, QT>() : 1)) void xa_fwd_kernel(TileArgs a) {
     using E = typename Frag<T>::E;
@@ -487,71 +524,106 @@ __global__ __launch_bounds__(64 * NW, (NW == 4 ? fwd_per_cu<Frag<T>::NP, KS, QT>
         m[t] = -INFINITY;
         l[t] = 0.f;
     }
+    const float c = NP == 3 ? 1.f : a.c;               // (float32: in q's fragments)
+    constexpr float BOUND = Shift<E>::fwd == 0.f ? 48.f : 0.f;
     const char *Kz = a.Kr + (long long)z * a.k_tiles * KS * NP * 1024, *Vz = a.Vt + (long long)z * a.k_tiles * DB * 2 * NP * 1024;
     auto fetch = [&](int step) {
         char *to = lds[step & 1];
         for (int i = wave; i < KC + VC; i += NW)
             load_chunk(i < KC ? Kz + ((long long)step * KC + i) * 1024 : Vz + ((long long)step * VC + i - KC) * 1024, to + i * 1024, lane);
     };
-    __syncthreads();                                   // the last piece's tiles have been read
-    if (w.first < last) fetch(w.first);
-    for (int step = w.first; step < last; ++step) {
+    // BOUNDED: no score of this piece can pass 2^BOUND either way, m stays 0.  TAIL: rows behind the last key
+    auto run = [&](auto bounded, auto tail, int step) {
+        constexpr bool BOUNDED = decltype(bounded)::value, TAIL = decltype(tail)::value;
         wait_loads_and_barrier();
         if (step + 1 < last) fetch(step + 1);
         const char *K = lds[step & 1], *V = K + KC * 1024;
+        f32x16 s[2][QT];
+        auto scores = [&](int u, f32x16 (&to)[QT]) {
 #pragma unroll
-        for (int t = 0; t < QT; ++t) {
-            f32x16 s[SUB];
+            for (int t = 0; t < QT; ++t) to[t] = (f32x16)0.f;
 #pragma unroll
-            for (int u = 0; u < SUB; ++u) {
-                s[u] = (f32x16)0.f;
+            for (int k = 0; k < KS; ++k) {
+                v8 f[NP];
+                read_frag<E, NP>(K + (u * KS + k) * NP * 1024, lane, f);
 #pragma unroll
-                for (int k = 0; k < KS; ++k) {
-                    v8 f[NP];
-                    read_frag<E, NP>(K + (u * KS + k) * NP * 1024, lane, f);
-                    s[u] = mfma_pieces<E, NP>(f, q[t][k], s[u]);
+                for (int t = 0; t < QT; ++t) to[t] = mfma_pieces<E, NP>(f, q[t][k], to[t]);
+            }
+        };
+        scores(0, s[0]);
+#pragma unroll
+        for (int u = 0; u < SUB; ++u) {
+            f32x16 (&x)[QT] = s[u & 1];
+            if constexpr (TAIL)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (step * TK + u * 32 + 8 * (r / 4) + 4 * half + r % 4 >= n)
+#pragma unroll
+                        for (int t = 0; t < QT; ++t) x[t][r] = -INFINITY;
+            if constexpr (!BOUNDED)
+#pragma unroll
+                for (int t = 0; t < QT; ++t) {
+                    float top = x[t][0];
+#pragma unroll
+                    for (int r = 1; r < 16; ++r) top = fmaxf(top, x[t][r]);
+                    top = swap_halves_max(top) * c;
+                    if (__any(top > m[t] + LAZY)) {
+                        const float up = fmaxf(m[t], top), f = __builtin_amdgcn_exp2f(m[t] - up);
+                        m[t] = up;
+                        l[t] *= f;
+#pragma unroll
+                        for (int b = 0; b < DB; ++b) o[t][b] *= f;
+                    }
                 }
-            }
-            if (step * TK + TK > n)                      // rows behind the last key
+            // the next half's products and this one's fragments are under way while the exponentials run
+            constexpr bool EARLY = DB * NP <= 4;           // (registers)
+            v8 vf[2][DB][NP];
+            if constexpr (EARLY)
 #pragma unroll
-                for (int u = 0; u < SUB; ++u)
+                for (int h = 0; h < 2; ++h)
 #pragma unroll
-                    for (int r = 0; r < 16; ++r)
-                        if (step * TK + u * 32 + 8 * (r / 4) + 4 * half + r % 4 >= n) s[u][r] = -INFINITY;
-            float top = s[0][0];
+                    for (int b = 0; b < DB; ++b) read_frag<E, NP>(V + ((u * DB + b) * 2 + h) * NP * 1024, lane, vf[h][b]);
+            if (u + 1 < SUB) scores(u + 1, s[(u + 1) & 1]);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int u = 0; u < SUB; ++u)
+            for (int h = 0; h < 2; ++h) {
+                v8 f[QT][NP];
 #pragma unroll
-                for (int r = 0; r < 16; ++r) top = fmaxf(top, s[u][r]);
-            top = swap_halves_max(top) * a.c;
-            if (__any(top > m[t] + LAZY)) {
-                const float up = fmaxf(m[t], top), f = __builtin_amdgcn_exp2f(m[t] - up);
-                m[t] = up;
-                l[t] *= f;
-#pragma unroll
-                for (int b = 0; b < DB; ++b) o[t][b] *= f;
-            }
-            const float base = m[t] - Shift<E>::fwd;
-#pragma unroll
-            for (int u = 0; u < SUB; ++u)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
+                for (int t = 0; t < QT; ++t) {
                     float p[8];
-                    v8 f[NP];
+                    const float base = m[t] - Shift<E>::fwd;
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
-                        p[e] = __builtin_amdgcn_exp2f(fmaf(s[u][8 * h + e], a.c, -base));
+                        const float y = x[t][8 * h + e];
+                        p[e] = __builtin_amdgcn_exp2f(BOUNDED ? (NP == 3 ? y : y * c) : fmaf(y, c, -base));
                         l[t] += p[e];
                     }
-                    split8<E, NP>(p, f);
-#pragma unroll
-                    for (int b = 0; b < DB; ++b) {
-                        v8 w[NP];
-                        read_frag<E, NP>(V + ((u * DB + b) * 2 + h) * NP * 1024, lane, w);
-                        o[t][b] = mfma_pieces<E, NP>(w, f, o[t][b]);
-                    }
+                    split8<E, NP>(p, f[t]);
                 }
+#pragma unroll
+                for (int b = 0; b < DB; ++b) {
+                    if constexpr (!EARLY) read_frag<E, NP>(V + ((u * DB + b) * 2 + h) * NP * 1024, lane, vf[h][b]);
+#pragma unroll
+                    for (int t = 0; t < QT; ++t) o[t][b] = mfma_pieces<E, NP>(vf[h][b], f[t], o[t][b]);
+                }
+            }
         }
+    };
+    const std::true_type yes;
+    const std::false_type no;
+    __syncthreads();                                   // the last piece's tiles have been read
+    if (w.first < last) fetch(w.first);
+    const int whole = min(last, n / TK);               // steps without rows behind the last key
+    int step = w.first;
+    if (BOUND > 0.f && row_norm(a.qn + (long long)z * a.q_tiles, w.block * NW * QT, min((w.block + 1) * NW * QT, a.q_tiles)) *
+                               row_norm(a.kn + (long long)z * a.k_tiles, w.first * SUB, last * SUB) * c <= BOUND) {
+#pragma unroll
+        for (int t = 0; t < QT; ++t) m[t] = 0.f;
+        for (; step < whole; ++step) run(yes, no, step);
+        if (step < last) run(yes, yes, step);
+    } else {
+        for (; step < whole; ++step) run(no, no, step);
+        if (step < last) run(no, yes, step);
     }
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
@@ -749,12 +821,11 @@ template <class E> __device__ __forceinline__ float ds_scale(const unsigned *ama
     return __uint_as_float((unsigned)(127 + k) << 23);
 }
 
-template <class T, int KS, int QT, int TK, int NW>
+template <class T, int KS, int QT, int NW>
 __global__ __launch_bounds__(64 * NW, (NW == 4 ? dq_per_cu<Frag<T>::NP, KS, QT>() : 1)) void xa_dq_kernel(TileArgs a) {
     using E = typename Frag<T>::E;
     using v8 = typename Vec<E>::v8;
-    constexpr int NP = Frag<T>::NP, DB = (KS + 1) / 2, SUB = TK / 32;
-    constexpr int RC = SUB * KS * NP, TC = SUB * DB * 2 * NP;
+    constexpr int NP = Frag<T>::NP, DB = (KS + 1) / 2, TK = DQ_KEYS, RC = KS * NP, TC = DB * 2 * NP;
     __shared__ __attribute__((aligned(1024))) char lds[2][(2 * RC + TC) * 1024];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, half = lane >> 5;
     const int worker = die_order(blockIdx.x, gridDim.x);
@@ -767,7 +838,7 @@ __global__ __launch_bounds__(64 * NW, (NW == 4 ? dq_per_cu<Frag<T>::NP, KS, QT>(
 
     v8 q[QT][KS][NP], g[QT][KS][NP];
     f32x16 dq[QT][DB];
-    float lse[QT], D[QT];
+    float lse[QT], D[QT];                              // negated
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
         const long long tile = (long long)z * a.q_tiles + (q0 + t < a.q_tiles ? q0 + t : a.q_tiles - 1);
@@ -790,48 +861,58 @@ __global__ __launch_bounds__(64 * NW, (NW == 4 ? dq_per_cu<Frag<T>::NP, KS, QT>(
                                                                                      : Tz + ((long long)step * TC + i - 2 * RC) * 1024,
                        to + i * 1024, lane);
     };
-    __syncthreads();                                   // the last piece's tiles have been read
-    if (first < last) fetch(first);
-    for (int step = first; step < last; ++step) {
+    auto run = [&](auto tail, int step) {
+        constexpr bool TAIL = decltype(tail)::value;
         wait_loads_and_barrier();
         if (step + 1 < last) fetch(step + 1);
         const char *K = lds[step & 1], *V = K + RC * 1024, *KT = V + RC * 1024;
+        f32x16 s[QT], dp[QT];
 #pragma unroll
-        for (int u = 0; u < SUB; ++u)
+        for (int t = 0; t < QT; ++t) s[t] = (f32x16)0.f, dp[t] = (f32x16)D[t];
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+            v8 f[NP];
+            read_frag<E, NP>(K + k * NP * 1024, lane, f);
+#pragma unroll
+            for (int t = 0; t < QT; ++t) s[t] = mfma_pieces<E, NP>(f, q[t][k], s[t]);
+            read_frag<E, NP>(V + k * NP * 1024, lane, f);
+#pragma unroll
+            for (int t = 0; t < QT; ++t) dp[t] = mfma_pieces<E, NP>(f, g[t][k], dp[t]);
+        }
+        if constexpr (TAIL)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                if (step * TK + 8 * (r / 4) + 4 * half + r % 4 >= n)
+#pragma unroll
+                    for (int t = 0; t < QT; ++t) s[t][r] = -INFINITY, dp[t][r] = 0.f;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            v8 f[QT][NP];
 #pragma unroll
             for (int t = 0; t < QT; ++t) {
-                f32x16 s = (f32x16)0.f, dp = (f32x16)(-D[t]);
+                float ds[8];
 #pragma unroll
-                for (int k = 0; k < KS; ++k) {
-                    v8 f[NP];
-                    read_frag<E, NP>(K + (u * KS + k) * NP * 1024, lane, f);
-                    s = mfma_pieces<E, NP>(f, q[t][k], s);
-                    read_frag<E, NP>(V + (u * KS + k) * NP * 1024, lane, f);
-                    dp = mfma_pieces<E, NP>(f, g[t][k], dp);
+                for (int e = 0; e < 8; ++e) {
+                    ds[e] = __builtin_amdgcn_exp2f(fmaf(s[t][8 * h + e], a.c, lse[t])) * dp[t][8 * h + e];
+                    if constexpr (Shift<E>::bwd != 0.f) ds[e] *= up;
                 }
-                if (step * TK + TK > n)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r)
-                        if (step * TK + u * 32 + 8 * (r / 4) + 4 * half + r % 4 >= n) s[r] = -INFINITY, dp[r] = 0.f;
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    float ds[8];
-                    v8 f[NP];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        ds[e] = __builtin_amdgcn_exp2f(fmaf(s[8 * h + e], a.c, -lse[t])) * dp[8 * h + e];
-                        if constexpr (Shift<E>::bwd != 0.f) ds[e] *= up;
-                    }
-                    split8<E, NP>(ds, f);
-#pragma unroll
-                    for (int b = 0; b < DB; ++b) {
-                        v8 w[NP];
-                        read_frag<E, NP>(KT + ((u * DB + b) * 2 + h) * NP * 1024, lane, w);
-                        dq[t][b] = mfma_pieces<E, NP>(w, f, dq[t][b]);
-                    }
-                }
+                split8<E, NP>(ds, f[t]);
             }
-    }
+#pragma unroll
+            for (int b = 0; b < DB; ++b) {
+                v8 x[NP];
+                read_frag<E, NP>(KT + (b * 2 + h) * NP * 1024, lane, x);
+#pragma unroll
+                for (int t = 0; t < QT; ++t) dq[t][b] = mfma_pieces<E, NP>(x, f[t], dq[t][b]);
+            }
+        }
+    };
+    __syncthreads();                                   // the last piece's tiles have been read
+    if (first < last) fetch(first);
+    const int whole = min(last, n / TK);               // steps without rows behind the last key
+    int step = first;
+    for (; step < whole; ++step) run(std::false_type(), step);
+    if (step < last) run(std::true_type(), step);
     const float back = a.scale / up;
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
@@ -843,7 +924,7 @@ __global__ __launch_bounds__(64 * NW, (NW == 4 ? dq_per_cu<Frag<T>::NP, KS, QT>(
 }
 
 // 32 KT keys per wave, steps of 32 queries
-template <class T, int KS, int KT>
+template <class T, int KS>
 struct DkvLds {
     static constexpr int NP = Frag<T>::NP, DB = (KS + 1) / 2, CHUNKS = 2 * KS * NP + 4 * DB * NP + 1;
     static constexpr int BUFFERS = CHUNKS <= 80 ? 2 : 1;
@@ -853,7 +934,7 @@ template <class T, int KS, int KT, int NW>
 __global__ __launch_bounds__(64 * NW, (NW == 4 ? dkv_per_cu<Frag<T>::NP, KS>() : 1)) void xa_dkv_kernel(TileArgs a) {
     using E = typename Frag<T>::E;
     using v8 = typename Vec<E>::v8;
-    using L = DkvLds<T, KS, KT>;
+    using L = DkvLds<T, KS>;
     constexpr int NP = L::NP, DB = L::DB, RC = KS * NP, TC = DB * 2 * NP, NB = L::BUFFERS;
     extern __shared__ __attribute__((aligned(1024))) char lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, half = lane >> 5;
@@ -885,7 +966,7 @@ __global__ __launch_bounds__(64 * NW, (NW == 4 ? dkv_per_cu<Frag<T>::NP, KS>() :
         for (int i = wave; i < L::CHUNKS; i += NW) {
             const char *from = i < RC ? a.Qr + (tile * RC + i) * 1024 : i < 2 * RC ? a.Gr + (tile * RC + i - RC) * 1024
                              : i < 2 * RC + TC ? a.Qt + (tile * TC + i - 2 * RC) * 1024
-                             : i < 2 * RC + 2 * TC ? a.Gt + (tile * TC + i - 2 * RC - TC) * 1024 : a.stat + tile * 1024;
+                             : i < 2 * (RC + TC) ? a.Gt + (tile * TC + i - 2 * RC - TC) * 1024 : a.stat + tile * 1024;
             load_chunk(from, to + i * 1024, lane);
         }
     };
@@ -896,46 +977,63 @@ __global__ __launch_bounds__(64 * NW, (NW == 4 ? dkv_per_cu<Frag<T>::NP, KS>() :
         if (NB == 2 && step + 1 < last) fetch(step + 1);
         const char *Q = lds + (NB == 2 ? (step & 1) * L::CHUNKS * 1024 : 0), *G = Q + RC * 1024, *QT = G + RC * 1024, *GT = QT + TC * 1024;
         const float *st = (const float *)(GT + TC * 1024);
+        f32x16 s[KT], dp[KT];
+        float lse[16];                                      // -lse
 #pragma unroll
-        for (int t = 0; t < KT; ++t) {
-            f32x16 s = (f32x16)0.f, dp;
-            float lse[16];
+        for (int r = 0; r < 16; ++r) {
+            lse[r] = st[8 * (r / 4) + 4 * half + r % 4];
+            if constexpr (Shift<E>::bwd != 0.f) lse[r] += Shift<E>::bwd;
+        }
+        auto scores = [&](int t) {
+            s[t] = (f32x16)0.f;
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                lse[r] = st[8 * (r / 4) + 4 * half + r % 4];
-                dp[r] = -st[32 + 8 * (r / 4) + 4 * half + r % 4];
-            }
+            for (int r = 0; r < 16; ++r) dp[t][r] = st[32 + 8 * (r / 4) + 4 * half + r % 4];    // -D
 #pragma unroll
             for (int k = 0; k < KS; ++k) {
                 v8 f[NP];
                 read_frag<E, NP>(Q + k * NP * 1024, lane, f);
-                s = mfma_pieces<E, NP>(f, kf[t][k], s);
+                s[t] = mfma_pieces<E, NP>(f, kf[t][k], s[t]);
                 read_frag<E, NP>(G + k * NP * 1024, lane, f);
-                dp = mfma_pieces<E, NP>(f, vf[t][k], dp);
+                dp[t] = mfma_pieces<E, NP>(f, vf[t][k], dp[t]);
             }
+        };
+        scores(0);
+#pragma unroll
+        for (int t = 0; t < KT; ++t) {
+            // the next tile's products and this one's fragments are under way while the exponentials run
+            constexpr bool EARLY = DB * NP <= 2 && KT > 1;           // (registers)
+            v8 gf[2][DB][NP], qf[2][DB][NP];
+            if constexpr (EARLY)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int b = 0; b < DB; ++b) {
+                    read_frag<E, NP>(GT + (b * 2 + h) * NP * 1024, lane, gf[h][b]);
+                    read_frag<E, NP>(QT + (b * 2 + h) * NP * 1024, lane, qf[h][b]);
+                }
+            if (t + 1 < KT) scores(t + 1);
+            if constexpr (EARLY) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 float p[8], ds[8];
                 v8 f[NP];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    p[e] = __builtin_amdgcn_exp2f(fmaf(s[8 * h + e], a.c, Shift<E>::bwd - lse[8 * h + e]));
-                    ds[e] = p[e] * dp[8 * h + e];
+                    p[e] = __builtin_amdgcn_exp2f(fmaf(s[t][8 * h + e], a.c, lse[8 * h + e]));
+                    ds[e] = p[e] * dp[t][8 * h + e];
                     if constexpr (Shift<E>::bwd != 0.f) ds[e] *= up * (1.f / 32768.f);
                 }
                 split8<E, NP>(p, f);
 #pragma unroll
                 for (int b = 0; b < DB; ++b) {
-                    v8 w[NP];
-                    read_frag<E, NP>(GT + (b * 2 + h) * NP * 1024, lane, w);
-                    dv[t][b] = mfma_pieces<E, NP>(w, f, dv[t][b]);
+                    if constexpr (!EARLY) read_frag<E, NP>(GT + (b * 2 + h) * NP * 1024, lane, gf[h][b]);
+                    dv[t][b] = mfma_pieces<E, NP>(gf[h][b], f, dv[t][b]);
                 }
                 split8<E, NP>(ds, f);
 #pragma unroll
                 for (int b = 0; b < DB; ++b) {
-                    v8 w[NP];
-                    read_frag<E, NP>(QT + (b * 2 + h) * NP * 1024, lane, w);
-                    dk[t][b] = mfma_pieces<E, NP>(w, f, dk[t][b]);
+                    if constexpr (!EARLY) read_frag<E, NP>(QT + (b * 2 + h) * NP * 1024, lane, qf[h][b]);
+                    dk[t][b] = mfma_pieces<E, NP>(qf[h][b], f, dk[t][b]);
                 }
             }
         }
@@ -1142,7 +1240,7 @@ struct Plan {
     bool few;
     int splits;                                   // few rows: of the keys
     Tiles fwd, dq, dkv;
-    size_t idx, cnt, Qr, Kr, Vt, Qt, Kt, Vr, Gr, Gt, stat, amax, part, ml, bytes;
+    size_t idx, cnt, qn, kn, Qr, Kr, Vt, Qt, Kt, Vr, Gr, Gt, stat, amax, part, ml, bytes;
 };
 
 // Workgroups that the chip holds at once, so that they all run to the end together -- unless that left them fewer than `least` steps: then one block of rows
@@ -1169,7 +1267,7 @@ template <int NP, int KS> Plan plan_of(const md_attn_desc &a, bool backward) {
     p.NP = NP;
     p.DB = (KS + 1) / 2;
     p.q_tiles = (p.M + 31) / 32;
-    p.k_tiles = (a.Nk + 63) / 64 * 2;
+    p.k_tiles = (a.Nk + 127) / 128 * 4;                       // whole steps of every kernel
     p.few = !backward && p.M <= FEW_ROWS;
     size_t at = 0;
     auto take = [&](size_t n) { const size_t r = at; at = align256(at + n); return r; };
@@ -1196,9 +1294,11 @@ template <int NP, int KS> Plan plan_of(const md_attn_desc &a, bool backward) {
     p.Qr = take(qR);
     p.Kr = take(kR);
     if (!backward) {
-        const int tk = p.NP == 3 && p.KS > 2 ? 32 : 64;
+        const int tk = fwd_keys<NP, KS>();
         p.Vt = take(kT);
-        p.fwd = tiles_for(p.Z, p.q_tiles, qt, tk, (a.Nk + tk - 1) / tk, 4, qt == 2 ? fwd_per_cu<NP, KS, 2>() : fwd_per_cu<NP, KS, 1>(), masked);
+        p.qn = take((size_t)p.Z * p.q_tiles * 4);
+        p.kn = take((size_t)p.Z * p.k_tiles * 4);
+        p.fwd = tiles_for(p.Z, p.q_tiles, qt, tk, (a.Nk + tk - 1) / tk, 256 / tk, qt == 2 ? fwd_per_cu<NP, KS, 2>() : fwd_per_cu<NP, KS, 1>(), masked);
         if (p.fwd.join) {
             p.fwd.part = take((size_t)2 * p.fwd.workers * p.fwd.rows * p.DB * 32 * 4);
             p.fwd.ml = take((size_t)2 * p.fwd.workers * p.fwd.rows * 8);
@@ -1212,8 +1312,8 @@ template <int NP, int KS> Plan plan_of(const md_attn_desc &a, bool backward) {
         p.Gt = take(qT);
         p.stat = take((size_t)p.Z * p.q_tiles * kb);
         p.amax = take(256);
-        p.dq = tiles_for(p.Z, p.q_tiles, qt, 32, (a.Nk + 31) / 32, 8, qt == 2 ? dq_per_cu<NP, KS, 2>() : dq_per_cu<NP, KS, 1>(), masked);
-        p.dkv = tiles_for(p.Z, (a.Nk + 31) / 32, 1, 0, p.q_tiles, 8, dkv_per_cu<NP, KS>(), masked);
+        p.dq = tiles_for(p.Z, p.q_tiles, qt, DQ_KEYS, (a.Nk + DQ_KEYS - 1) / DQ_KEYS, 256 / DQ_KEYS, qt == 2 ? dq_per_cu<NP, KS, 2>() : dq_per_cu<NP, KS, 1>(), masked);
+        p.dkv = tiles_for(p.Z, (a.Nk + 31) / 32, key_tiles<NP, KS>(), 0, p.q_tiles, 8, dkv_per_cu<NP, KS>(), masked);
         const size_t nq = p.dq.join ? (size_t)2 * p.dq.workers * p.dq.rows * p.DB * 32 * 4 : 0, nk = p.dkv.join ? (size_t)2 * p.dkv.workers * p.dkv.rows * p.DB * 32 * 4 : 0;
         p.dq.part = p.dkv.part = take(std::max(nq, nk));            // dq's are summed before dk's are written (and `first` likewise)
         p.dkv.part2 = take(nk);
@@ -1289,9 +1389,9 @@ int start(const md_attn_desc &a, const Plan &p, char *ws, hipStream_t s, Shape &
     return MD_OK;
 }
 
-PackJob job_of(const void *x, long long sb, long long sn, long long sh, size_t size, int d, char *R, char *T, int tiles, int query, float sign) {
+PackJob job_of(const void *x, long long sb, long long sn, long long sh, size_t size, int d, char *R, char *T, int tiles, int query, float factor) {
     PackJob j{};
-    j.x = x, j.sb = sb, j.sn = sn, j.sh = sh, j.R = R, j.T = T, j.tiles = tiles, j.query = query, j.sign = sign;
+    j.x = x, j.sb = sb, j.sn = sn, j.sh = sh, j.R = R, j.T = T, j.tiles = tiles, j.query = query, j.factor = factor;
     j.vec = aligned_rows(x, size, d, sb, sn, sh);
     return j;
 }
@@ -1320,15 +1420,18 @@ TileArgs tile_args(const Shape &sh, const Plan &p, const Tiles &w, char *ws) {
 }
 
 template <class T, int KS> int run_fwd(const md_attn_desc &a, const Plan &p, const Shape &sh, char *ws, hipStream_t s) {
-    constexpr int NP = Frag<T>::NP, TK = NP == 3 && KS > 2 ? 32 : 64;
-    const float sign = a.scale < 0.f ? -1.f : 1.f;          // c > 0 in the kernels: a negative scale goes into q's sign
+    constexpr int NP = Frag<T>::NP, TK = fwd_keys<NP, KS>();
+    // c > 0 in the kernels: a negative scale goes into q's sign.  In float32 q takes all of it (2^-24 like every other product of the sums)
+    const float factor = NP == 3 ? a.scale * LOG2E : a.scale < 0.f ? -1.f : 1.f;
     PackArgs k{};
     k.s = sh, k.jobs = 3;
-    k.job[0] = job_of(a.q, a.q_sb, a.q_sn, a.q_sh, sizeof(T), a.d, ws + p.Qr, nullptr, p.q_tiles, 1, sign);
+    k.job[0] = job_of(a.q, a.q_sb, a.q_sn, a.q_sh, sizeof(T), a.d, ws + p.Qr, nullptr, p.q_tiles, 1, factor);
     k.job[1] = job_of(a.k, a.k_sb, a.k_sn, a.k_sh, sizeof(T), a.d, ws + p.Kr, nullptr, p.k_tiles, 0, 1.f);
     k.job[2] = job_of(a.v, a.v_sb, a.v_sn, a.v_sh, sizeof(T), a.d, nullptr, ws + p.Vt, p.k_tiles, 0, 1.f);
+    k.job[0].norm = (float *)(ws + p.qn), k.job[1].norm = (float *)(ws + p.kn);
     if (int rc = launch_pack<T, KS>(k, p, 0, s)) return rc;
     TileArgs t = tile_args(sh, p, p.fwd, ws);
+    t.qn = (float *)(ws + p.qn), t.kn = (float *)(ws + p.kn);
     t.Qr = ws + p.Qr, t.Kr = ws + p.Kr, t.Vt = ws + p.Vt;
     t.c = fmaxf(fabsf(a.scale) * LOG2E, 1.2e-38f);         // not 0: the scores of rows behind the last key are -inf
     t.o = a.o, t.lse = a.lse;
@@ -1382,12 +1485,12 @@ template <class T, int KS> int run_bwd(const md_attn_desc &a, const Plan &p, con
         TileArgs t = args(p.dq);
         t.scale = a.scale;
         const unsigned grid = grid8(t.workers);
-        if (p.dq.nw == 1) xa_dq_kernel<T, KS, 1, 32, 1><<<grid, 64, 0, s>>>(t);
+        if (p.dq.nw == 1) xa_dq_kernel<T, KS, 1, 1><<<grid, 64, 0, s>>>(t);
         else if constexpr (query_tiles<NP, KS>() == 2) {
-            if (p.dq.t == 2) xa_dq_kernel<T, KS, 2, 32, 4><<<grid, 256, 0, s>>>(t);
-            else xa_dq_kernel<T, KS, 1, 32, 4><<<grid, 256, 0, s>>>(t);
+            if (p.dq.t == 2) xa_dq_kernel<T, KS, 2, 4><<<grid, 256, 0, s>>>(t);
+            else xa_dq_kernel<T, KS, 1, 4><<<grid, 256, 0, s>>>(t);
         } else
-            xa_dq_kernel<T, KS, 1, 32, 4><<<grid, 256, 0, s>>>(t);
+            xa_dq_kernel<T, KS, 1, 4><<<grid, 256, 0, s>>>(t);
         MD_CHECK_LAUNCH("md_cross_attn_bwd: dq");
         if (p.dq.join) {
             xa_sum_kernel<T, (KS + 1) / 2><<<dim3(t.workers, t.rows / 32), 256, 0, s>>>(t);
@@ -1398,14 +1501,15 @@ template <class T, int KS> int run_bwd(const md_attn_desc &a, const Plan &p, con
         TileArgs t = args(p.dkv);
         t.scale = fabsf(a.scale);                          // Q's fragments carry the sign
         const unsigned grid = grid8(t.workers);
-        using L = DkvLds<T, KS, 1>;
+        using L = DkvLds<T, KS>;
         const int lds = L::BUFFERS * L::CHUNKS * 1024;
         if (p.dkv.nw == 1) {
             if (int rc = set_lds(xa_dkv_kernel<T, KS, 1, 1>, lds)) return rc;
             xa_dkv_kernel<T, KS, 1, 1><<<grid, 64, lds, s>>>(t);
         } else {
-            if (int rc = set_lds(xa_dkv_kernel<T, KS, 1, 4>, lds)) return rc;
-            xa_dkv_kernel<T, KS, 1, 4><<<grid, 256, lds, s>>>(t);
+            constexpr int KT = key_tiles<NP, KS>();
+            if (int rc = set_lds(xa_dkv_kernel<T, KS, KT, 4>, lds)) return rc;
+            xa_dkv_kernel<T, KS, KT, 4><<<grid, 256, lds, s>>>(t);
         }
         MD_CHECK_LAUNCH("md_cross_attn_bwd: dk, dv");
         if (p.dkv.join) {
