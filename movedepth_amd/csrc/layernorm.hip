@@ -48,15 +48,23 @@ __global__ __launch_bounds__(256) void ln_fwd_kernel(const T *__restrict__ x, lo
         }
     const float inv = 1.f / (float)C;
     const int groups = (C + MD_ACT8_GROUP - 1) / MD_ACT8_GROUP;
-    // every lane runs the same rounds: sums cross lanes
-    for (long long at = (long long)blockIdx.x * RPB; at < rows; at += (long long)gridDim.x * RPB) {
+    // every lane runs the same rounds: sums cross lanes.  The next row is on its way while this one is summed and stored
+    const long long step = (long long)gridDim.x * RPB;
+    md_u32x4 next[NV];
+    auto fetch = [&](long long row) {
+        const T *xr = x + (row < rows ? row : 0) * ldx;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) next[i] = md_load_raw<T>(xr, (i * TPR + sub) * W, C);
+    };
+    fetch((long long)blockIdx.x * RPB + threadIdx.x / TPR);
+    for (long long at = (long long)blockIdx.x * RPB; at < rows; at += step) {
         const long long row = at + threadIdx.x / TPR;
         const bool live = row < rows;
-        const T *xr = x + (live ? row : 0) * ldx;
         float v[NV][W];
         float s = 0.f;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) md_load_wide<T>(xr, (i * TPR + sub) * W, C, v[i]);
+        for (int i = 0; i < NV; ++i) md_floats<T>(next[i], v[i]);
+        if (at + step < rows) fetch(row + step);
         if constexpr (ACT8)
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
@@ -330,7 +338,9 @@ Split split_of(int wide) {
     return {0, 0};                                 // too long for registers
 }
 int pieces(int dtype, int C) { return md_cdiv(C, 16 / (int)md_dtype_bytes(dtype)); }
-int fwd_blocks(long long rows, int tpr) { return (int)std::min<long long>(md_cdiv(rows, 256 / tpr), 8 * CUS); }
+// workgroups of the forward pass: w and b are read once per workgroup, so no more than keep the loads in flight (32768 x 2048 bf16: 79 us with 8 a CU, 56 with 2;
+// 122880 x 64: 16.6 us with 2, 13.1 with 4)
+int fwd_blocks(long long rows, Split s) { return (int)std::min<long long>(md_cdiv(rows, 256 / s.tpr), (s.nv == 1 ? 4 : 2) * CUS); }
 // workgroups of the backward pass: each leaves 2 C partial sums, so no more than the chip needs to stream
 int bwd_blocks(long long rows, int tpr) { return (int)std::min<long long>(md_cdiv(rows, 256 / tpr), 2 * CUS); }
 int column_slices(long long rows) { return (int)std::min<long long>(rows, 64); }
@@ -369,7 +379,7 @@ extern "C" int md_layer_norm_fwd(const void *x, int dtype, long long rows, int C
         MD_DISPATCH_DTYPE(dtype, "md_layer_norm_fwd",
                           ln_long_fwd_kernel<T><<<(unsigned)rows, LONG, 0, s>>>((const T *)x, ldx, w, b, C, eps, (T *)y, stat, cd, sc));
     } else {
-        const int grid = fwd_blocks(rows, sp.tpr);
+        const int grid = fwd_blocks(rows, sp);
         MD_DISPATCH_DTYPE(dtype, "md_layer_norm_fwd", LN_CONFIG(sp, {
             if (codes) ln_fwd_kernel<T, TPR, NV, true><<<grid, 256, 0, s>>>((const T *)x, ldx, w, b, (int)rows, C, eps, (T *)y, stat, cd, sc);
             else ln_fwd_kernel<T, TPR, NV, false><<<grid, 256, 0, s>>>((const T *)x, ldx, w, b, (int)rows, C, eps, (T *)y, stat, cd, sc);

@@ -63,19 +63,25 @@ template <class T> struct Wide {
     struct __attribute__((packed, aligned(1))) Codes { unsigned char b[n]; };
 };
 
-// elements at .. at + n - 1 of a row of `len`, zeros behind its end
-template <class T> __device__ __forceinline__ void md_load_wide(const T *row, int at, int len, float (&v)[Wide<T>::n]) {
+// elements at .. at + n - 1 of a row of `len`, zeros behind its end; as they are in memory, and as floats
+template <class T> __device__ __forceinline__ md_u32x4 md_load_raw(const T *row, int at, int len) {
     constexpr int n = Wide<T>::n;
+    if (at + n <= len) return ((const typename Wide<T>::Mem *)(row + at))->v;
     T raw[n];
-    if (at + n <= len) {
-        const md_u32x4 w = ((const typename Wide<T>::Mem *)(row + at))->v;
-        __builtin_memcpy(raw, &w, 16);
-    } else {
 #pragma unroll
-        for (int j = 0; j < n; ++j) raw[j] = at + j < len ? row[at + j] : (T)0.f;
-    }
+    for (int j = 0; j < n; ++j) raw[j] = at + j < len ? row[at + j] : (T)0.f;
+    md_u32x4 w;
+    __builtin_memcpy(&w, raw, 16);
+    return w;
+}
+template <class T> __device__ __forceinline__ void md_floats(md_u32x4 w, float (&v)[Wide<T>::n]) {
+    T raw[Wide<T>::n];
+    __builtin_memcpy(raw, &w, 16);
 #pragma unroll
-    for (int j = 0; j < n; ++j) v[j] = (float)raw[j];
+    for (int j = 0; j < Wide<T>::n; ++j) v[j] = (float)raw[j];
+}
+template <class T> __device__ __forceinline__ void md_load_wide(const T *row, int at, int len, float (&v)[Wide<T>::n]) {
+    md_floats<T>(md_load_raw<T>(row, at, len), v);
 }
 template <class T> __device__ __forceinline__ void md_store_wide(T *row, int at, int len, const float (&v)[Wide<T>::n]) {
     constexpr int n = Wide<T>::n;

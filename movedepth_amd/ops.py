@@ -1484,7 +1484,7 @@ _NO_GUARD = contextlib.nullcontext()
 
 def _on(device):
     """context in which launches go to `device`; nothing to enter (and nothing to pay for) where it is current already"""
-    return _NO_GUARD if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+    return _NO_GUARD if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
 
 
 def _stream_of(device):
@@ -1566,7 +1566,8 @@ def saved_act8(min_numel=1 << 20):
 # --------------------------------------------------------------------------- layer norm
 def _rows(t, C):
     """(..., C) -> ((rows, C) tensor with contiguous columns, row stride); a copy only if the rows are not evenly spaced already"""
-    t = t.reshape(-1, C)
+    if t.dim() != 2:
+        t = t.reshape(-1, C)
     if (C > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < C):
         t = t.contiguous()
     return t, (t.stride(0) if t.shape[0] > 1 else C)
@@ -1580,7 +1581,7 @@ def _layer_norm_fwd(x, weight, bias, eps, act_bits, keep):
     with _on(dev):
         x2, ldx = _rows(x, C)
         rows = x2.shape[0]
-        y = torch.empty(x.shape, device=dev, dtype=x.dtype)
+        y = torch.empty_like(x, memory_format=torch.contiguous_format)
         stat = codes = scales = None
         if keep:
             stat = torch.empty(rows, 2, device=dev, dtype=torch.float32)
@@ -1614,7 +1615,7 @@ class _LayerNorm(torch.autograd.Function):
             rows = gy.numel() // C
             ldx = C if x2 is None or rows <= 1 else x2.stride(0)
             need_x, need_w, need_b = ctx.needs_input_grad[:3]
-            dx = torch.empty(gy.shape, device=dev, dtype=dtype) if need_x else None
+            dx = torch.empty_like(gy, memory_format=torch.contiguous_format) if need_x else None
             dw = torch.empty(C, device=dev, dtype=torch.float32) if need_w else None
             db = torch.empty(C, device=dev, dtype=torch.float32) if need_b else None
             nbytes = _lib.load().md_layer_norm_bwd_ws_bytes(rows, C) if need_w or need_b else 0
