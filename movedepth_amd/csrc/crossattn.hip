@@ -657,10 +657,16 @@ struct Joint {
         const bool same = last.x == me.x && last.y == me.y;
         if (same && last.z > 0) return false;
         z = me.x, block = me.y, from = worker - 1, tail = !same;
-        for (to = worker + 1; to < a.workers; ++to) {
-            const int4 next = a.first[to];
-            if (next.x != z || next.y != block || next.z == 0) break;
+        for (to = worker + 1; to < a.workers; to += 64) {              // 64 notes at a time; every lane calls this
+            const int i = to + (threadIdx.x & 63);
+            const int4 next = a.first[i < a.workers ? i : worker];
+            const unsigned long long other = __ballot(i >= a.workers || next.x != z || next.y != block || next.z == 0);
+            if (other) {
+                to += __ffsll(other) - 1;
+                break;
+            }
         }
+        to = min(to, a.workers);
         return true;
     }
     __device__ __forceinline__ int slot(int i) const { return 2 * i + (tail && i == from ? 1 : 0); }
@@ -1217,6 +1223,7 @@ int check(const md_attn_desc &a, const char *what) {
     MD_REQUIRE(a.d >= 1 && a.d <= MD_ATTN_MAX_D, "%s: head size %d (1 .. %d)", what, a.d, MD_ATTN_MAX_D);
     MD_REQUIRE(a.Hk >= 1 && a.Hq >= 1 && a.Hq % a.Hk == 0, "%s: %d query heads are not a multiple of %d key heads", what, a.Hq, a.Hk);
     MD_REQUIRE(a.Hq <= 65535 && a.B <= 65535, "%s: more than 65535 heads or sequences", what);
+    MD_REQUIRE((long long)a.B * a.Hq < (1LL << 31) - 65536, "%s: 2^31 heads of sequences or more", what);
     MD_REQUIRE((long long)a.B * a.Hq * a.Nq < (1LL << 31) - 65536 && (long long)a.B * a.Hk * a.Nk < (1LL << 31) - 65536 &&
                    a.Nk < (1 << 30) && (long long)a.Hq / a.Hk * a.Nq < (1 << 30),
                "%s: 2^31 rows or more", what);

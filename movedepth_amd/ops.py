@@ -1553,7 +1553,8 @@ def saved_act8(min_numel=1 << 20):
     carry the rounding of the kept activations; the forward pass does not change."""
 
     def pack(t):
-        if t.is_cuda and t.dtype in _TOKEN_DTYPE and t.numel() >= min_numel and not (t.is_leaf and t.requires_grad) and _is_dense(t):
+        if (t.is_cuda and t.dtype in _TOKEN_DTYPE and t.numel() >= min_numel and t.layout is torch.strided
+                and not (t.is_leaf and t.requires_grad) and _is_dense(t)):
             return act8_pack(t)
         return t
 

@@ -386,6 +386,44 @@ def test_cross_attention_refusals():
             ops.cross_attention(q, k, k, key_mask=m)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("B,Nq,Nk,Hq,Hk,d", [(1, 12, 9000, 1, 1, 32), (2, 5, 5000, 4, 2, 64), (1, 3000, 40, 2, 1, 16), (3, 33, 1200, 1, 1, 128)])
+def test_cross_attention_long_axes(B, Nq, Nk, Hq, Hk, d, dtype):
+    """few rows against many: the work of a block of rows is spread over many workgroups and joined"""
+    attention_case(B, Nq, Nk, Hq, Hk, d, dtype, "none")
+    attention_case(B, Nq, Nk, Hq, Hk, d, dtype, "tail")
+
+
+@pytest.mark.parametrize("size", [1e-4, 1.0, 300.0])
+def test_cross_attention_float16_gradient_sizes(size):
+    """gradients far below and above 1: dS of a long row would fall below float16's range, or above it.  Relative to the largest: the scaled dS keeps 2^-25 of
+    2^15 / (2 |g| |v|), so what is lost is below 2^-40 of |g| |v| per key, under the bound's own terms; the results themselves must fit the type"""
+    g = gen(40)
+    q, k, v = randn(g, 1, 70, 2, 32, dtype=torch.float16), randn(g, 1, 400, 2, 32, dtype=torch.float16), randn(g, 1, 400, 2, 32, dtype=torch.float16)
+    go = randn(g, 1, 70, 2, 32, dtype=torch.float16, scale=size)
+    got = run_attention(q, k, v, None, 0.2, go)
+    check(got, ref.cross_attention(q, k, v, None, 0.2, go), "gradient of size %g" % size)
+    if size < 1:                # 1024 times the gradient gives 1024 times the gradients, but for the small ones' own last step
+        big = run_attention(q, k, v, None, 0.2, go * 1024)
+        for name in ("dq", "dk", "dv"):
+            a, b = got[name].double() * 1024, big[name].double()
+            assert bool(((a - b).abs() <= 1024 * ref.tiny_of(torch.float16) + 2 * ref.u_of(torch.float16) * b.abs()).all()), name
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_cross_attention_where_the_norms_bound_the_scores_and_where_not(dtype):
+    """rows and keys of very different sizes in one call: some blocks of rows run without a running maximum, some with, and parts of both are joined"""
+    g, dt = gen(41), DT[dtype]
+    q = randn(g, 1, 400, 1, 32) * torch.where(torch.arange(400) < 200, 0.3, 12.0)[None, :, None, None].cuda()
+    k = randn(g, 1, 2000, 1, 32) * torch.where(torch.arange(2000) < 900, 0.5, 4.0)[None, :, None, None].cuda()
+    v, go = randn(g, 1, 2000, 1, 32, dtype=dt), randn(g, 1, 400, 1, 32, dtype=dt)
+    q, k = q.to(dt), k.to(dt)
+    check(run_attention(q, k, v, None, 0.4, go), ref.cross_attention(q, k, v, None, 0.4, go), "mixed norms")
+    k = -k.abs()                                            # every score far below 0
+    q = q.abs()
+    check(run_attention(q, k, v, None, 0.4, go), ref.cross_attention(q, k, v, None, 0.4, go), "low scores")
+
+
 @pytest.mark.parametrize("Nq", [1, 40])
 def test_cross_attention_offsets_beyond_32_bits(Nq):
     """rows of a cache whose last offset passes 2^32 elements"""
@@ -437,13 +475,13 @@ def test_gradients_against_differences(op):
         assert abs(want - d1) <= abs(d2 - d1) + 3 * noise + 1e-4 * abs(d1), "%s input %d: %.6g, by differences %.6g" % (op, i, want, d1)
 
 
-def operators(g, dt=torch.bfloat16):
+def operators(g, dt=torch.bfloat16, d=32):
     """closures that make every kernel of the operators run once on fixed inputs -> (inputs, function of them)"""
     from movedepth_amd import ops
 
     x, w, b, gx = randn(g, 300, 96, dtype=dt), randn(g, 96), randn(g, 96), randn(g, 300, 96, dtype=dt)
-    q, k, v, go = randn(g, 2, 140, 4, 32, dtype=dt), randn(g, 2, 210, 2, 32, dtype=dt), randn(g, 2, 210, 2, 32, dtype=dt), randn(g, 2, 140, 4, 32, dtype=dt)
-    q1 = randn(g, 2, 1, 4, 32, dtype=dt)
+    q, k, v, go = randn(g, 2, 140, 4, d, dtype=dt), randn(g, 2, 210, 2, d, dtype=dt), randn(g, 2, 210, 2, d, dtype=dt), randn(g, 2, 140, 4, d, dtype=dt)
+    q1 = randn(g, 2, 1, 4, d, dtype=dt)
     mask = make_mask("random", 2, 210, g)
 
     def f(x, w, b, gx, q, k, v, go, q1):
@@ -482,9 +520,10 @@ def test_another_stream():
     assert all(torch.equal(x, y) and torch.equal(x, z) for x, y, z in zip(want, a, b))
 
 
-def test_captured_graphs():
+@pytest.mark.parametrize("dtype,d", [("bf16", 32), ("f32", 128), ("f16", 64)])
+def test_captured_graphs(dtype, d):
     """two graphs of one memory pool, replayed in turn with new inputs and eager work between"""
-    ins, f = operators(gen(20))
+    ins, f = operators(gen(20), DT[dtype], d)
     s = torch.cuda.Stream()
     s.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(s):
@@ -499,7 +538,7 @@ def test_captured_graphs():
         pool = g.pool()
         graphs.append(g)
     for i in range(4):
-        new, _ = operators(gen(30 + i))
+        new, _ = operators(gen(30 + i), DT[dtype], d)
         for t, n in zip(ins, new):
             t.copy_(n)
         want = [t.clone() for t in f(*ins)]
