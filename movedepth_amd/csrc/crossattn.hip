@@ -436,11 +436,28 @@ struct Walk {
                 const long long per = line.units(a.s.Hk);
                 b = (int)quotient(at, per);
                 at -= per * b;
-            } else
-                for (line = line_of(a, 0); at >= line.units(a.s.Hk); line = line_of(a, b)) {
-                    at -= line.units(a.s.Hk);
-                    ++b;
+            } else {
+                const int lane = threadIdx.x & 63;         // 64 sequences at a time
+                for (;; b += 64) {
+                    long long upto = b + lane < a.s.B ? line_of(a, b + lane).units(a.s.Hk) : 0;
+#pragma unroll
+                    for (int o = 1; o < 64; o <<= 1) {
+                        const long long v = __shfl_up(upto, o);
+                        if (lane >= o) upto += v;
+                    }
+                    const unsigned long long behind = __ballot(upto > at);
+                    if (behind) {
+                        const int i = __ffsll(behind) - 1;
+                        if (i > 0) at -= __shfl(upto, i - 1);
+                        b += i;
+                        break;
+                    }
+                    at -= __shfl(upto, 63);
                 }
+                at = uniform(at);
+                b = __builtin_amdgcn_readfirstlane(b);
+                line = line_of(a, b);
+            }
             const long long per = (long long)line.blocks * line.steps;
             hk = (int)quotient(at, per);
             at -= hk * per;
@@ -1214,7 +1231,9 @@ __global__ __launch_bounds__(256) void xa_few_kernel(FewArgs a) {
 }
 
 // ---------------------------------------------------------------- host side
-constexpr int FEW_ROWS = 8;                  // query rows per key head up to which K and V are read in place
+// Query rows per key head up to which K and V are read in place.  8 rows on 8 x 20480 keys of 4 heads of 64 (bf16): 73 us, through the tiles 129 us, most of it
+// packing; 16 rows would take two such passes (128 us through the tiles).  1 row: 43 us, 3.9 TB/s of K and V
+constexpr int FEW_ROWS = 8;
 constexpr int CUS = 256;
 
 int check(const md_attn_desc &a, const char *what) {

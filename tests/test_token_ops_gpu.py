@@ -654,3 +654,14 @@ def test_evaluation_with_match_attention():
     del t.models["match_attn"]
     c = predict_depth(t.models, data, t.opt, t.vol_layout)["depth_mvs"]
     assert torch.allclose(a, c, rtol=1e-4) and not torch.allclose(b, c, rtol=1e-4) and bool(torch.isfinite(b).all())
+
+
+def test_cross_attention_many_sequences():
+    """more masked sequences than a wave has lanes, of every number of valid keys, some without any"""
+    g = gen(50)
+    q, go = randn(g, 150, 10, 1, 16), randn(g, 150, 10, 1, 16)
+    k, v = randn(g, 150, 70, 1, 16), randn(g, 150, 70, 1, 16)
+    mask = (torch.arange(70)[None, :] < torch.randint(0, 71, (150,), generator=g)[:, None]).cuda()
+    mask[60:70] = False
+    mask[0] = False
+    check(run_attention(q, k, v, mask, 0.25, go), ref.cross_attention(q, k, v, mask, 0.25, go), "many sequences")
