@@ -179,6 +179,8 @@ __global__ __launch_bounds__(1024) void xa_compact_kernel(const unsigned char *_
 }
 
 // ---------------------------------------------------------------- operands into fragment order
+// A wave per tile of 32 rows; bound by memory: 2 x 16 heads of 64, 4096 queries and 8192 keys, bf16, takes 56 us on average
+// of the forward call's launch (168 MB) and the backward call's (285 MB)
 struct PackJob {
     const void *x;
     long long sb, sn, sh;
@@ -513,6 +515,8 @@ __device__ __forceinline__ float row_norm(const float *norm, int from, int to) {
 // Where |q| |k| scale of a piece's rows bounds its scores by 2^48 either way, m is 0 throughout: no maximum, no rescaling, and the step is straight-line code in
 // which the products of one half run beside the exponentials of the other.  P and its sums stay within 2^+-48 times the row length then (bf16 has
 // float32's exponents; float16 has not and always takes the running maximum).
+// 2 x 2 x 20480^2 heads of 32, bf16: 351 us (with the running maximum 425), 0.61 PFLOP/s: 20 cycles of vector and 8 of matrix instructions per 64 pairs and
+// SIMD, 25 to 28 in all at the 2.0 GHz the clock falls to.  2 x 16 x 4096 x 8192 heads of 64: 330 us, 0.83 PFLOP/s
 template <class T, int KS, int QT, int TK, int NW>
 __global__ __launch_bounds__(64 * NW, (NW == 4 ? fwd_per_cu<Frag<T>::NP, KS, QT>() : 1)) void xa_fwd_kernel(TileArgs a) {
     using E = typename Frag<T>::E;
@@ -525,140 +529,140 @@ __global__ __launch_bounds__(64 * NW, (NW == 4 ? fwd_per_cu<Frag<T>::NP, KS, QT>
     if (worker >= a.workers) return;
     Piece w;
     for (Walk walk(a, worker); walk.next(a, w);) {
-    const int z = w.z, n = keys_of(a.s, z), last = min(w.last, (n + TK - 1) / TK);
-    const int q0 = (w.block * NW + wave) * QT;          // this wave's first query tile
+        const int z = w.z, n = keys_of(a.s, z), last = min(w.last, (n + TK - 1) / TK);
+        const int q0 = (w.block * NW + wave) * QT;          // this wave's first query tile
 
-    v8 q[QT][KS][NP];
-    f32x16 o[QT][DB];
-    float m[QT], l[QT];
+        v8 q[QT][KS][NP];
+        f32x16 o[QT][DB];
+        float m[QT], l[QT];
 #pragma unroll
-    for (int t = 0; t < QT; ++t) {
-        const int tile = q0 + t < a.q_tiles ? q0 + t : a.q_tiles - 1;
+        for (int t = 0; t < QT; ++t) {
+            const int tile = q0 + t < a.q_tiles ? q0 + t : a.q_tiles - 1;
 #pragma unroll
-        for (int k = 0; k < KS; ++k) read_frag<E, NP>(a.Qr + (((long long)z * a.q_tiles + tile) * KS + k) * NP * 1024, lane, q[t][k]);
+            for (int k = 0; k < KS; ++k) read_frag<E, NP>(a.Qr + (((long long)z * a.q_tiles + tile) * KS + k) * NP * 1024, lane, q[t][k]);
 #pragma unroll
-        for (int b = 0; b < DB; ++b) o[t][b] = (f32x16)0.f;
-        m[t] = -INFINITY;
-        l[t] = 0.f;
-    }
-    const float c = NP == 3 ? 1.f : a.c;               // (float32: in q's fragments)
-    constexpr float BOUND = Shift<E>::fwd == 0.f ? 48.f : 0.f;
-    const char *Kz = a.Kr + (long long)z * a.k_tiles * KS * NP * 1024, *Vz = a.Vt + (long long)z * a.k_tiles * DB * 2 * NP * 1024;
-    auto fetch = [&](int step) {
-        char *to = lds[step & 1];
-        for (int i = wave; i < KC + VC; i += NW)
-            load_chunk(i < KC ? Kz + ((long long)step * KC + i) * 1024 : Vz + ((long long)step * VC + i - KC) * 1024, to + i * 1024, lane);
-    };
-    // BOUNDED: no score of this piece can pass 2^BOUND either way, m stays 0.  TAIL: rows behind the last key
-    auto run = [&](auto bounded, auto tail, int step) {
-        constexpr bool BOUNDED = decltype(bounded)::value, TAIL = decltype(tail)::value;
-        wait_loads_and_barrier();
-        if (step + 1 < last) fetch(step + 1);
-        const char *K = lds[step & 1], *V = K + KC * 1024;
-        f32x16 s[2][QT];
-        auto scores = [&](int u, f32x16 (&to)[QT]) {
+            for (int b = 0; b < DB; ++b) o[t][b] = (f32x16)0.f;
+            m[t] = -INFINITY;
+            l[t] = 0.f;
+        }
+        const float c = NP == 3 ? 1.f : a.c;               // (float32: in q's fragments)
+        constexpr float BOUND = Shift<E>::fwd == 0.f ? 48.f : 0.f;
+        const char *Kz = a.Kr + (long long)z * a.k_tiles * KS * NP * 1024, *Vz = a.Vt + (long long)z * a.k_tiles * DB * 2 * NP * 1024;
+        auto fetch = [&](int step) {
+            char *to = lds[step & 1];
+            for (int i = wave; i < KC + VC; i += NW)
+                load_chunk(i < KC ? Kz + ((long long)step * KC + i) * 1024 : Vz + ((long long)step * VC + i - KC) * 1024, to + i * 1024, lane);
+        };
+        // BOUNDED: no score of this piece can pass 2^BOUND either way, m stays 0.  TAIL: rows behind the last key
+        auto run = [&](auto bounded, auto tail, int step) {
+            constexpr bool BOUNDED = decltype(bounded)::value, TAIL = decltype(tail)::value;
+            wait_loads_and_barrier();
+            if (step + 1 < last) fetch(step + 1);
+            const char *K = lds[step & 1], *V = K + KC * 1024;
+            f32x16 s[2][QT];
+            auto scores = [&](int u, f32x16 (&to)[QT]) {
 #pragma unroll
-            for (int t = 0; t < QT; ++t) to[t] = (f32x16)0.f;
+                for (int t = 0; t < QT; ++t) to[t] = (f32x16)0.f;
 #pragma unroll
-            for (int k = 0; k < KS; ++k) {
-                v8 f[NP];
-                read_frag<E, NP>(K + (u * KS + k) * NP * 1024, lane, f);
+                for (int k = 0; k < KS; ++k) {
+                    v8 f[NP];
+                    read_frag<E, NP>(K + (u * KS + k) * NP * 1024, lane, f);
 #pragma unroll
-                for (int t = 0; t < QT; ++t) to[t] = mfma_pieces<E, NP>(f, q[t][k], to[t]);
+                    for (int t = 0; t < QT; ++t) to[t] = mfma_pieces<E, NP>(f, q[t][k], to[t]);
+                }
+            };
+            scores(0, s[0]);
+#pragma unroll
+            for (int u = 0; u < SUB; ++u) {
+                f32x16 (&x)[QT] = s[u & 1];
+                if constexpr (TAIL)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        if (step * TK + u * 32 + 8 * (r / 4) + 4 * half + r % 4 >= n)
+#pragma unroll
+                            for (int t = 0; t < QT; ++t) x[t][r] = -INFINITY;
+                if constexpr (!BOUNDED)
+#pragma unroll
+                    for (int t = 0; t < QT; ++t) {
+                        float top = x[t][0];
+#pragma unroll
+                        for (int r = 1; r < 16; ++r) top = fmaxf(top, x[t][r]);
+                        top = swap_halves_max(top) * c;
+                        if (__any(top > m[t] + LAZY)) {
+                            const float up = fmaxf(m[t], top), f = __builtin_amdgcn_exp2f(m[t] - up);
+                            m[t] = up;
+                            l[t] *= f;
+#pragma unroll
+                            for (int b = 0; b < DB; ++b) o[t][b] *= f;
+                        }
+                    }
+                // the next half's products and this one's fragments are under way while the exponentials run
+                constexpr bool EARLY = DB * NP <= 4;           // (registers)
+                v8 vf[2][DB][NP];
+                if constexpr (EARLY)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int b = 0; b < DB; ++b) read_frag<E, NP>(V + ((u * DB + b) * 2 + h) * NP * 1024, lane, vf[h][b]);
+                if (u + 1 < SUB) scores(u + 1, s[(u + 1) & 1]);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    v8 f[QT][NP];
+#pragma unroll
+                    for (int t = 0; t < QT; ++t) {
+                        float p[8];
+                        const float base = m[t] - Shift<E>::fwd;
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            const float y = x[t][8 * h + e];
+                            p[e] = __builtin_amdgcn_exp2f(BOUNDED ? (NP == 3 ? y : y * c) : fmaf(y, c, -base));
+                            l[t] += p[e];
+                        }
+                        split8<E, NP>(p, f[t]);
+                    }
+#pragma unroll
+                    for (int b = 0; b < DB; ++b) {
+                        if constexpr (!EARLY) read_frag<E, NP>(V + ((u * DB + b) * 2 + h) * NP * 1024, lane, vf[h][b]);
+#pragma unroll
+                        for (int t = 0; t < QT; ++t) o[t][b] = mfma_pieces<E, NP>(vf[h][b], f[t], o[t][b]);
+                    }
+                }
             }
         };
-        scores(0, s[0]);
+        const std::true_type yes;
+        const std::false_type no;
+        __syncthreads();                                   // the last piece's tiles have been read
+        if (w.first < last) fetch(w.first);
+        const int whole = min(last, n / TK);               // steps without rows behind the last key
+        int step = w.first;
+        if (BOUND > 0.f && row_norm(a.qn + (long long)z * a.q_tiles, w.block * NW * QT, min((w.block + 1) * NW * QT, a.q_tiles)) *
+                                   row_norm(a.kn + (long long)z * a.k_tiles, w.first * SUB, last * SUB) * c <= BOUND) {
 #pragma unroll
-        for (int u = 0; u < SUB; ++u) {
-            f32x16 (&x)[QT] = s[u & 1];
-            if constexpr (TAIL)
+            for (int t = 0; t < QT; ++t) m[t] = 0.f;
+            for (; step < whole; ++step) run(yes, no, step);
+            if (step < last) run(yes, yes, step);
+        } else {
+            for (; step < whole; ++step) run(no, no, step);
+            if (step < last) run(no, yes, step);
+        }
 #pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    if (step * TK + u * 32 + 8 * (r / 4) + 4 * half + r % 4 >= n)
-#pragma unroll
-                        for (int t = 0; t < QT; ++t) x[t][r] = -INFINITY;
-            if constexpr (!BOUNDED)
-#pragma unroll
-                for (int t = 0; t < QT; ++t) {
-                    float top = x[t][0];
-#pragma unroll
-                    for (int r = 1; r < 16; ++r) top = fmaxf(top, x[t][r]);
-                    top = swap_halves_max(top) * c;
-                    if (__any(top > m[t] + LAZY)) {
-                        const float up = fmaxf(m[t], top), f = __builtin_amdgcn_exp2f(m[t] - up);
-                        m[t] = up;
-                        l[t] *= f;
-#pragma unroll
-                        for (int b = 0; b < DB; ++b) o[t][b] *= f;
-                    }
+        for (int t = 0; t < QT; ++t) {
+            const int row = (q0 + t) * 32 + col;
+            const float sum = swap_halves_sum(l[t]), base = m[t] - Shift<E>::fwd;
+            if (!w.whole) {
+                const long long tile = (long long)w.slot * (NW * QT) + wave * QT + t;
+                if (half == 0) {
+                    a.ml[2 * (tile * 32 + col)] = base;
+                    a.ml[2 * (tile * 32 + col) + 1] = sum;
                 }
-            // the next half's products and this one's fragments are under way while the exponentials run
-            constexpr bool EARLY = DB * NP <= 4;           // (registers)
-            v8 vf[2][DB][NP];
-            if constexpr (EARLY)
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int b = 0; b < DB; ++b) read_frag<E, NP>(V + ((u * DB + b) * 2 + h) * NP * 1024, lane, vf[h][b]);
-            if (u + 1 < SUB) scores(u + 1, s[(u + 1) & 1]);
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                v8 f[QT][NP];
-#pragma unroll
-                for (int t = 0; t < QT; ++t) {
-                    float p[8];
-                    const float base = m[t] - Shift<E>::fwd;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const float y = x[t][8 * h + e];
-                        p[e] = __builtin_amdgcn_exp2f(BOUNDED ? (NP == 3 ? y : y * c) : fmaf(y, c, -base));
-                        l[t] += p[e];
-                    }
-                    split8<E, NP>(p, f[t]);
-                }
-#pragma unroll
-                for (int b = 0; b < DB; ++b) {
-                    if constexpr (!EARLY) read_frag<E, NP>(V + ((u * DB + b) * 2 + h) * NP * 1024, lane, vf[h][b]);
-#pragma unroll
-                    for (int t = 0; t < QT; ++t) o[t][b] = mfma_pieces<E, NP>(vf[h][b], f[t], o[t][b]);
-                }
+                store_part<DB>(a.part + tile * DB * 1024, lane, o[t], 1.f);
+            } else if (row < a.s.M) {
+                const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);     // (NaN stays NaN)
+                if (half == 0 && a.lse) a.lse[(long long)z * a.s.M + row] = sum == 0.f ? INFINITY : base + __log2f(sum);
+                store_row<T, DB>((T *)a.o + q_row(a.s, z, row) * a.s.d, a.s.d, half, o[t], inv);
             }
         }
-    };
-    const std::true_type yes;
-    const std::false_type no;
-    __syncthreads();                                   // the last piece's tiles have been read
-    if (w.first < last) fetch(w.first);
-    const int whole = min(last, n / TK);               // steps without rows behind the last key
-    int step = w.first;
-    if (BOUND > 0.f && row_norm(a.qn + (long long)z * a.q_tiles, w.block * NW * QT, min((w.block + 1) * NW * QT, a.q_tiles)) *
-                               row_norm(a.kn + (long long)z * a.k_tiles, w.first * SUB, last * SUB) * c <= BOUND) {
-#pragma unroll
-        for (int t = 0; t < QT; ++t) m[t] = 0.f;
-        for (; step < whole; ++step) run(yes, no, step);
-        if (step < last) run(yes, yes, step);
-    } else {
-        for (; step < whole; ++step) run(no, no, step);
-        if (step < last) run(no, yes, step);
-    }
-#pragma unroll
-    for (int t = 0; t < QT; ++t) {
-        const int row = (q0 + t) * 32 + col;
-        const float sum = swap_halves_sum(l[t]), base = m[t] - Shift<E>::fwd;
-        if (!w.whole) {
-            const long long tile = (long long)w.slot * (NW * QT) + wave * QT + t;
-            if (half == 0) {
-                a.ml[2 * (tile * 32 + col)] = base;
-                a.ml[2 * (tile * 32 + col) + 1] = sum;
-            }
-            store_part<DB>(a.part + tile * DB * 1024, lane, o[t], 1.f);
-        } else if (row < a.s.M) {
-            const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);     // (NaN stays NaN)
-            if (half == 0 && a.lse) a.lse[(long long)z * a.s.M + row] = sum == 0.f ? INFINITY : base + __log2f(sum);
-            store_row<T, DB>((T *)a.o + q_row(a.s, z, row) * a.s.d, a.s.d, half, o[t], inv);
-        }
-    }
     }
 }
 
@@ -844,6 +848,10 @@ template <class E> __device__ __forceinline__ float ds_scale(const unsigned *ama
     return __uint_as_float((unsigned)(127 + k) << 23);
 }
 
+// dq: 32 QT queries per wave, steps of 32 keys.  S and g V^T again, dS from both, dQ^T += K^T dS.  -D is what the accumulators of g V^T start from.
+// 2 x 2 x 20480^2 heads of 32, bf16: 458 us (64 % of the vector pipe's and 36 % of the matrix pipe's cycles; a matrix instruction
+// takes about half of its own from the vector pipe);
+// 2 x 16 x 4096 x 8192 heads of 64: 468 us, 0.88 PFLOP/s
 template <class T, int KS, int QT, int NW>
 __global__ __launch_bounds__(64 * NW, (NW == 4 ? dq_per_cu<Frag<T>::NP, KS, QT>() : 1)) void xa_dq_kernel(TileArgs a) {
     using E = typename Frag<T>::E;
@@ -856,97 +864,99 @@ __global__ __launch_bounds__(64 * NW, (NW == 4 ? dq_per_cu<Frag<T>::NP, KS, QT>(
     const float up = ds_scale<E>(a.amax);
     Piece w;
     for (Walk walk(a, worker); walk.next(a, w);) {
-    const int z = w.z, n = keys_of(a.s, z), first = w.first, last = min(w.last, (n + TK - 1) / TK);
-    const int q0 = (w.block * NW + wave) * QT;
+        const int z = w.z, n = keys_of(a.s, z), first = w.first, last = min(w.last, (n + TK - 1) / TK);
+        const int q0 = (w.block * NW + wave) * QT;
 
-    v8 q[QT][KS][NP], g[QT][KS][NP];
-    f32x16 dq[QT][DB];
-    float lse[QT], D[QT];                              // negated
+        v8 q[QT][KS][NP], g[QT][KS][NP];
+        f32x16 dq[QT][DB];
+        float lse[QT], D[QT];                              // negated
 #pragma unroll
-    for (int t = 0; t < QT; ++t) {
-        const long long tile = (long long)z * a.q_tiles + (q0 + t < a.q_tiles ? q0 + t : a.q_tiles - 1);
+        for (int t = 0; t < QT; ++t) {
+            const long long tile = (long long)z * a.q_tiles + (q0 + t < a.q_tiles ? q0 + t : a.q_tiles - 1);
 #pragma unroll
-        for (int k = 0; k < KS; ++k) {
-            read_frag<E, NP>(a.Qr + (tile * KS + k) * NP * 1024, lane, q[t][k]);
-            read_frag<E, NP>(a.Gr + (tile * KS + k) * NP * 1024, lane, g[t][k]);
+            for (int k = 0; k < KS; ++k) {
+                read_frag<E, NP>(a.Qr + (tile * KS + k) * NP * 1024, lane, q[t][k]);
+                read_frag<E, NP>(a.Gr + (tile * KS + k) * NP * 1024, lane, g[t][k]);
+            }
+#pragma unroll
+            for (int b = 0; b < DB; ++b) dq[t][b] = (f32x16)0.f;
+            lse[t] = ((const float *)(a.stat + tile * 1024))[col];
+            D[t] = ((const float *)(a.stat + tile * 1024))[32 + col];
         }
+        const char *Kz = a.Kr + (long long)z * a.k_tiles * KS * NP * 1024, *Vz = a.Vr + (long long)z * a.k_tiles * KS * NP * 1024;
+        const char *Tz = a.Kt + (long long)z * a.k_tiles * DB * 2 * NP * 1024;
+        auto fetch = [&](int step) {
+            char *to = lds[step & 1];
+            for (int i = wave; i < 2 * RC + TC; i += NW)
+                load_chunk(i < RC ? Kz + ((long long)step * RC + i) * 1024 : i < 2 * RC ? Vz + ((long long)step * RC + i - RC) * 1024
+                                                                                         : Tz + ((long long)step * TC + i - 2 * RC) * 1024,
+                           to + i * 1024, lane);
+        };
+        auto run = [&](auto tail, int step) {
+            constexpr bool TAIL = decltype(tail)::value;
+            wait_loads_and_barrier();
+            if (step + 1 < last) fetch(step + 1);
+            const char *K = lds[step & 1], *V = K + RC * 1024, *KT = V + RC * 1024;
+            f32x16 s[QT], dp[QT];
 #pragma unroll
-        for (int b = 0; b < DB; ++b) dq[t][b] = (f32x16)0.f;
-        lse[t] = ((const float *)(a.stat + tile * 1024))[col];
-        D[t] = ((const float *)(a.stat + tile * 1024))[32 + col];
-    }
-    const char *Kz = a.Kr + (long long)z * a.k_tiles * KS * NP * 1024, *Vz = a.Vr + (long long)z * a.k_tiles * KS * NP * 1024;
-    const char *Tz = a.Kt + (long long)z * a.k_tiles * DB * 2 * NP * 1024;
-    auto fetch = [&](int step) {
-        char *to = lds[step & 1];
-        for (int i = wave; i < 2 * RC + TC; i += NW)
-            load_chunk(i < RC ? Kz + ((long long)step * RC + i) * 1024 : i < 2 * RC ? Vz + ((long long)step * RC + i - RC) * 1024
-                                                                                     : Tz + ((long long)step * TC + i - 2 * RC) * 1024,
-                       to + i * 1024, lane);
-    };
-    auto run = [&](auto tail, int step) {
-        constexpr bool TAIL = decltype(tail)::value;
-        wait_loads_and_barrier();
-        if (step + 1 < last) fetch(step + 1);
-        const char *K = lds[step & 1], *V = K + RC * 1024, *KT = V + RC * 1024;
-        f32x16 s[QT], dp[QT];
+            for (int t = 0; t < QT; ++t) s[t] = (f32x16)0.f, dp[t] = (f32x16)D[t];
 #pragma unroll
-        for (int t = 0; t < QT; ++t) s[t] = (f32x16)0.f, dp[t] = (f32x16)D[t];
+            for (int k = 0; k < KS; ++k) {
+                v8 f[NP];
+                read_frag<E, NP>(K + k * NP * 1024, lane, f);
 #pragma unroll
-        for (int k = 0; k < KS; ++k) {
-            v8 f[NP];
-            read_frag<E, NP>(K + k * NP * 1024, lane, f);
+                for (int t = 0; t < QT; ++t) s[t] = mfma_pieces<E, NP>(f, q[t][k], s[t]);
+                read_frag<E, NP>(V + k * NP * 1024, lane, f);
 #pragma unroll
-            for (int t = 0; t < QT; ++t) s[t] = mfma_pieces<E, NP>(f, q[t][k], s[t]);
-            read_frag<E, NP>(V + k * NP * 1024, lane, f);
+                for (int t = 0; t < QT; ++t) dp[t] = mfma_pieces<E, NP>(f, g[t][k], dp[t]);
+            }
+            if constexpr (TAIL)
 #pragma unroll
-            for (int t = 0; t < QT; ++t) dp[t] = mfma_pieces<E, NP>(f, g[t][k], dp[t]);
-        }
-        if constexpr (TAIL)
+                for (int r = 0; r < 16; ++r)
+                    if (step * TK + 8 * (r / 4) + 4 * half + r % 4 >= n)
 #pragma unroll
-            for (int r = 0; r < 16; ++r)
-                if (step * TK + 8 * (r / 4) + 4 * half + r % 4 >= n)
+                        for (int t = 0; t < QT; ++t) s[t][r] = -INFINITY, dp[t][r] = 0.f;
 #pragma unroll
-                    for (int t = 0; t < QT; ++t) s[t][r] = -INFINITY, dp[t][r] = 0.f;
+            for (int h = 0; h < 2; ++h) {
+                v8 f[QT][NP];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            v8 f[QT][NP];
+                for (int t = 0; t < QT; ++t) {
+                    float ds[8];
 #pragma unroll
-            for (int t = 0; t < QT; ++t) {
-                float ds[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    ds[e] = __builtin_amdgcn_exp2f(fmaf(s[t][8 * h + e], a.c, lse[t])) * dp[t][8 * h + e];
-                    if constexpr (Shift<E>::bwd != 0.f) ds[e] *= up;
+                    for (int e = 0; e < 8; ++e) {
+                        ds[e] = __builtin_amdgcn_exp2f(fmaf(s[t][8 * h + e], a.c, lse[t])) * dp[t][8 * h + e];
+                        if constexpr (Shift<E>::bwd != 0.f) ds[e] *= up;
+                    }
+                    split8<E, NP>(ds, f[t]);
                 }
-                split8<E, NP>(ds, f[t]);
-            }
 #pragma unroll
-            for (int b = 0; b < DB; ++b) {
-                v8 x[NP];
-                read_frag<E, NP>(KT + (b * 2 + h) * NP * 1024, lane, x);
+                for (int b = 0; b < DB; ++b) {
+                    v8 x[NP];
+                    read_frag<E, NP>(KT + (b * 2 + h) * NP * 1024, lane, x);
 #pragma unroll
-                for (int t = 0; t < QT; ++t) dq[t][b] = mfma_pieces<E, NP>(x, f[t], dq[t][b]);
+                    for (int t = 0; t < QT; ++t) dq[t][b] = mfma_pieces<E, NP>(x, f[t], dq[t][b]);
+                }
             }
+        };
+        __syncthreads();                                   // the last piece's tiles have been read
+        if (first < last) fetch(first);
+        const int whole = min(last, n / TK);               // steps without rows behind the last key
+        int step = first;
+        for (; step < whole; ++step) run(std::false_type(), step);
+        if (step < last) run(std::true_type(), step);
+        const float back = a.scale / up;
+#pragma unroll
+        for (int t = 0; t < QT; ++t) {
+            const int row = (q0 + t) * 32 + col;
+            if (!w.whole) store_part<DB>(a.part + ((long long)w.slot * (NW * QT) + wave * QT + t) * DB * 1024, lane, dq[t], back);
+            else if (row < a.s.M) store_row<T, DB>((T *)a.dq + q_row(a.s, z, row) * a.s.d, a.s.d, half, dq[t], back);
         }
-    };
-    __syncthreads();                                   // the last piece's tiles have been read
-    if (first < last) fetch(first);
-    const int whole = min(last, n / TK);               // steps without rows behind the last key
-    int step = first;
-    for (; step < whole; ++step) run(std::false_type(), step);
-    if (step < last) run(std::true_type(), step);
-    const float back = a.scale / up;
-#pragma unroll
-    for (int t = 0; t < QT; ++t) {
-        const int row = (q0 + t) * 32 + col;
-        if (!w.whole) store_part<DB>(a.part + ((long long)w.slot * (NW * QT) + wave * QT + t) * DB * 1024, lane, dq[t], back);
-        else if (row < a.s.M) store_row<T, DB>((T *)a.dq + q_row(a.s, z, row) * a.s.d, a.s.d, half, dq[t], back);
-    }
     }
 }
 
-// 32 KT keys per wave, steps of 32 queries
+// dk, dv: 32 KT keys per wave, steps of 32 queries.  A lane owns a key here: S = Q K^T, dV^T += g^T P, dK^T += Q^T dS; lse and D of a step's queries lie
+// across a lane's registers and come from LDS with the fragments.  2 x 2 x 20480^2 heads of 32, bf16: 563 us (57 % of the vector and 40 % of the matrix pipe's
+// cycles); 2 x 16 x 4096 x 8192 heads of 64: 659 us, 0.83 PFLOP/s, bound by the fragments it reads from LDS (24 KB per 32 x 32 pairs, about 60 % of 128 bytes a cycle)
 template <class T, int KS>
 struct DkvLds {
     static constexpr int NP = Frag<T>::NP, DB = (KS + 1) / 2, CHUNKS = 2 * KS * NP + 4 * DB * NP + 1;
@@ -966,119 +976,119 @@ __global__ __launch_bounds__(64 * NW, (NW == 4 ? dkv_per_cu<Frag<T>::NP, KS>() :
     const float up = ds_scale<E>(a.amax);
     Piece w;
     for (Walk walk(a, worker); walk.next(a, w);) {
-    const int z = w.z, n = keys_of(a.s, z), first = w.first, last = min(w.last, a.q_tiles);
-    const int k0 = (w.block * NW + wave) * KT;
+        const int z = w.z, n = keys_of(a.s, z), first = w.first, last = min(w.last, a.q_tiles);
+        const int k0 = (w.block * NW + wave) * KT;
 
-    v8 kf[KT][KS][NP], vf[KT][KS][NP];
-    f32x16 dk[KT][DB], dv[KT][DB];
-#pragma unroll
-    for (int t = 0; t < KT; ++t) {
-        const long long tile = (long long)z * a.k_tiles + (k0 + t < a.k_tiles ? k0 + t : a.k_tiles - 1);
-#pragma unroll
-        for (int k = 0; k < KS; ++k) {
-            read_frag<E, NP>(a.Kr + (tile * KS + k) * NP * 1024, lane, kf[t][k]);
-            read_frag<E, NP>(a.Vr + (tile * KS + k) * NP * 1024, lane, vf[t][k]);
-        }
-#pragma unroll
-        for (int b = 0; b < DB; ++b) dk[t][b] = dv[t][b] = (f32x16)0.f;
-    }
-    const long long qz = (long long)z * a.q_tiles;
-    auto fetch = [&](int step) {
-        char *to = lds + (NB == 2 ? (step & 1) * L::CHUNKS * 1024 : 0);
-        const long long tile = qz + step;
-        for (int i = wave; i < L::CHUNKS; i += NW) {
-            const char *from = i < RC ? a.Qr + (tile * RC + i) * 1024 : i < 2 * RC ? a.Gr + (tile * RC + i - RC) * 1024
-                             : i < 2 * RC + TC ? a.Qt + (tile * TC + i - 2 * RC) * 1024
-                             : i < 2 * (RC + TC) ? a.Gt + (tile * TC + i - 2 * RC - TC) * 1024 : a.stat + tile * 1024;
-            load_chunk(from, to + i * 1024, lane);
-        }
-    };
-    __syncthreads();                                   // the last piece's tiles have been read
-    if (first < last) fetch(first);
-    for (int step = first; step < last; ++step) {
-        wait_loads_and_barrier();
-        if (NB == 2 && step + 1 < last) fetch(step + 1);
-        const char *Q = lds + (NB == 2 ? (step & 1) * L::CHUNKS * 1024 : 0), *G = Q + RC * 1024, *QT = G + RC * 1024, *GT = QT + TC * 1024;
-        const float *st = (const float *)(GT + TC * 1024);
-        f32x16 s[KT], dp[KT];
-        float lse[16];                                      // -lse
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            lse[r] = st[8 * (r / 4) + 4 * half + r % 4];
-            if constexpr (Shift<E>::bwd != 0.f) lse[r] += Shift<E>::bwd;
-        }
-        auto scores = [&](int t) {
-            s[t] = (f32x16)0.f;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) dp[t][r] = st[32 + 8 * (r / 4) + 4 * half + r % 4];    // -D
-#pragma unroll
-            for (int k = 0; k < KS; ++k) {
-                v8 f[NP];
-                read_frag<E, NP>(Q + k * NP * 1024, lane, f);
-                s[t] = mfma_pieces<E, NP>(f, kf[t][k], s[t]);
-                read_frag<E, NP>(G + k * NP * 1024, lane, f);
-                dp[t] = mfma_pieces<E, NP>(f, vf[t][k], dp[t]);
-            }
-        };
-        scores(0);
+        v8 kf[KT][KS][NP], vf[KT][KS][NP];
+        f32x16 dk[KT][DB], dv[KT][DB];
 #pragma unroll
         for (int t = 0; t < KT; ++t) {
-            // the next tile's products and this one's fragments are under way while the exponentials run
-            constexpr bool EARLY = DB * NP <= 2 && KT > 1;           // (registers)
-            v8 gf[2][DB][NP], qf[2][DB][NP];
-            if constexpr (EARLY)
+            const long long tile = (long long)z * a.k_tiles + (k0 + t < a.k_tiles ? k0 + t : a.k_tiles - 1);
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
+            for (int k = 0; k < KS; ++k) {
+                read_frag<E, NP>(a.Kr + (tile * KS + k) * NP * 1024, lane, kf[t][k]);
+                read_frag<E, NP>(a.Vr + (tile * KS + k) * NP * 1024, lane, vf[t][k]);
+            }
 #pragma unroll
-                for (int b = 0; b < DB; ++b) {
-                    read_frag<E, NP>(GT + (b * 2 + h) * NP * 1024, lane, gf[h][b]);
-                    read_frag<E, NP>(QT + (b * 2 + h) * NP * 1024, lane, qf[h][b]);
+            for (int b = 0; b < DB; ++b) dk[t][b] = dv[t][b] = (f32x16)0.f;
+        }
+        const long long qz = (long long)z * a.q_tiles;
+        auto fetch = [&](int step) {
+            char *to = lds + (NB == 2 ? (step & 1) * L::CHUNKS * 1024 : 0);
+            const long long tile = qz + step;
+            for (int i = wave; i < L::CHUNKS; i += NW) {
+                const char *from = i < RC ? a.Qr + (tile * RC + i) * 1024 : i < 2 * RC ? a.Gr + (tile * RC + i - RC) * 1024
+                                 : i < 2 * RC + TC ? a.Qt + (tile * TC + i - 2 * RC) * 1024
+                                 : i < 2 * (RC + TC) ? a.Gt + (tile * TC + i - 2 * RC - TC) * 1024 : a.stat + tile * 1024;
+                load_chunk(from, to + i * 1024, lane);
+            }
+        };
+        __syncthreads();                                   // the last piece's tiles have been read
+        if (first < last) fetch(first);
+        for (int step = first; step < last; ++step) {
+            wait_loads_and_barrier();
+            if (NB == 2 && step + 1 < last) fetch(step + 1);
+            const char *Q = lds + (NB == 2 ? (step & 1) * L::CHUNKS * 1024 : 0), *G = Q + RC * 1024, *QT = G + RC * 1024, *GT = QT + TC * 1024;
+            const float *st = (const float *)(GT + TC * 1024);
+            f32x16 s[KT], dp[KT];
+            float lse[16];                                      // -lse
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                lse[r] = st[8 * (r / 4) + 4 * half + r % 4];
+                if constexpr (Shift<E>::bwd != 0.f) lse[r] += Shift<E>::bwd;
+            }
+            auto scores = [&](int t) {
+                s[t] = (f32x16)0.f;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) dp[t][r] = st[32 + 8 * (r / 4) + 4 * half + r % 4];    // -D
+#pragma unroll
+                for (int k = 0; k < KS; ++k) {
+                    v8 f[NP];
+                    read_frag<E, NP>(Q + k * NP * 1024, lane, f);
+                    s[t] = mfma_pieces<E, NP>(f, kf[t][k], s[t]);
+                    read_frag<E, NP>(G + k * NP * 1024, lane, f);
+                    dp[t] = mfma_pieces<E, NP>(f, vf[t][k], dp[t]);
                 }
-            if (t + 1 < KT) scores(t + 1);
-            if constexpr (EARLY) __builtin_amdgcn_sched_barrier(0);
+            };
+            scores(0);
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                float p[8], ds[8];
-                v8 f[NP];
+            for (int t = 0; t < KT; ++t) {
+                // the next tile's products and this one's fragments are under way while the exponentials run
+                constexpr bool EARLY = DB * NP <= 2 && KT > 1;           // (registers)
+                v8 gf[2][DB][NP], qf[2][DB][NP];
+                if constexpr (EARLY)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    p[e] = __builtin_amdgcn_exp2f(fmaf(s[t][8 * h + e], a.c, lse[8 * h + e]));
-                    ds[e] = p[e] * dp[t][8 * h + e];
-                    if constexpr (Shift<E>::bwd != 0.f) ds[e] *= up * (1.f / 32768.f);
-                }
-                split8<E, NP>(p, f);
+                for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int b = 0; b < DB; ++b) {
-                    if constexpr (!EARLY) read_frag<E, NP>(GT + (b * 2 + h) * NP * 1024, lane, gf[h][b]);
-                    dv[t][b] = mfma_pieces<E, NP>(gf[h][b], f, dv[t][b]);
-                }
-                split8<E, NP>(ds, f);
+                    for (int b = 0; b < DB; ++b) {
+                        read_frag<E, NP>(GT + (b * 2 + h) * NP * 1024, lane, gf[h][b]);
+                        read_frag<E, NP>(QT + (b * 2 + h) * NP * 1024, lane, qf[h][b]);
+                    }
+                if (t + 1 < KT) scores(t + 1);
+                if constexpr (EARLY) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int b = 0; b < DB; ++b) {
-                    if constexpr (!EARLY) read_frag<E, NP>(QT + (b * 2 + h) * NP * 1024, lane, qf[h][b]);
-                    dk[t][b] = mfma_pieces<E, NP>(qf[h][b], f, dk[t][b]);
+                for (int h = 0; h < 2; ++h) {
+                    float p[8], ds[8];
+                    v8 f[NP];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        p[e] = __builtin_amdgcn_exp2f(fmaf(s[t][8 * h + e], a.c, lse[8 * h + e]));
+                        ds[e] = p[e] * dp[t][8 * h + e];
+                        if constexpr (Shift<E>::bwd != 0.f) ds[e] *= up * (1.f / 32768.f);
+                    }
+                    split8<E, NP>(p, f);
+#pragma unroll
+                    for (int b = 0; b < DB; ++b) {
+                        if constexpr (!EARLY) read_frag<E, NP>(GT + (b * 2 + h) * NP * 1024, lane, gf[h][b]);
+                        dv[t][b] = mfma_pieces<E, NP>(gf[h][b], f, dv[t][b]);
+                    }
+                    split8<E, NP>(ds, f);
+#pragma unroll
+                    for (int b = 0; b < DB; ++b) {
+                        if constexpr (!EARLY) read_frag<E, NP>(QT + (b * 2 + h) * NP * 1024, lane, qf[h][b]);
+                        dk[t][b] = mfma_pieces<E, NP>(qf[h][b], f, dk[t][b]);
+                    }
                 }
             }
+            if (NB == 1) {
+                __syncthreads();
+                if (step + 1 < last) fetch(step + 1);
+            }
         }
-        if (NB == 1) {
-            __syncthreads();
-            if (step + 1 < last) fetch(step + 1);
-        }
-    }
-    const float back_k = a.scale / up, back_v = Shift<E>::bwd != 0.f ? 1.f / 32768.f : 1.f;
+        const float back_k = a.scale / up, back_v = Shift<E>::bwd != 0.f ? 1.f / 32768.f : 1.f;
 #pragma unroll
-    for (int t = 0; t < KT; ++t) {
-        const int i = (k0 + t) * 32 + col;
-        if (!w.whole) {
-            const long long tile = (long long)w.slot * (NW * KT) + wave * KT + t;
-            store_part<DB>(a.part + tile * DB * 1024, lane, dk[t], back_k);
-            store_part<DB>(a.part2 + tile * DB * 1024, lane, dv[t], back_v);
-        } else if (i < n) {
-            const long long to = k_row(a.s, z, i) * a.s.d;
-            store_row<T, DB>((T *)a.dk + to, a.s.d, half, dk[t], back_k);
-            store_row<T, DB>((T *)a.dv + to, a.s.d, half, dv[t], back_v);
+        for (int t = 0; t < KT; ++t) {
+            const int i = (k0 + t) * 32 + col;
+            if (!w.whole) {
+                const long long tile = (long long)w.slot * (NW * KT) + wave * KT + t;
+                store_part<DB>(a.part + tile * DB * 1024, lane, dk[t], back_k);
+                store_part<DB>(a.part2 + tile * DB * 1024, lane, dv[t], back_v);
+            } else if (i < n) {
+                const long long to = k_row(a.s, z, i) * a.s.d;
+                store_row<T, DB>((T *)a.dk + to, a.s.d, half, dk[t], back_k);
+                store_row<T, DB>((T *)a.dv + to, a.s.d, half, dv[t], back_v);
+            }
         }
-    }
     }
 }
 
