@@ -418,7 +418,8 @@ int md_act8_unpack(const void *codes, const void *scales, int dtype, long long n
  * The last axis of q, k, v, g is contiguous, *_sb / *_sn / *_sh are the strides of sequence, token and head in elements (0 allowed);
  * o, dq [B][Nq][Hq][d] and dk, dv [B][Nk][Hk][d] are contiguous.  lse [B][Hq][Nq]: log2 of the softmax denominator including its
  * maximum, +inf without a key; written by the forward pass (or NULL there), read by the backward pass.  dq may be NULL, dk and dv both may.
- * ws: md_cross_attn_ws_bytes(desc, backward) bytes, 256-byte aligned. */
+ * ws: md_cross_attn_ws_bytes(desc, backward) bytes, 256-byte aligned.
+ * Refused: 65536 sequences or heads, B Hk of 2^24, B Hq Nq or B Hk Nk of 2^31 - 65536, Nk or Nq Hq / Hk of 2^30, and what is beyond. */
 #define MD_ATTN_MAX_D 128
 typedef struct {
     int dtype, B, Nq, Nk, Hq, Hk, d;

@@ -1,6 +1,8 @@
 // 8-bit activation checkpoints: what a forward pass keeps for its backward pass, in 1 + 1/32 byte per element.  Format: md_types.hpp.
 // Both kernels only move bytes: a lane takes 16 bytes of the tensor (4 or 8 elements), the 8 or 4 lanes of a group find its largest magnitude
 // with in-register exchanges, and a few such pieces per lane are in flight together.
+#include <algorithm>
+
 #include "md_types.hpp"
 
 namespace {
@@ -8,6 +10,7 @@ namespace {
 // pieces per lane: writing a quarter of what is read, packing gains nothing from more than one (70.8 M floats: 74 us, with four 84; 4.8 TB/s); unpacking does
 // (69 us against 74; 5.2 TB/s)
 constexpr int PACK = 1, UNPACK = 4;
+constexpr long long CHUNK = 1LL << 32;        // elements per launch, which has fewer than 2^32 threads
 
 template <class T>
 __global__ __launch_bounds__(256) void act8_pack_kernel(const T *__restrict__ x, long long n, signed char *__restrict__ codes,
@@ -55,9 +58,13 @@ extern "C" int md_act8_pack(const void *x, int dtype, long long n, void *codes, 
     MD_REQUIRE(x && codes && scales, "md_act8_pack: null pointer");
     MD_REQUIRE(n <= (1LL << 38), "md_act8_pack: more than 2^38 elements");
     hipStream_t s = (hipStream_t)stream;
-    MD_DISPATCH_DTYPE(dtype, "md_act8_pack",
-                      act8_pack_kernel<T><<<md_cdiv(n, 256 * Wide<T>::n * PACK), 256, 0, s>>>((const T *)x, n, (signed char *)codes,
-                                                                                               (signed char *)scales));
+    MD_DISPATCH_DTYPE(dtype, "md_act8_pack", {
+        for (long long at = 0; at < n; at += CHUNK) {
+            const long long m = std::min(n - at, CHUNK);
+            act8_pack_kernel<T><<<md_cdiv(m, 256 * Wide<T>::n * PACK), 256, 0, s>>>((const T *)x + at, m, (signed char *)codes + at,
+                                                                                    (signed char *)scales + at / MD_ACT8_GROUP);
+        }
+    });
     MD_CHECK_LAUNCH("md_act8_pack");
     return MD_OK;
 }
@@ -68,9 +75,13 @@ extern "C" int md_act8_unpack(const void *codes, const void *scales, int dtype, 
     MD_REQUIRE(x && codes && scales, "md_act8_unpack: null pointer");
     MD_REQUIRE(n <= (1LL << 38), "md_act8_unpack: more than 2^38 elements");
     hipStream_t s = (hipStream_t)stream;
-    MD_DISPATCH_DTYPE(dtype, "md_act8_unpack",
-                      act8_unpack_kernel<T><<<md_cdiv(n, 256 * Wide<T>::n * UNPACK), 256, 0, s>>>((const signed char *)codes,
-                                                                                                 (const signed char *)scales, n, (T *)x));
+    MD_DISPATCH_DTYPE(dtype, "md_act8_unpack", {
+        for (long long at = 0; at < n; at += CHUNK) {
+            const long long m = std::min(n - at, CHUNK);
+            act8_unpack_kernel<T><<<md_cdiv(m, 256 * Wide<T>::n * UNPACK), 256, 0, s>>>((const signed char *)codes + at,
+                                                                                        (const signed char *)scales + at / MD_ACT8_GROUP, m, (T *)x + at);
+        }
+    });
     MD_CHECK_LAUNCH("md_act8_unpack");
     return MD_OK;
 }

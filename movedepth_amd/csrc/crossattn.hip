@@ -195,7 +195,7 @@ struct PackJob {
 struct PackArgs {
     PackJob job[4];
     int blocks[5];               // jobs' first workgroups; behind the last job: rows of masked keys to be zeroed in dk, dv
-    int jobs;
+    int jobs, first;             // first: of this launch's workgroups
     Shape s;
     const void *o;               // with `stat`: of job 0 (the gradient g) also -lse and -D = -g . o, per tile 32 + 32 floats in 1 KB
     const float *lse;
@@ -212,9 +212,10 @@ __global__ __launch_bounds__(64) void xa_pack_kernel(PackArgs a) {
     __shared__ __attribute__((aligned(16))) T rows[32 * LD];
     const int lane = threadIdx.x, col = lane & 31, half = lane >> 5;
     const Shape &s = a.s;
+    const int block = a.first + (int)blockIdx.x;
     int j = 0;
-    while (j < a.jobs && (int)blockIdx.x >= a.blocks[j + 1]) ++j;
-    const int local = blockIdx.x - a.blocks[j];
+    while (j < a.jobs && block >= a.blocks[j + 1]) ++j;
+    const int local = block - a.blocks[j];
     if (j == a.jobs) {           // 32 rows of one sequence's dk, dv
         const int per = (s.N + 31) / 32, b = local / per, n0 = (local % per) * 32;
         const int len = s.Hk * s.d;
@@ -1256,6 +1257,7 @@ int check(const md_attn_desc &a, const char *what) {
     MD_REQUIRE((long long)a.B * a.Hq * a.Nq < (1LL << 31) - 65536 && (long long)a.B * a.Hk * a.Nk < (1LL << 31) - 65536 &&
                    a.Nk < (1 << 30) && (long long)a.Hq / a.Hk * a.Nq < (1 << 30),
                "%s: 2^31 rows or more", what);
+    MD_REQUIRE((long long)a.B * a.Hk < 1 << 24, "%s: 2^24 key heads of sequences or more", what);          // a launch has fewer than 2^32 threads
     MD_REQUIRE(a.scale - a.scale == 0.f, "%s: scale is not finite", what);
     return MD_OK;
 }
@@ -1432,6 +1434,8 @@ PackJob job_of(const void *x, long long sb, long long sn, long long sh, size_t s
     return j;
 }
 
+constexpr int MAX_PACK = 1 << 25;             // a launch has fewer than 2^32 threads
+
 template <class T, int KS> int launch_pack(PackArgs &k, const Plan &p, long long more, hipStream_t s) {
     long long n = 0;
     for (int i = 0; i < k.jobs; ++i) {
@@ -1441,7 +1445,10 @@ template <class T, int KS> int launch_pack(PackArgs &k, const Plan &p, long long
     k.blocks[k.jobs] = (int)n;
     n += more;
     MD_REQUIRE(n < (1LL << 31), "md_cross_attn: too many tiles");
-    if (n) xa_pack_kernel<T, KS><<<(unsigned)n, 64, 0, s>>>(k);
+    for (long long at = 0; at < n; at += MAX_PACK) {
+        k.first = (int)at;
+        xa_pack_kernel<T, KS><<<(unsigned)std::min<long long>(n - at, MAX_PACK), 64, 0, s>>>(k);
+    }
     MD_CHECK_LAUNCH("md_cross_attn: pack");
     return MD_OK;
 }

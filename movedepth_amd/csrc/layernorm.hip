@@ -198,6 +198,7 @@ __global__ __launch_bounds__(256) void ln_bwd_kernel(const T *__restrict__ g, lo
 
 // ---------------------------------------------------------------- rows too long for a workgroup's registers: read again for each sum
 constexpr int LONG = 1024;
+constexpr long long LONG_ROWS = 1 << 20;      // rows per launch, which has fewer than 2^32 threads
 
 __device__ __forceinline__ float block_sum(float v, float *shared) {
     v = md_wave_sum(v);
@@ -376,8 +377,12 @@ extern "C" int md_layer_norm_fwd(const void *x, int dtype, long long rows, int C
     signed char *cd = (signed char *)codes, *sc = (signed char *)scales;
     const Split sp = split_of(pieces(dtype, C));
     if (!sp.tpr) {
-        MD_DISPATCH_DTYPE(dtype, "md_layer_norm_fwd",
-                          ln_long_fwd_kernel<T><<<(unsigned)rows, LONG, 0, s>>>((const T *)x, ldx, w, b, C, eps, (T *)y, stat, cd, sc));
+        MD_DISPATCH_DTYPE(dtype, "md_layer_norm_fwd", {
+            for (long long r = 0; r < rows; r += LONG_ROWS)
+                ln_long_fwd_kernel<T><<<(unsigned)std::min(rows - r, LONG_ROWS), LONG, 0, s>>>(
+                    (const T *)x + r * ldx, ldx, w, b, C, eps, (T *)y + r * C, stat ? stat + 2 * r : nullptr, cd ? cd + r * C : nullptr,
+                    sc ? sc + r * md_cdiv(C, MD_ACT8_GROUP) : nullptr);
+        });
     } else {
         const int grid = fwd_blocks(rows, sp);
         MD_DISPATCH_DTYPE(dtype, "md_layer_norm_fwd", LN_CONFIG(sp, {
@@ -412,7 +417,10 @@ extern "C" int md_layer_norm_bwd(const void *g, long long ldg, const void *x, lo
         if (!sp.tpr) {
             slices = column_slices(rows);
             MD_DISPATCH_DTYPE(dtype, "md_layer_norm_bwd", {
-                if (dx) ln_long_dx_kernel<T><<<(unsigned)rows, LONG, 0, s>>>((const T *)g, ldg, (const T *)x, ldx, cd, sc, stat, w, C, (T *)dx);
+                for (long long r = 0; dx && r < rows; r += LONG_ROWS)
+                    ln_long_dx_kernel<T><<<(unsigned)std::min(rows - r, LONG_ROWS), LONG, 0, s>>>(
+                        (const T *)g + r * ldg, ldg, x ? (const T *)x + r * ldx : nullptr, ldx, cd ? cd + r * C : nullptr,
+                        sc ? sc + r * md_cdiv(C, MD_ACT8_GROUP) : nullptr, stat + 2 * r, w, C, (T *)dx + r * C);
                 if (sums) ln_long_columns_kernel<T><<<dim3(md_cdiv(C, 256), slices), 256, 0, s>>>((const T *)g, ldg, (const T *)x, ldx, cd, sc, stat, rows,
                                                                                                    C, (float *)ws);
             });

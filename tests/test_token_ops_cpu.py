@@ -91,6 +91,7 @@ def test_cross_attention_refuses(entry):
     refused(call(B=-1), "negative")
     refused(call(B=1 << 17), "65535")
     refused(call(B=60000, Hq=60000, Hk=60000, Nq=0, Nk=0), "2^31")
+    refused(call(B=60000, Hq=300, Hk=300, Nq=0, Nk=0), "2^24")
     refused(call(scale=float("nan")), "scale")
     refused(call(q=None), "null")
     refused(call(k=None), "null")

@@ -665,3 +665,34 @@ def test_cross_attention_many_sequences():
     mask[60:70] = False
     mask[0] = False
     check(run_attention(q, k, v, mask, 0.25, go), ref.cross_attention(q, k, v, mask, 0.25, go), "many sequences")
+
+
+def test_more_than_one_launch_holds():
+    """a launch takes 2^32 elements of act8_pack and 2^20 long rows of layer_norm: what lies behind them is the next launch's.  Elements and rows are
+    independent of each other, so those on both sides of the seam have the bits that a call of theirs alone gives."""
+    from movedepth_amd import ops
+
+    g = gen(51)
+    n, edge = (1 << 32) + 100, 4096
+    x = torch.ones(n, device="cuda", dtype=torch.bfloat16)
+    around = torch.cat([randn(g, edge).bfloat16(), randn(g, 100).bfloat16()])
+    x[n - edge - 100:] = around
+    p, few = ops.act8_pack(x), ops.act8_pack(around)
+    back = ops.act8_unpack(p)
+    assert torch.equal(p.codes[n - edge - 100:], few.codes) and torch.equal(p.scales[-few.scales.numel():], few.scales)
+    assert torch.equal(back[n - edge - 100:], ops.act8_unpack(few)) and bool((back[:n - edge - 100] == 1).all())
+    del x, p, back
+    rows, C = (1 << 20) + 3, 8193
+    at = torch.tensor([0, 1, (1 << 20) - 1, 1 << 20, (1 << 20) + 2], device="cuda")
+    few, go = randn(g, 5, C).bfloat16().requires_grad_(), randn(g, 5, C).bfloat16()
+    x, gy = torch.ones(rows, C, device="cuda", dtype=torch.bfloat16), torch.zeros(rows, C, device="cuda", dtype=torch.bfloat16)
+    x[at], gy[at] = few.detach(), go
+    w = randn(g, C)
+    for act_bits in (0, 8):
+        y = ops.layer_norm(x.requires_grad_(), w, None, 1e-5, act_bits)
+        y1 = ops.layer_norm(few, w, None, 1e-5, act_bits)
+        dx, = torch.autograd.grad(y, x, gy)
+        dx1, = torch.autograd.grad(y1, few, go)
+        assert torch.equal(y.detach()[at], y1) and torch.equal(dx[at], dx1)
+        assert not bool(y.detach()[2:(1 << 20) - 1].any()) and not bool(dx[2:(1 << 20) - 1].any())      # constant rows, no gradient
+        del y, dx
