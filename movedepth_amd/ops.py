@@ -1496,6 +1496,16 @@ def _at(t):
     return None if t is None else t.data_ptr()
 
 
+# Rows' statistics are kept for the backward pass as 32-bit words of no floating-point type: hooks that keep what autograd saves in fewer bits
+# (saved_act8, or a user's own) take floating-point tensors for activations, and an exponent's error would be the gradients'.
+_STAT_WORDS = torch.int32
+
+
+def _words(t, source):
+    """t, or its words if it is a copy that was made of `source`"""
+    return t if t is None or t is source else t.view(_STAT_WORDS)
+
+
 # --------------------------------------------------------------------------- 8-bit activation checkpoints
 class Act8:
     """A tensor in 8 bits (act8_pack): `codes` int8 per element in storage order, `scales` int8 per 32 of them (the exponent of
@@ -1585,13 +1595,13 @@ def _layer_norm_fwd(x, weight, bias, eps, act_bits, keep):
         y = torch.empty_like(x, memory_format=torch.contiguous_format)
         stat = codes = scales = None
         if keep:
-            stat = torch.empty(rows, 2, device=dev, dtype=torch.float32)
+            stat = torch.empty(rows, 2, device=dev, dtype=_STAT_WORDS)
             if act_bits:
                 codes = torch.empty(rows, C, device=dev, dtype=torch.int8)
                 scales = torch.empty(rows, (C + 31) // 32, device=dev, dtype=torch.int8)
         _timed_call("md_layer_norm_fwd", x2.data_ptr(), _TOKEN_DTYPE[x.dtype], rows, C, ldx, _at(w), _at(b), eps, y.data_ptr(), _at(stat), _at(codes),
                     _at(scales), _stream_of(dev))
-    return y, (None if codes is not None else x2, codes, scales, stat, w)
+    return y, (None if codes is not None else x2, codes, scales, stat, _words(w, weight))
 
 
 class _LayerNorm(torch.autograd.Function):
@@ -1685,7 +1695,7 @@ def _cross_attention_fwd(q, k, v, key_mask, scale, keep):
             key_mask = key_mask.contiguous()
         a = _attn_desc(q, k, v, key_mask, scale)
         o = torch.empty(q.shape, device=dev, dtype=q.dtype)
-        lse = torch.empty(a.B, a.Hq, a.Nq, device=dev, dtype=torch.float32) if keep else None
+        lse = torch.empty(a.B, a.Hq, a.Nq, device=dev, dtype=_STAT_WORDS) if keep else None
         a.o, a.lse = o.data_ptr(), _at(lse)
         nbytes = _lib.load().md_cross_attn_ws_bytes(ctypes.byref(a), 0)
         ws = _ws(nbytes, dev) if nbytes else None

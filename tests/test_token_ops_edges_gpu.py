@@ -1,0 +1,83 @@
+"""Token operators where a call can go wrong without failing: their statistics and a module's weights inside the 8-bit context, scores of minus infinity and values
+that three bf16 pieces cannot hold, float16 gradients of very different sizes in one call, rows without deviation far from zero, forward-mode
+tangents, and what the trainer builds from them."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import test_token_ops_gpu as base
+import token_ref as ref
+
+pytestmark = pytest.mark.gpu
+
+DT, gen, randn, check = base.DT, base.gen, base.randn, base.check
+
+
+def relative(got, want):
+    got, want = got.detach().double().cpu(), want.detach().double().cpu()
+    return float((got - want).norm() / want.norm())
+
+
+# --------------------------------------------------------------------------- the 8-bit context
+@pytest.mark.parametrize("act_bits", [0, 8])
+def test_saved_act8_leaves_layer_norms_statistics(act_bits):
+    """the rows' means and deviations stay in 32 bits whatever the context's limit: what is kept of x is its 8-bit value, as with act_bits=8 (rows of 64: the
+    same groups of 32), and nothing else changes"""
+    from movedepth_amd import ops
+
+    g = gen(1)
+    x, w, b, go = randn(g, 300, 64, shift=3.0).requires_grad_(), randn(g, 64).requires_grad_(), randn(g, 64).requires_grad_(), randn(g, 300, 64)
+    with ops.saved_act8(min_numel=1):
+        y = ops.layer_norm(x * 1.0, w, b, 1e-5, act_bits)
+    got = dict(zip(("dx", "dw", "db"), torch.autograd.grad(y, (x, w, b), go)), y=y)
+    check(got, ref.layer_norm(x, w, b, 1e-5, go, 8), "layer_norm in the 8-bit context")
+
+
+def test_saved_act8_leaves_the_statistics_of_many_rows():
+    """as many rows as bring the statistics to the context's default limit"""
+    from movedepth_amd import ops
+
+    g = gen(2)
+    x, go = randn(g, 1 << 19, 32, shift=3.0).requires_grad_(), randn(g, 1 << 19, 32)
+    want, = torch.autograd.grad(ops.layer_norm(x, act_bits=8), x, go)
+    with ops.saved_act8():
+        y = ops.layer_norm(x * 1.0)
+    got, = torch.autograd.grad(y, x, go)
+    assert relative(got, want) <= 8 * ref.U32                # the same formula on the same 8-bit values and statistics
+
+
+@pytest.mark.parametrize("B,Nq,Nk,Hq,Hk,d,limit", [(3, 21, 50, 2, 1, 16, 1), (8, 8192, 40, 16, 4, 8, 1 << 20)])
+def test_saved_act8_leaves_cross_attentions_statistics(B, Nq, Nk, Hq, Hk, d, limit):
+    """what is kept of q, k, v and o is their 8-bit value, the row sums stay: the gradients are the formula's on those values (in 64 bits below; the exponents' error,
+    2^-24 times scores of up to ~64, and sums of up to 2^15 terms leave 1e-4 norm-wise).  A sequence without keys lies between the others: its
+    rows' infinite sums must not reach a neighbour"""
+    from movedepth_amd import ops
+
+    g = gen(3)
+    q, k, v = (randn(g, B, n, h, d, scale=s).requires_grad_() for n, h, s in ((Nq, Hq, 2.0), (Nk, Hk, 2.0), (Nk, Hk, 1.0)))
+    go = randn(g, B, Nq, Hq, d)
+    mask = (torch.rand(B, Nk, generator=g) < 0.8).cuda()
+    mask[1] = False
+    with ops.saved_act8(min_numel=limit):
+        o = ops.cross_attention(q * 1.0, k * 1.0, v * 1.0, mask, 0.5)
+    got = torch.autograd.grad(o, (q, k, v), go)
+
+    def kept(t):
+        t = t.detach()
+        return (ops.act8_unpack(ops.act8_pack(t)) if t.numel() >= limit else t).double()
+
+    G, live = Hq // Hk, mask[:, None, None, :]
+    head = lambda t, r: t.transpose(1, 2).repeat_interleave(r, 1)  # noqa: E731
+    s = 0.5 * head(q.detach().double(), 1) @ head(k.detach().double(), G).transpose(2, 3).contiguous()
+    lse = s.masked_fill(~live, float("-inf")).logsumexp(3, keepdim=True)
+    q8, k8, v8, o8, g64 = head(kept(q), 1), head(kept(k), G), head(kept(v), G), head(kept(o), 1), head(go.double(), 1)
+    p = torch.where(live & torch.isfinite(lse), torch.exp(0.5 * q8 @ k8.transpose(2, 3).contiguous() - lse), 0.0)
+    ds = p * (g64 @ v8.transpose(2, 3).contiguous() - (g64 * o8).sum(3, keepdim=True)) * 0.5
+    shared = lambda t: t.view(B, Hk, G, Nk, d).sum(2)  # noqa: E731
+    want = [ds @ k8, shared(ds.transpose(2, 3).contiguous() @ q8), shared(p.transpose(2, 3).contiguous() @ g64)]
+    for name, a, b in zip(("dq", "dk", "dv"), got, want):
+        assert bool(torch.isfinite(a).all()), name
+        assert relative(a, b.transpose(1, 2)) <= 1e-4, name
+    assert not any(bool(t[1].any()) for t in got)
