@@ -1556,15 +1556,42 @@ def act8_unpack(packed):
     return x
 
 
-def saved_act8(min_numel=1 << 20):
+# graph nodes of views and copies of one tensor: what lies behind them holds the same values, in another order or type
+_VIEW_NODES = {n + "Backward%d" % i for i in (0, 1) for n in ("T", "Transpose", "Permute", "View", "UnsafeView", "ReshapeAlias", "Unsqueeze", "Squeeze", "Expand", "Slice",
+                                                              "Select", "Alias", "AsStrided", "Narrow", "Clone", "ToCopy")}
+
+
+def _is_weight(t):
+    """t is a parameter (frozen or not) or another leaf that requires grad, a view of one, or, as its graph shows, a view or a cast of one"""
+    base = t if t._base is None else t._base
+    if isinstance(base, torch.nn.Parameter) or (base.is_leaf and base.requires_grad):
+        return True
+    node = t.grad_fn
+    while node is not None and node.name() in _VIEW_NODES:
+        node = node.next_functions[0][0]
+    return node is not None and node.name() == "torch::autograd::AccumulateGrad"
+
+
+def _left_alone(weights):
+    """-> is t a weight, or (what made it is not known: see saved_act8) of the shape of one of `weights` in some order of its axes"""
+    shapes = {tuple(sorted(w.shape)) for w in weights}
+    return lambda t: (tuple(sorted(t.shape)) in shapes if shapes else False) or _is_weight(t)
+
+
+def saved_act8(min_numel=1 << 20, weights=()):
     """Context manager: activations that autograd keeps for the backward pass inside it are kept in 8 bits (act8_pack) and restored when the
-    backward pass reads them.  Left as they are: parameters and other leaves, tensors below `min_numel` elements (statistics, weights cast
-    by autocast), other types, CPU tensors, and tensors that do not fill their memory (expanded or cut-out views).  Gradients then
-    carry the rounding of the kept activations; the forward pass does not change."""
+    backward pass reads them.  Gradients then carry the rounding of the kept activations; the forward pass does not change.  Left as they are:
+      * parameters, frozen or not, other leaves that require grad, and views and casts of either (a transposed weight, autocast's copy);
+      * what layer_norm and cross_attention keep per row, masks, other types, CPU tensors;
+      * tensors below `min_numel` elements, and those that do not fill their memory (expanded or cut-out views).
+    Everything else of `min_numel` elements and more counts as an activation.  That is wrong of two kinds of tensor that nothing tells apart from one: weights
+    formed without a graph (autocast's copy of a frozen weight, a function's own) -- give the modules' parameters as `weights`, and tensors of
+    their shapes, in any order of the axes, are left as they are -- and what other operators keep per row (the log-sums of torch's own attention, say):
+    run these outside the context where they reach `min_numel`."""
+    left_alone = _left_alone(weights)
 
     def pack(t):
-        if (t.is_cuda and t.dtype in _TOKEN_DTYPE and t.numel() >= min_numel and t.layout is torch.strided
-                and not (t.is_leaf and t.requires_grad) and _is_dense(t)):
+        if (t.is_cuda and t.dtype in _TOKEN_DTYPE and t.numel() >= min_numel and t.layout is torch.strided and _is_dense(t) and not left_alone(t)):
             return act8_pack(t)
         return t
 

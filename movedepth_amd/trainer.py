@@ -364,8 +364,9 @@ class Trainer:
                                         relative_poses[:, f_idx], opt.reg3d_c, layout=self.vol_layout, **sched)
                     for f_idx in range(len(self.matching_ids) - 1)]
             cor_feats, _ = ops.fuse_volumes(vols, layout=self.vol_layout)
-            with ops.saved_act8() if getattr(opt, "act_bits", 0) else contextlib.nullcontext():
-                logits = self.models["reg3d"](cor_feats)  # B D h w
+            reg3d = self.models["reg3d"]
+            with ops.saved_act8(weights=reg3d.parameters()) if getattr(opt, "act_bits", 0) else contextlib.nullcontext():
+                logits = reg3d(cor_feats)  # B D h w
             return ops.softmax_entropy_localmax(logits, min_inv, max_inv, opt.norm_radius, want_prob=want_prob)
 
         depth_mvs, cost_prob_entropy, _ = mvs_branch(ref_match_feat)

@@ -81,3 +81,29 @@ def test_saved_act8_leaves_cross_attentions_statistics(B, Nq, Nk, Hq, Hk, d, lim
         assert bool(torch.isfinite(a).all()), name
         assert relative(a, b.transpose(1, 2)) <= 1e-4, name
     assert not any(bool(t[1].any()) for t in got)
+
+
+@pytest.mark.parametrize("kind", ["trainable", "frozen", "autocast", "autocast transposed", "frozen autocast"])
+def test_saved_act8_leaves_weights(kind):
+    """the input's gradient needs the weight and not the input: bit for bit that of the plain run.  (A frozen weight's autocast copy has no graph that leads to the
+    weight: there the context is told)"""
+    from movedepth_amd import ops
+
+    torch.manual_seed(0)
+    m = torch.nn.Linear(1024, 1024, bias=False).cuda()
+    f = (lambda t: t @ m.weight) if kind == "autocast transposed" else m
+    if kind.startswith("frozen"):
+        m.weight.requires_grad_(False)
+    g = gen(4)
+    x, go = randn(g, 2048, 1024).requires_grad_(), randn(g, 2048, 1024)
+
+    def run():
+        with torch.autocast("cuda", torch.bfloat16, enabled="autocast" in kind):
+            return f(x * 1.0)
+
+    y = run()
+    want, = torch.autograd.grad(y, x, go.to(y.dtype))
+    with ops.saved_act8(weights=m.parameters()) if kind == "frozen autocast" else ops.saved_act8():
+        y = run()
+    got, = torch.autograd.grad(y, x, go.to(y.dtype))
+    assert torch.equal(got, want)
