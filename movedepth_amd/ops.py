@@ -1593,10 +1593,16 @@ def saved_act8(min_numel=1 << 20, weights=()):
     def pack(t):
         if (t.is_cuda and t.dtype in _TOKEN_DTYPE and t.numel() >= min_numel and t.layout is torch.strided and _is_dense(t) and not left_alone(t)):
             return act8_pack(t)
-        return t
+        return t.detach(), t._version          # (detached: an operator's own result must not keep the graph that keeps it)
 
     def unpack(p):
-        return act8_unpack(p) if isinstance(p, Act8) else p
+        if isinstance(p, Act8):
+            return act8_unpack(p)
+        t, version = p
+        if t._version != version:              # autograd checks this only where no hooks are set
+            raise RuntimeError("saved_act8: a tensor %s of %s that the backward pass reads was modified in place after it was saved (version %d, saved at %d)"
+                               % (tuple(t.shape), t.dtype, t._version, version))
+        return t
 
     return torch.autograd.graph.saved_tensors_hooks(pack, unpack)
 

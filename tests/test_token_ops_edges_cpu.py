@@ -65,3 +65,40 @@ def test_the_context_is_told_of_weights_by_shape():
 
     left = ops._left_alone([torch.empty(6, 8), torch.empty(5, 3, 2, 2)])
     assert left(torch.empty(8, 6)) and left(torch.empty(5, 2, 2, 3)) and not left(torch.empty(48)) and not left(torch.empty(8, 7))
+
+
+def test_tensors_left_alone_are_checked_for_changes():
+    from movedepth_amd import ops
+
+    x = torch.randn(5, 7, requires_grad=True)
+    with ops.saved_act8(min_numel=1):
+        a = x * 1.0
+        y = a * a
+    a.add_(1)
+    with pytest.raises(RuntimeError, match="modified"):
+        y.sum().backward()
+
+
+def test_outputs_left_alone_do_not_keep_themselves_alive():
+    """an operator that keeps its own result: the graph must not hold the tensor that holds the graph"""
+    from movedepth_amd import ops
+
+    x = torch.randn(5, 7, requires_grad=True)
+    with ops.saved_act8(min_numel=1):
+        y = torch.sigmoid(x * 1.0)
+    r = weakref.ref(y)
+    del y
+    gc.collect()
+    assert r() is None
+
+
+def test_second_derivatives_through_tensors_left_alone():
+    from movedepth_amd import ops
+
+    x = torch.randn(5, 7, dtype=torch.float64, requires_grad=True)
+
+    def f(t):
+        with ops.saved_act8(min_numel=1):
+            return torch.sigmoid(t * t) * t
+
+    assert torch.autograd.gradgradcheck(f, (x,))

@@ -1,9 +1,6 @@
 """Token operators where a call can go wrong without failing: their statistics and a module's weights inside the 8-bit context, scores of minus infinity and values
 that three bf16 pieces cannot hold, float16 gradients of very different sizes in one call, rows without deviation far from zero, forward-mode
 tangents, and what the trainer builds from them."""
-import math
-
-import numpy as np
 import pytest
 import torch
 
