@@ -323,9 +323,6 @@ class Trainer:
         ref_match_feat, ref_context_feat = self.models["mvs_encoder"](inputs["color_aug", 0, 0])
         src_match_feats = [self.models["mvs_encoder"](inputs["color_aug", f_i, 0])[0] for f_i in self.matching_ids[1:]]
         match_attn = self.models.get("match_attn")
-        frame_feats = src_match_feats                # as they come from the encoder: what the reference features attend to
-        if match_attn is not None:
-            src_match_feats = [match_attn(f, [ref_match_feat]) for f in frame_feats]
 
         # single frame path + mono reprojection loss
         feats = self.models["mono_encoder"](inputs["color_aug", 0, 0])
@@ -358,9 +355,11 @@ class Trainer:
         min_inv, max_inv = 1 / end_planes[:, 1], 1 / end_planes[:, 0]  # swapped on purpose (App. B-6)
 
         def mvs_branch(ref_feat, want_prob=False):
+            src_feats = src_match_feats
             if match_attn is not None:
-                ref_feat = match_attn(ref_feat, frame_feats)
-            vols = [ops.costvol_grouped(ref_feat, src_match_feats[f_idx], inputs[("K", 2)], inputs[("inv_K", 2)],
+                # both sides from this pass's own reference features: the masked pass must not see what its image has lost
+                ref_feat, src_feats = match_attn(ref_feat, src_feats), [match_attn(f, [ref_feat]) for f in src_feats]
+            vols = [ops.costvol_grouped(ref_feat, src_feats[f_idx], inputs[("K", 2)], inputs[("inv_K", 2)],
                                         relative_poses[:, f_idx], opt.reg3d_c, layout=self.vol_layout, **sched)
                     for f_idx in range(len(self.matching_ids) - 1)]
             cor_feats, _ = ops.fuse_volumes(vols, layout=self.vol_layout)

@@ -104,3 +104,49 @@ def test_saved_act8_leaves_weights(kind):
         y = run()
     got, = torch.autograd.grad(y, x, go.to(y.dtype))
     assert torch.equal(got, want)
+
+
+# --------------------------------------------------------------------------- the trainer
+def test_the_erased_region_does_not_come_back_through_the_other_frames(monkeypatch):
+    """--match_attention: in the pass whose reference image has a rectangle erased nothing may depend on what stood there; both sides of its cost volume are compared
+    between two images that differ in the rectangle only.  The encoder's library normalisation sums in an order that changes from run to run (the same image
+    twice, without any attention: 6e-7 of 2), so 32-bit rounding through its layers, 1e-4 of the largest, is allowed; what leaks in is of the features' size"""
+    from movedepth_amd import ops, synthetic, trainer
+
+    monkeypatch.setattr(trainer, "random_image_mask", lambda img, size: erase(img))
+    keep = {}
+
+    def erase(img):
+        m = torch.ones_like(img)
+        m[:, :, 10:31, 20:62] = 0
+        return img * m, m
+
+    calls, real = [], ops.costvol_grouped
+
+    def record(ref_feat, src_feat, *a, **kw):
+        calls.append((ref_feat.detach().clone(), src_feat.detach().clone()))
+        return real(ref_feat, src_feat, *a, **kw)
+
+    monkeypatch.setattr(ops, "costvol_grouped", record)
+    make = synthetic.make_inputs
+    _, _, t = base.step(["--match_attention", "2"])
+    torch.nn.init.normal_(t.models["match_attn"].out.weight, std=0.5)
+    state = {n: {k: v.clone() for k, v in m.state_dict().items()} for n, m in t.models.items()}
+
+    def changed(*a, **kw):
+        inputs = make(*a, **kw)
+        inputs["color_aug", 0, 0] = inputs["color_aug", 0, 0].clone()
+        inputs["color_aug", 0, 0][:, :, 10:31, 20:62] = 0.9
+        return inputs
+
+    for name, inputs in (("plain", make), ("changed", changed)):
+        calls.clear()
+        monkeypatch.setattr(synthetic, "make_inputs", inputs)
+        base.step(["--match_attention", "2"], models=state)
+        keep[name] = list(calls)
+    n = len(keep["plain"]) // 2
+    assert n >= 1 and len(keep["changed"]) == 2 * n
+    r0, r1 = keep["plain"][0][0], keep["changed"][0][0]
+    assert float((r0 - r1).abs().max()) > 0.1 * float(r0.abs().max())          # the first pass sees the difference
+    for (r0, s0), (r1, s1) in zip(keep["plain"][n:], keep["changed"][n:]):
+        assert float((r0 - r1).abs().max()) <= 1e-4 * float(r0.abs().max()) and float((s0 - s1).abs().max()) <= 1e-4 * float(s0.abs().max())
