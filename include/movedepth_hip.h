@@ -414,7 +414,8 @@ int md_act8_unpack(const void *codes, const void *scales, int dtype, long long n
 
 /* Attention of queries [B][Nq][Hq][d] to keys / values [B][Nk][Hk][d] of another sequence; query head i reads key head
  * i / (Hq / Hk).  key_mask [B][Nk] bytes (NULL: every key is valid): a key whose byte is 0 takes no part, whatever stands in its
- * row; a query left without a key gets o = 0 and gives no gradients; dk, dv of masked keys are 0.
+ * row; a query left without a key gets o = 0 and gives no gradients; dk, dv of masked keys are 0.  A valid key whose score is -inf weighs 0, and a
+ * query whose scores are all -inf is as one without a key; otherwise infinities and NaN go the way of the formula in IEEE arithmetic.
  * The last axis of q, k, v, g is contiguous, *_sb / *_sn / *_sh are the strides of sequence, token and head in elements (0 allowed);
  * o, dq [B][Nq][Hq][d] and dk, dv [B][Nk][Hk][d] are contiguous.  lse [B][Hq][Nq]: log2 of the softmax denominator including its
  * maximum, +inf without a key; written by the forward pass (or NULL there), read by the backward pass.  dq may be NULL, dk and dv both may.

@@ -31,6 +31,9 @@ namespace {
 
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LAZY = 8.f;     // m is raised only when a score passes it by more than 2^8: the sums stay exact, O is rarely rescaled
+// m starts at the lowest finite number: a valid key whose score is -inf then weighs exp2(-inf - m) = 0, wherever it stands, while every finite score raises m or
+// (that number itself) weighs exp2(0).  From -inf it would be exp2(-inf + inf).  A row whose scores are all -inf ends with a sum of 0, as one without keys
+constexpr float LOWEST = -3.402823466e38f;
 
 using f32x16 = float __attribute__((ext_vector_type(16)));
 template <class E> struct Vec { using v8 = E __attribute__((ext_vector_type(8))); };
@@ -185,7 +188,7 @@ struct PackJob {
     const void *x;
     long long sb, sn, sh;
     char *R, *T;                 // where to, either may be null
-    int tiles;                   // of 32 rows, per z; rows behind the last are written as zeros
+    int tiles;                   // of 32 rows, per z; behind the last key are zeros, behind the last query row copies of it
     int query;                   // rows are query rows (else valid keys)
     int vec;                     // 16-byte loads: d and all strides are multiples of 8 elements, x is aligned
     float factor;
@@ -232,7 +235,8 @@ __global__ __launch_bounds__(64) void xa_pack_kernel(PackArgs a) {
     const int count = job.query ? s.M : keys_of(s, z);
 #pragma unroll
     for (int c = 0; c < KS; ++c) {
-        const int chunk = c * 64 + lane, r = chunk / (2 * KS), off = chunk % (2 * KS) * 8, i = tile * 32 + r;
+        // a copy of the last query row, its weights 0 by its `lse`, gives keys what that row gives them: a row of zeros would make NaN of an infinite key
+        const int chunk = c * 64 + lane, r = chunk / (2 * KS), off = chunk % (2 * KS) * 8, i = job.query ? min(tile * 32 + r, count - 1) : tile * 32 + r;
         T v[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = (T)0.f;
@@ -543,7 +547,7 @@ __global__ __launch_bounds__(64 * NW, (NW == 4 ? fwd_per_cu<Frag<T>::NP, KS, QT>
             for (int k = 0; k < KS; ++k) read_frag<E, NP>(a.Qr + (((long long)z * a.q_tiles + tile) * KS + k) * NP * 1024, lane, q[t][k]);
 #pragma unroll
             for (int b = 0; b < DB; ++b) o[t][b] = (f32x16)0.f;
-            m[t] = -INFINITY;
+            m[t] = LOWEST;
             l[t] = 0.f;
         }
         const float c = NP == 3 ? 1.f : a.c;               // (float32: in q's fragments)
@@ -1141,7 +1145,7 @@ __global__ __launch_bounds__(256) void xa_few_kernel(FewArgs a) {
             q[r][e] *= a.c;
             o[r][e] = 0.f;
         }
-        m[r] = -INFINITY;
+        m[r] = LOWEST;
         l[r] = 0.f;
     }
     // every lane of a wave runs the same number of rounds: the row sums cross lanes
@@ -1176,7 +1180,7 @@ __global__ __launch_bounds__(256) void xa_few_kernel(FewArgs a) {
 #pragma unroll
             for (int u = 1; u < U; ++u) top = fmaxf(top, s[u]);
             if (__any(top > m[r] + LAZY)) {
-                const float up = fmaxf(m[r], top), f = up == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[r] - up);
+                const float up = fmaxf(m[r], top), f = __builtin_amdgcn_exp2f(m[r] - up);
                 m[r] = up;
                 l[r] *= f;
 #pragma unroll
@@ -1197,7 +1201,7 @@ __global__ __launch_bounds__(256) void xa_few_kernel(FewArgs a) {
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             const float m2 = __shfl_xor(m[r], x), l2 = __shfl_xor(l[r], x), up = fmaxf(m[r], m2);
-            const float f = m[r] == -INFINITY ? 0.f : exp2f(m[r] - up), f2 = m2 == -INFINITY ? 0.f : exp2f(m2 - up);
+            const float f = exp2f(m[r] - up), f2 = exp2f(m2 - up);
             m[r] = up;
             l[r] = l[r] * f + l2 * f2;
 #pragma unroll
@@ -1222,7 +1226,7 @@ __global__ __launch_bounds__(256) void xa_few_kernel(FewArgs a) {
         for (int w = 1; w < 4; ++w) up = fmaxf(up, sm[w][r][0]);
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-            const float f = sm[w][r][0] == -INFINITY ? 0.f : exp2f(sm[w][r][0] - up);
+            const float f = exp2f(sm[w][r][0] - up);
             sum = fmaf(f, sm[w][r][1], sum);
             x = fmaf(f, so[w][r][dim], x);
         }

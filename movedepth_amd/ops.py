@@ -1777,6 +1777,7 @@ def cross_attention(q, k, v, key_mask=None, scale=None):
     Hk (query head i reads key head i // (Hq // Hk)), d <= 128, scale defaults to d ** -0.5; float32, bfloat16 or float16, all alike; any
     strides (the last axis is copied if it is not contiguous).  key_mask (B, Nk) bool, True where a key takes part: what stands in the
     other rows of k and v is not used, whatever it is, and their gradients are 0; a query without any key gets zeros and gives no gradients.
+    A key whose score is -inf weighs 0, and a query whose scores are all -inf is as one without a key.
     Softmax statistics and sums are float32; with 2-byte types the softmax weights are rounded to that type before the product with v."""
     for t, nm in ((q, "q"), (k, "k"), (v, "v")):
         _token_check(t, nm, "cross_attention")

@@ -106,6 +106,73 @@ def test_saved_act8_leaves_weights(kind):
     assert torch.equal(got, want)
 
 
+# --------------------------------------------------------------------------- scores of minus infinity, values beyond the pieces
+def masked_reference(q, k, v, out, scale, go):
+    """the definition without the keys `out`, whose weight is 0"""
+    mask = torch.ones(k.shape[:2], dtype=torch.bool)
+    mask[:, out] = False
+    return ref.cross_attention(q, k, v, mask, scale, go)
+
+
+PLACES = {"first": [0], "first tile": list(range(40)), "a later tile": [70, 71, 130], "last": [149], "most": list(range(3, 150))}
+
+
+@pytest.mark.parametrize("Nq", [1, 40, 300])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("place", PLACES)
+def test_a_score_of_minus_infinity_has_weight_zero(place, dtype, Nq):
+    """every query's first element is 1 or 2, some keys' -inf: those scores are -inf and their weights 0, whichever key comes first.  The gradient of q's first
+    element multiplies that weight with the infinity and is left out; the keys' own gradients are 0"""
+    g, dt = gen(5), DT[dtype]
+    q, go = randn(g, 2, Nq, 2, 32, dtype=dt), randn(g, 2, Nq, 2, 32, dtype=dt)
+    k, v = randn(g, 2, 150, 2, 32, dtype=dt), randn(g, 2, 150, 2, 32, dtype=dt)
+    q[..., 0] = torch.randint(1, 3, q.shape[:3], generator=g).to(dt).cuda()
+    out = PLACES[place]
+    want = masked_reference(q, k, v, out, 0.2, go)
+    vals = want["dv"]
+    want["dv"] = (vals[0], vals[1] + ref.tiny_of(dt))
+    k[:, out, :, 0] = float("-inf")
+    got = base.run_attention(q, k, v, None, 0.2, go)
+    ref.within(got["o"], *want["o"], "o")
+    ref.within(got["dq"][..., 1:], want["dq"][0][..., 1:], want["dq"][1][..., 1:], "dq")
+    for name in ("dk", "dv"):
+        ref.within(got[name], *want[name], name)
+
+
+@pytest.mark.parametrize("Nq", [1, 50])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_every_score_of_minus_infinity(dtype, Nq):
+    """no key with a weight: zeros and no gradients, as for a query whose keys are all masked"""
+    g, dt = gen(6), DT[dtype]
+    q, go = randn(g, 1, Nq, 1, 16, dtype=dt), randn(g, 1, Nq, 1, 16, dtype=dt)
+    k, v = randn(g, 1, 90, 1, 16, dtype=dt), randn(g, 1, 90, 1, 16, dtype=dt)
+    q[..., 0] = 1
+    k[..., 0] = float("-inf")
+    got = base.run_attention(q, k, v, None, 0.2, go)
+    for name in ("o", "dk", "dv"):
+        assert not bool(got[name].any()), name
+    assert not bool(got["dq"][..., 1:].any())
+
+
+@pytest.mark.parametrize("Nq", [1, 40, 300])
+@pytest.mark.parametrize("dtype", ["bf16"])
+def test_scores_beyond_the_range_below(dtype, Nq):
+    """finite rows whose product passes the range of 32 bits below (-1e38 and less): weight 0, and gradients as without those keys"""
+    g, dt = gen(7), DT[dtype]
+    q, go = randn(g, 2, Nq, 2, 32, dtype=dt), randn(g, 2, Nq, 2, 32, dtype=dt)
+    k, v = randn(g, 2, 150, 2, 32, dtype=dt), randn(g, 2, 150, 2, 32, dtype=dt)
+    out = [0, 1, 35, 149]
+    q[..., 0], k[..., 0] = 1e25, 0
+    want = masked_reference(q, k, v, out, 0.2, go)
+    k[:, out, :, 0] = -1e20
+    got = base.run_attention(q, k, v, None, 0.2, go)
+    for name in ("o", "dk", "dv"):
+        ref.within(got[name], *want[name], name)
+    # 0 times -1e20 is 0; but the sums' own rounding in front of it is not of the other keys' size
+    ref.within(got["dq"][..., 1:], want["dq"][0][..., 1:], want["dq"][1][..., 1:], "dq")
+    assert bool(torch.isfinite(got["dq"]).all())
+
+
 # --------------------------------------------------------------------------- the trainer
 def test_the_erased_region_does_not_come_back_through_the_other_frames(monkeypatch):
     """--match_attention: in the pass whose reference image has a rectangle erased nothing may depend on what stood there; both sides of its cost volume are compared
