@@ -192,7 +192,7 @@ struct PackJob {
     int query;                   // rows are query rows (else valid keys)
     int vec;                     // 16-byte loads: d and all strides are multiples of 8 elements, x is aligned
     float factor;
-    float *norm;                 // largest |row| (after `factor`) of each tile, or null
+    float *norm;                 // no less than the largest |row| (after `factor`) of each tile, or null
     unsigned *amax;              // largest |row|^2 as float bits, or null
 };
 struct PackArgs {
@@ -207,6 +207,8 @@ struct PackArgs {
     long long mask_sb;
     void *dk, *dv;
 };
+
+constexpr float LOST_SQUARES = 0x1p-110f;     // more than 128 squares that fall below float32's normal range can add up to
 
 template <class T, int KS>
 __global__ __launch_bounds__(64) void xa_pack_kernel(PackArgs a) {
@@ -300,12 +302,14 @@ __global__ __launch_bounds__(64) void xa_pack_kernel(PackArgs a) {
         else st[32 + col] = -D;
     }
     if (job.amax || job.norm) {
+        // NaN elements do not count: what they meet is NaN whatever the bound
         float q = 0.f;
-        for (int e = half * 8 * KS; e < (half + 1) * 8 * KS; ++e) q = fmaf((float)rows[col * LD + e], (float)rows[col * LD + e], q);
-        q = swap_halves_sum(q);
-        const bool nan = __any(q != q);
-        q = nan ? NAN : md_wave_max(q);
-        if (lane == 0 && job.norm) job.norm[at] = sqrtf(q) * fabsf(job.factor);
+        for (int e = half * 8 * KS; e < (half + 1) * 8 * KS; ++e) {
+            const float x = (float)rows[col * LD + e], more = fmaf(x, x, q);
+            q = more == more ? more : q;
+        }
+        q = md_wave_max(swap_halves_sum(q));
+        if (lane == 0 && job.norm) job.norm[at] = sqrtf(q + LOST_SQUARES) * fabsf(job.factor);
         if (lane == 0 && job.amax) atomicMax(job.amax, __float_as_uint(q));       // non-negative floats order as their bits; a maximum does not depend on the order
     }
 }
@@ -364,7 +368,7 @@ template <int DB> __device__ __forceinline__ void add_part(const float *from, in
 struct TileArgs {
     Shape s;
     const char *Qr, *Kr, *Vt;                          // forward
-    const float *qn, *kn;                              // largest row norm of each tile of 32
+    const float *qn, *kn, *vn;                         // largest row norm of each tile of 32
     const char *Qt, *Kt, *Vr, *Gr, *Gt, *stat;         // backward
     int q_tiles, k_tiles, workers, rows, step;          // `step`: keys per step; 0: blocks are of keys, a step is a tile of 32 queries
     long long units;                                    // all of them; with a mask the device counts
@@ -505,7 +509,7 @@ struct Walk {
 template <class E> struct Shift { static constexpr float fwd = 0.f, bwd = 0.f; };
 template <> struct Shift<f16_t> { static constexpr float fwd = 7.f, bwd = 15.f; };
 
-// largest of the norms of tiles `from` .. `to` - 1 (a NaN stays): every lane of a wave calls it
+// largest of the norms of tiles `from` .. `to` - 1 (a NaN, of an infinite row times a factor of 0, stays): every lane of a wave calls it
 __device__ __forceinline__ float row_norm(const float *norm, int from, int to) {
     float x = 0.f;
     bool nan = false;
@@ -517,9 +521,9 @@ __device__ __forceinline__ float row_norm(const float *norm, int from, int to) {
 }
 
 // ---------------------------------------------------------------- forward: 32 QT queries per wave, NW waves, steps of TK keys
-// Where |q| |k| scale of a piece's rows bounds its scores by 2^48 either way, m is 0 throughout: no maximum, no rescaling, and the step is straight-line code in
-// which the products of one half run beside the exponentials of the other.  P and its sums stay within 2^+-48 times the row length then (bf16 has
-// float32's exponents; float16 has not and always takes the running maximum).
+// Where |q| |k| scale of a piece's rows bounds its scores by 48 either way, and |v| is below 2^40, m is 0 throughout: no maximum, no rescaling, and the step is
+// straight-line code in which the products of one half run beside the exponentials of the other.  P stays within 2^+-48 then, and O's sums within 2^88 times the
+// row length (bf16 has float32's exponents; float16 has not and always takes the running maximum).
 // 2 x 2 x 20480^2 heads of 32, bf16: 351 us (with the running maximum 425), 0.61 PFLOP/s: 20 cycles of vector and 8 of matrix instructions per 64 pairs and
 // SIMD, 25 to 28 in all at the 2.0 GHz the clock falls to.  2 x 16 x 4096 x 8192 heads of 64: 330 us, 0.83 PFLOP/s
 template <class T, int KS, int QT, int TK, int NW>
@@ -551,14 +555,14 @@ __global__ __launch_bounds__(64 * NW, (NW == 4 ? fwd_per_cu<Frag<T>::NP, KS, QT>
             l[t] = 0.f;
         }
         const float c = NP == 3 ? 1.f : a.c;               // (float32: in q's fragments)
-        constexpr float BOUND = Shift<E>::fwd == 0.f ? 48.f : 0.f;
+        constexpr float BOUND = Shift<E>::fwd == 0.f ? 48.f : 0.f, V_BOUND = 0x1p40f;
         const char *Kz = a.Kr + (long long)z * a.k_tiles * KS * NP * 1024, *Vz = a.Vt + (long long)z * a.k_tiles * DB * 2 * NP * 1024;
         auto fetch = [&](int step) {
             char *to = lds[step & 1];
             for (int i = wave; i < KC + VC; i += NW)
                 load_chunk(i < KC ? Kz + ((long long)step * KC + i) * 1024 : Vz + ((long long)step * VC + i - KC) * 1024, to + i * 1024, lane);
         };
-        // BOUNDED: no score of this piece can pass 2^BOUND either way, m stays 0.  TAIL: rows behind the last key
+        // BOUNDED: no score of this piece can pass BOUND either way, m stays 0.  TAIL: rows behind the last key
         auto run = [&](auto bounded, auto tail, int step) {
             constexpr bool BOUNDED = decltype(bounded)::value, TAIL = decltype(tail)::value;
             wait_loads_and_barrier();
@@ -642,7 +646,8 @@ __global__ __launch_bounds__(64 * NW, (NW == 4 ? fwd_per_cu<Frag<T>::NP, KS, QT>
         const int whole = min(last, n / TK);               // steps without rows behind the last key
         int step = w.first;
         if (BOUND > 0.f && row_norm(a.qn + (long long)z * a.q_tiles, w.block * NW * QT, min((w.block + 1) * NW * QT, a.q_tiles)) *
-                                   row_norm(a.kn + (long long)z * a.k_tiles, w.first * SUB, last * SUB) * c <= BOUND) {
+                                   row_norm(a.kn + (long long)z * a.k_tiles, w.first * SUB, last * SUB) * c <= BOUND &&
+            row_norm(a.vn + (long long)z * a.k_tiles, w.first * SUB, last * SUB) <= V_BOUND) {
 #pragma unroll
             for (int t = 0; t < QT; ++t) m[t] = 0.f;
             for (; step < whole; ++step) run(yes, no, step);
@@ -1282,7 +1287,7 @@ struct Plan {
     bool few;
     int splits;                                   // few rows: of the keys
     Tiles fwd, dq, dkv;
-    size_t idx, cnt, qn, kn, Qr, Kr, Vt, Qt, Kt, Vr, Gr, Gt, stat, amax, part, ml, bytes;
+    size_t idx, cnt, qn, kn, vn, Qr, Kr, Vt, Qt, Kt, Vr, Gr, Gt, stat, amax, part, ml, bytes;
 };
 
 // Workgroups that the chip holds at once, so that they all run to the end together -- unless that left them fewer than `least` steps: then one block of rows
@@ -1340,6 +1345,7 @@ template <int NP, int KS> Plan plan_of(const md_attn_desc &a, bool backward) {
         p.Vt = take(kT);
         p.qn = take((size_t)p.Z * p.q_tiles * 4);
         p.kn = take((size_t)p.Z * p.k_tiles * 4);
+        p.vn = take((size_t)p.Z * p.k_tiles * 4);
         p.fwd = tiles_for(p.Z, p.q_tiles, qt, tk, (a.Nk + tk - 1) / tk, 256 / tk, qt == 2 ? fwd_per_cu<NP, KS, 2>() : fwd_per_cu<NP, KS, 1>(), masked);
         if (p.fwd.join) {
             p.fwd.part = take((size_t)2 * p.fwd.workers * p.fwd.rows * p.DB * 32 * 4);
@@ -1475,10 +1481,10 @@ template <class T, int KS> int run_fwd(const md_attn_desc &a, const Plan &p, con
     k.job[0] = job_of(a.q, a.q_sb, a.q_sn, a.q_sh, sizeof(T), a.d, ws + p.Qr, nullptr, p.q_tiles, 1, factor);
     k.job[1] = job_of(a.k, a.k_sb, a.k_sn, a.k_sh, sizeof(T), a.d, ws + p.Kr, nullptr, p.k_tiles, 0, 1.f);
     k.job[2] = job_of(a.v, a.v_sb, a.v_sn, a.v_sh, sizeof(T), a.d, nullptr, ws + p.Vt, p.k_tiles, 0, 1.f);
-    k.job[0].norm = (float *)(ws + p.qn), k.job[1].norm = (float *)(ws + p.kn);
+    k.job[0].norm = (float *)(ws + p.qn), k.job[1].norm = (float *)(ws + p.kn), k.job[2].norm = (float *)(ws + p.vn);
     if (int rc = launch_pack<T, KS>(k, p, 0, s)) return rc;
     TileArgs t = tile_args(sh, p, p.fwd, ws);
-    t.qn = (float *)(ws + p.qn), t.kn = (float *)(ws + p.kn);
+    t.qn = (float *)(ws + p.qn), t.kn = (float *)(ws + p.kn), t.vn = (float *)(ws + p.vn);
     t.Qr = ws + p.Qr, t.Kr = ws + p.Kr, t.Vt = ws + p.Vt;
     t.c = fmaxf(fabsf(a.scale) * LOG2E, 1.2e-38f);         // not 0: the scores of rows behind the last key are -inf
     t.o = a.o, t.lse = a.lse;

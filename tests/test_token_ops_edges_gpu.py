@@ -173,6 +173,22 @@ def test_scores_beyond_the_range_below(dtype, Nq):
     assert bool(torch.isfinite(got["dq"]).all())
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_the_bound_on_the_scores_holds_at_its_ends(dtype):
+    """rows so small that their squares vanish, against large keys and a large scale: the scores are in the hundreds; and weights of 2^45 times values of 1e28, whose
+    sums pass the range unless the running maximum is taken off"""
+    from movedepth_amd import ops
+
+    g, dt = gen(10), DT[dtype]
+    q = (randn(g, 1, 64, 1, 16).sign() * 5e-24).to(dt)
+    k, v = (randn(g, 1, 200, 1, 16) * 1e18).to(dt), randn(g, 1, 200, 1, 16, dtype=dt)
+    with torch.no_grad():
+        ref.within(ops.cross_attention(q, k, v, None, 1e7), *ref.cross_attention(q, k, v, None, 1e7)["o"], "small rows")
+        q, k = torch.full((1, 64, 1, 16), 1.4, device="cuda", dtype=dt), torch.full((1, 200, 1, 16), 1.4, device="cuda", dtype=dt)
+        v = (randn(g, 1, 200, 1, 16) + 3).to(dt) * 1e28
+        ref.within(ops.cross_attention(q, k, v, None, 1.0), *ref.cross_attention(q, k, v, None, 1.0)["o"], "large values")
+
+
 # --------------------------------------------------------------------------- the trainer
 def test_the_erased_region_does_not_come_back_through_the_other_frames(monkeypatch):
     """--match_attention: in the pass whose reference image has a rectangle erased nothing may depend on what stood there; both sides of its cost volume are compared
