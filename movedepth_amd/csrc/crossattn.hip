@@ -1250,6 +1250,127 @@ __global__ __launch_bounds__(256) void xa_few_kernel(FewArgs a) {
     }
 }
 
+// ---------------------------------------------------------------- float32 beyond the pieces
+// Three bf16 pieces hold a float32 up to 3.39e38 and not infinity, whose remainder is inf - inf, and the six products of two operands overflow one by one, with
+// either sign, where the sum of their exact values would not.  Rows of the tile kernels' operands up to 2^36 keep every product and sum of both passes finite (dS K:
+// 2^36 to the third, times 2, times 2^17 rows); a z with a row beyond, an infinite one among them, is computed again here, from the formula in
+// float32 arithmetic and from the tensors themselves.  Such rows are not met in earnest, so this is the simplest kernel: a wave takes a row, its lanes
+// 64 rows of the other side and then the row's dims.  Otherwise a workgroup reads the tiles' norms of its z and ends: 5 us forward and 6 backward, of 1430 for
+// 6 x 2 x 7680^2 heads of 16.
+struct BeyondArgs {
+    Shape s;
+    const float *q, *k, *v, *g;
+    long long q_sb, q_sn, q_sh, k_sb, k_sn, k_sh, v_sb, v_sn, v_sh, g_sb, g_sn, g_sh;
+    const float *qn, *kn, *vn, *gn;      // gn: backward
+    const char *stat;                    // -lse and -D, as xa_pack left them
+    int q_tiles, k_tiles, blocks;        // blocks: workgroups of a z
+    float c, scale;                      // c: of the exponents, in units of log 2
+    float *o, *lse, *dq, *dk, *dv;
+};
+constexpr float PIECES_BOUND = 0x1p36f;
+__device__ __forceinline__ bool beyond(const BeyondArgs &a, int z) {       // every lane of a wave calls it
+    const long long q0 = (long long)z * a.q_tiles, k0 = (long long)z * a.k_tiles;
+    bool out = false;
+    for (int i = threadIdx.x & 63; i < a.k_tiles; i += 64) out |= !(fmaxf(a.kn[k0 + i], a.vn[k0 + i]) <= PIECES_BOUND);
+    for (int i = threadIdx.x & 63; i < a.q_tiles; i += 64) out |= !(a.qn[q0 + i] <= PIECES_BOUND) || (a.gn && !(a.gn[q0 + i] <= PIECES_BOUND));
+    return __any(out);
+}
+__device__ __forceinline__ float beyond_dot(const float *x, const float *y, int d, float f) {
+    float s = 0.f;
+    for (int e = 0; e < d; ++e) s = fmaf(x[e] * f, y[e], s);
+    return s;
+}
+struct BeyondRows {                      // of one z
+    const float *q, *k, *v, *g;
+    int b, Nq;
+    __device__ __forceinline__ BeyondRows(const BeyondArgs &a, int z) {
+        b = z / a.s.Hk, Nq = a.s.Nq;
+        const int hk = z - b * a.s.Hk;
+        q = a.q + b * a.q_sb + hk * a.s.G * a.q_sh, k = a.k + b * a.k_sb + hk * a.k_sh, v = a.v + b * a.v_sb + hk * a.v_sh;
+        g = a.g ? a.g + b * a.g_sb + hk * a.s.G * a.g_sh : nullptr;
+    }
+    __device__ __forceinline__ const float *query(const float *x, long long sn, long long sh, int r) const { return x + (r % Nq) * sn + (r / Nq) * sh; }
+    __device__ __forceinline__ long long key(const Shape &s, int i) const { return s.idx ? s.idx[(long long)b * s.N + i] : i; }
+};
+
+__global__ __launch_bounds__(256) void xa_beyond_fwd_kernel(BeyondArgs a) {
+    const int z = blockIdx.x / a.blocks, lane = threadIdx.x & 63, n = keys_of(a.s, z), d = a.s.d;
+    if (!beyond(a, z)) return;
+    const BeyondRows at(a, z);
+    for (int r = (blockIdx.x % a.blocks) * 4 + (threadIdx.x >> 6); r < a.s.M; r += a.blocks * 4) {
+        const float *q = at.query(at.q, a.q_sn, a.q_sh, r);
+        auto score = [&](int i) { return beyond_dot(q, at.k + at.key(a.s, i) * a.k_sn, d, a.c); };
+        float m = LOWEST, l = 0.f, o0 = 0.f, o1 = 0.f;
+        for (int i = lane; i < n; i += 64) m = fmaxf(m, score(i));
+        m = md_wave_max(m);
+        for (int i = lane; i < n; i += 64) l += exp2f(score(i) - m);
+        l = md_wave_sum(l);
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        for (int i0 = 0; i0 < n; i0 += 64) {
+            const float p = i0 + lane < n ? exp2f(score(i0 + lane) - m) * inv : 0.f;     // normalised first: sums of large values stay in range
+            for (int i = 0; i < 64 && i0 + i < n; ++i) {
+                const float pi = __shfl(p, i), *v = at.v + at.key(a.s, i0 + i) * a.v_sn;
+                if (lane < d) o0 = fmaf(pi, v[lane], o0);
+                if (lane + 64 < d) o1 = fmaf(pi, v[lane + 64], o1);
+            }
+        }
+        float *o = a.o + q_row(a.s, z, r) * d;
+        if (lane < d) o[lane] = l == 0.f ? 0.f : o0;
+        if (lane + 64 < d) o[lane + 64] = l == 0.f ? 0.f : o1;
+        if (lane == 0 && a.lse) a.lse[(long long)z * a.s.M + r] = l == 0.f ? INFINITY : m + log2f(l);
+    }
+}
+
+// rows of dq, then of dk and dv
+__global__ __launch_bounds__(256) void xa_beyond_bwd_kernel(BeyondArgs a) {
+    const int z = blockIdx.x / a.blocks, lane = threadIdx.x & 63, n = keys_of(a.s, z), d = a.s.d;
+    if (!beyond(a, z)) return;
+    const BeyondRows at(a, z);
+    // weight and scale dS of a pair (scaled first: sums of large values stay in range): `st` are the query row's -lse and -D
+    auto pair = [&](const float *q, const float *g, int r, int i, float &p, float &ds) {
+        const float *st = (const float *)(a.stat + ((long long)z * a.q_tiles + r / 32) * 1024) + r % 32;
+        const long long key = at.key(a.s, i);
+        p = exp2f(beyond_dot(q, at.k + key * a.k_sn, d, a.c) + st[0]);
+        ds = p * (beyond_dot(g, at.v + key * a.v_sn, d, 1.f) + st[32]) * a.scale;
+    };
+    const int queries = a.dq ? a.s.M : 0, keys = a.dk ? n : 0;
+    for (long long row = (blockIdx.x % a.blocks) * 4 + (threadIdx.x >> 6); row < (long long)queries + keys; row += a.blocks * 4) {
+        float x0 = 0.f, x1 = 0.f, y0 = 0.f, y1 = 0.f;
+        if (row < queries) {
+            const int r = (int)row;
+            const float *q = at.query(at.q, a.q_sn, a.q_sh, r), *g = at.query(at.g, a.g_sn, a.g_sh, r);
+            for (int i0 = 0; i0 < n; i0 += 64) {
+                float p = 0.f, ds = 0.f;
+                if (i0 + lane < n) pair(q, g, r, i0 + lane, p, ds);
+                for (int i = 0; i < 64 && i0 + i < n; ++i) {
+                    const float di = __shfl(ds, i), *k = at.k + at.key(a.s, i0 + i) * a.k_sn;
+                    if (lane < d) x0 = fmaf(di, k[lane], x0);
+                    if (lane + 64 < d) x1 = fmaf(di, k[lane + 64], x1);
+                }
+            }
+            float *dq = a.dq + q_row(a.s, z, r) * d;
+            if (lane < d) dq[lane] = x0;
+            if (lane + 64 < d) dq[lane + 64] = x1;
+        } else {
+            const int i = (int)(row - queries);
+            for (int r0 = 0; r0 < a.s.M; r0 += 64) {
+                float p = 0.f, ds = 0.f;
+                if (r0 + lane < a.s.M)
+                    pair(at.query(at.q, a.q_sn, a.q_sh, r0 + lane), at.query(at.g, a.g_sn, a.g_sh, r0 + lane), r0 + lane, i, p, ds);
+                for (int r = 0; r < 64 && r0 + r < a.s.M; ++r) {
+                    const float di = __shfl(ds, r), pi = __shfl(p, r);
+                    const float *q = at.query(at.q, a.q_sn, a.q_sh, r0 + r), *g = at.query(at.g, a.g_sn, a.g_sh, r0 + r);
+                    if (lane < d) x0 = fmaf(di, q[lane], x0), y0 = fmaf(pi, g[lane], y0);
+                    if (lane + 64 < d) x1 = fmaf(di, q[lane + 64], x1), y1 = fmaf(pi, g[lane + 64], y1);
+                }
+            }
+            const long long to = k_row(a.s, z, i) * d;
+            if (lane < d) a.dk[to + lane] = x0, a.dv[to + lane] = y0;
+            if (lane + 64 < d) a.dk[to + lane + 64] = x1, a.dv[to + lane + 64] = y1;
+        }
+    }
+}
+
 // ---------------------------------------------------------------- host side
 // Query rows per key head up to which K and V are read in place.  8 rows on 8 x 20480 keys of 4 heads of 64 (bf16): 73 us, through the tiles 129 us, most of it
 // packing; 16 rows would take two such passes (128 us through the tiles).  1 row: 43 us, 3.9 TB/s of K and V
@@ -1287,7 +1408,7 @@ struct Plan {
     bool few;
     int splits;                                   // few rows: of the keys
     Tiles fwd, dq, dkv;
-    size_t idx, cnt, qn, kn, vn, Qr, Kr, Vt, Qt, Kt, Vr, Gr, Gt, stat, amax, part, ml, bytes;
+    size_t idx, cnt, qn, kn, vn, gn, Qr, Kr, Vt, Qt, Kt, Vr, Gr, Gt, stat, amax, part, ml, bytes;
 };
 
 // Workgroups that the chip holds at once, so that they all run to the end together -- unless that left them fewer than `least` steps: then one block of rows
@@ -1340,12 +1461,12 @@ template <int NP, int KS> Plan plan_of(const md_attn_desc &a, bool backward) {
     const int qt = p.q_tiles >= 8 ? query_tiles<NP, KS>() : 1;
     p.Qr = take(qR);
     p.Kr = take(kR);
+    p.qn = take((size_t)p.Z * p.q_tiles * 4);
+    p.kn = take((size_t)p.Z * p.k_tiles * 4);
+    p.vn = take((size_t)p.Z * p.k_tiles * 4);
     if (!backward) {
         const int tk = fwd_keys<NP, KS>();
         p.Vt = take(kT);
-        p.qn = take((size_t)p.Z * p.q_tiles * 4);
-        p.kn = take((size_t)p.Z * p.k_tiles * 4);
-        p.vn = take((size_t)p.Z * p.k_tiles * 4);
         p.fwd = tiles_for(p.Z, p.q_tiles, qt, tk, (a.Nk + tk - 1) / tk, 256 / tk, qt == 2 ? fwd_per_cu<NP, KS, 2>() : fwd_per_cu<NP, KS, 1>(), masked);
         if (p.fwd.join) {
             p.fwd.part = take((size_t)2 * p.fwd.workers * p.fwd.rows * p.DB * 32 * 4);
@@ -1353,6 +1474,7 @@ template <int NP, int KS> Plan plan_of(const md_attn_desc &a, bool backward) {
             p.fwd.first = take((size_t)p.fwd.workers * 16);
         }
     } else {
+        p.gn = take((size_t)p.Z * p.q_tiles * 4);
         p.Vr = take(kR);
         p.Kt = take(kT);
         p.Qt = take(qT);
@@ -1472,6 +1594,19 @@ TileArgs tile_args(const Shape &sh, const Plan &p, const Tiles &w, char *ws) {
     return t;
 }
 
+// what the float32 kernels beyond the pieces are told, and their workgroups: as many as keep the chip busy should they have work, one for each z at the least
+BeyondArgs beyond_args(const md_attn_desc &a, const Plan &p, const Shape &sh, char *ws, long long rows) {
+    BeyondArgs b{};
+    b.s = sh;
+    b.q = (const float *)a.q, b.k = (const float *)a.k, b.v = (const float *)a.v;
+    b.q_sb = a.q_sb, b.q_sn = a.q_sn, b.q_sh = a.q_sh, b.k_sb = a.k_sb, b.k_sn = a.k_sn, b.k_sh = a.k_sh, b.v_sb = a.v_sb, b.v_sn = a.v_sn, b.v_sh = a.v_sh;
+    b.qn = (const float *)(ws + p.qn), b.kn = (const float *)(ws + p.kn), b.vn = (const float *)(ws + p.vn);
+    b.q_tiles = p.q_tiles, b.k_tiles = p.k_tiles;
+    b.blocks = (int)std::max<long long>(1, std::min<long long>((rows + 3) / 4, CUS / p.Z));
+    b.c = a.scale * LOG2E, b.scale = a.scale;
+    return b;
+}
+
 template <class T, int KS> int run_fwd(const md_attn_desc &a, const Plan &p, const Shape &sh, char *ws, hipStream_t s) {
     constexpr int NP = Frag<T>::NP, TK = fwd_keys<NP, KS>();
     // c > 0 in the kernels: a negative scale goes into q's sign.  In float32 q takes all of it (2^-24 like every other product of the sums)
@@ -1481,7 +1616,7 @@ template <class T, int KS> int run_fwd(const md_attn_desc &a, const Plan &p, con
     k.job[0] = job_of(a.q, a.q_sb, a.q_sn, a.q_sh, sizeof(T), a.d, ws + p.Qr, nullptr, p.q_tiles, 1, factor);
     k.job[1] = job_of(a.k, a.k_sb, a.k_sn, a.k_sh, sizeof(T), a.d, ws + p.Kr, nullptr, p.k_tiles, 0, 1.f);
     k.job[2] = job_of(a.v, a.v_sb, a.v_sn, a.v_sh, sizeof(T), a.d, nullptr, ws + p.Vt, p.k_tiles, 0, 1.f);
-    k.job[0].norm = (float *)(ws + p.qn), k.job[1].norm = (float *)(ws + p.kn), k.job[2].norm = (float *)(ws + p.vn);
+    if (Shift<typename Frag<T>::E>::fwd == 0.f) k.job[0].norm = (float *)(ws + p.qn), k.job[1].norm = (float *)(ws + p.kn), k.job[2].norm = (float *)(ws + p.vn);
     if (int rc = launch_pack<T, KS>(k, p, 0, s)) return rc;
     TileArgs t = tile_args(sh, p, p.fwd, ws);
     t.qn = (float *)(ws + p.qn), t.kn = (float *)(ws + p.kn), t.vn = (float *)(ws + p.vn);
@@ -1500,6 +1635,12 @@ template <class T, int KS> int run_fwd(const md_attn_desc &a, const Plan &p, con
         xa_join_kernel<T, (KS + 1) / 2><<<dim3(t.workers, t.rows / 32), 256, 0, s>>>(t);
         MD_CHECK_LAUNCH("md_cross_attn_fwd: join");
     }
+    if constexpr (NP == 3) {
+        BeyondArgs b = beyond_args(a, p, sh, ws, p.M);
+        b.o = (float *)a.o, b.lse = a.lse;
+        xa_beyond_fwd_kernel<<<(unsigned)p.Z * b.blocks, 256, 0, s>>>(b);
+        MD_CHECK_LAUNCH("md_cross_attn_fwd: rows beyond the pieces");
+    }
     return MD_OK;
 }
 
@@ -1514,6 +1655,8 @@ template <class T, int KS> int run_bwd(const md_attn_desc &a, const Plan &p, con
     k.job[2] = job_of(a.k, a.k_sb, a.k_sn, a.k_sh, sizeof(T), a.d, ws + p.Kr, ws + p.Kt, p.k_tiles, 0, 1.f);
     k.job[3] = job_of(a.v, a.v_sb, a.v_sn, a.v_sh, sizeof(T), a.d, ws + p.Vr, nullptr, p.k_tiles, 0, 1.f);
     k.o = a.o, k.lse = a.lse, k.stat = ws + p.stat;
+    if (NP == 3)
+        k.job[0].norm = (float *)(ws + p.gn), k.job[1].norm = (float *)(ws + p.qn), k.job[2].norm = (float *)(ws + p.kn), k.job[3].norm = (float *)(ws + p.vn);
     if (a.dtype == 2) {
         unsigned *amax = (unsigned *)(ws + p.amax);
         xa_clear_kernel<<<1, 2, 0, s>>>(amax);
@@ -1569,6 +1712,14 @@ template <class T, int KS> int run_bwd(const md_attn_desc &a, const Plan &p, con
             xa_sum_kernel<T, (KS + 1) / 2><<<dim3(t.workers, t.rows / 32), 256, 0, s>>>(t);
             MD_CHECK_LAUNCH("md_cross_attn_bwd: dk, dv sums");
         }
+    }
+    if constexpr (NP == 3) {
+        BeyondArgs b = beyond_args(a, p, sh, ws, (a.dq ? (long long)p.M : 0) + (a.dk ? a.Nk : 0));
+        b.g = (const float *)a.g, b.g_sb = a.g_sb, b.g_sn = a.g_sn, b.g_sh = a.g_sh;
+        b.gn = (const float *)(ws + p.gn), b.stat = ws + p.stat;
+        b.dq = (float *)a.dq, b.dk = (float *)a.dk, b.dv = (float *)a.dv;
+        xa_beyond_bwd_kernel<<<(unsigned)p.Z * b.blocks, 256, 0, s>>>(b);
+        MD_CHECK_LAUNCH("md_cross_attn_bwd: rows beyond the pieces");
     }
     return MD_OK;
 }

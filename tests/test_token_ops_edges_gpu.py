@@ -118,7 +118,7 @@ PLACES = {"first": [0], "first tile": list(range(40)), "a later tile": [70, 71, 
 
 
 @pytest.mark.parametrize("Nq", [1, 40, 300])
-@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("dtype", DT)
 @pytest.mark.parametrize("place", PLACES)
 def test_a_score_of_minus_infinity_has_weight_zero(place, dtype, Nq):
     """every query's first element is 1 or 2, some keys' -inf: those scores are -inf and their weights 0, whichever key comes first.  The gradient of q's first
@@ -140,7 +140,7 @@ def test_a_score_of_minus_infinity_has_weight_zero(place, dtype, Nq):
 
 
 @pytest.mark.parametrize("Nq", [1, 50])
-@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("dtype", DT)
 def test_every_score_of_minus_infinity(dtype, Nq):
     """no key with a weight: zeros and no gradients, as for a query whose keys are all masked"""
     g, dt = gen(6), DT[dtype]
@@ -155,7 +155,7 @@ def test_every_score_of_minus_infinity(dtype, Nq):
 
 
 @pytest.mark.parametrize("Nq", [1, 40, 300])
-@pytest.mark.parametrize("dtype", ["bf16"])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_scores_beyond_the_range_below(dtype, Nq):
     """finite rows whose product passes the range of 32 bits below (-1e38 and less): weight 0, and gradients as without those keys"""
     g, dt = gen(7), DT[dtype]
@@ -171,6 +171,53 @@ def test_scores_beyond_the_range_below(dtype, Nq):
     # 0 times -1e20 is 0; but the sums' own rounding in front of it is not of the other keys' size
     ref.within(got["dq"][..., 1:], want["dq"][0][..., 1:], want["dq"][1][..., 1:], "dq")
     assert bool(torch.isfinite(got["dq"]).all())
+
+
+@pytest.mark.parametrize("Nq", [40])
+@pytest.mark.parametrize("size", [1e12, 1e20, 3.3e38])
+def test_float32_values_beyond_the_pieces(size, Nq):
+    """large q against small k and the other way round, and large v and g: the products are ordinary numbers whatever the operands' own size.  Gradients of the small
+    ones can fall below the normal range, where each of a sum's additions is off by up to half of the smallest step, 2^-150"""
+
+    def check(got, want, what):
+        base.check(got, {n: (val, tol + (70 + 2 * Nq) * 2.0 ** -150) for n, (val, tol) in want.items()}, what)
+
+    g = gen(8)
+    q, go = randn(g, 2, Nq, 2, 24), randn(g, 2, Nq, 2, 24)
+    k, v = randn(g, 2, 70, 2, 24), randn(g, 2, 70, 2, 24)
+    mask = base.make_mask("random", 2, 70, g)
+    big = (q / q.abs().max()).sign() * size
+    gq = go / 1e3 if Nq > 2 else go                          # (40 rows of 3.3e38: dk would be up to 9.2e38, which float32 does not hold)
+    check(base.run_attention(big, k / size, v, mask, 0.3, gq), ref.cross_attention(big, k / size, v, mask, 0.3, gq), "large q")
+    big = torch.where(k > 0, size, -size)
+    check(base.run_attention(q / size, big, v, mask, 0.3, go / 1e3), ref.cross_attention(q / size, big, v, mask, 0.3, go / 1e3), "large k")
+    big = torch.where(v > 0, size, -size) / 4
+    check(base.run_attention(q, k, big, mask, 0.3, go / size), ref.cross_attention(q, k, big, mask, 0.3, go / size), "large v")
+    if size < 1e30:
+        check(base.run_attention(q, k, v / size, mask, 0.3, go * size), ref.cross_attention(q, k, v / size, mask, 0.3, go * size), "large g")
+
+
+@pytest.mark.parametrize("Nq", [1, 40])
+@pytest.mark.parametrize("dtype", DT)
+def test_an_infinite_value_reaches_its_own_column(dtype, Nq):
+    """v = inf under a positive weight: that element of every output is inf, the others are what they were; a NaN query stays in its own row"""
+    from movedepth_amd import ops
+
+    g, dt = gen(9), DT[dtype]
+    q, k, v = randn(g, 1, Nq, 1, 32, dtype=dt), randn(g, 1, 60, 1, 32, dtype=dt), randn(g, 1, 60, 1, 32, dtype=dt)
+    want = ref.cross_attention(q, k, v, None, 0.1)["o"]
+    v[0, 33, 0, 5] = float("inf")
+    with torch.no_grad():
+        o = ops.cross_attention(q, k, v, None, 0.1)
+        assert bool((o[..., 5] == float("inf")).all())
+        keep = [i for i in range(32) if i != 5]
+        ref.within(o[..., keep], want[0][..., keep], want[1][..., keep], "o")
+        if Nq > 1:
+            q[0, 7, 0, 3] = float("nan")
+            o = ops.cross_attention(q, k, v, None, 0.1)
+            rows = [i for i in range(Nq) if i != 7]
+            assert bool(torch.isnan(o[0, 7]).all())
+            ref.within(o[:, rows][..., keep], want[0][:, rows][..., keep], want[1][:, rows][..., keep], "o")
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
