@@ -372,7 +372,7 @@ struct TileArgs {
     const char *Qt, *Kt, *Vr, *Gr, *Gt, *stat;         // backward
     int q_tiles, k_tiles, workers, rows, step;          // `step`: keys per step; 0: blocks are of keys, a step is a tile of 32 queries
     long long units;                                    // all of them; with a mask the device counts
-    float c, scale;
+    float c, scale, down;                               // 2^-down times the weights of all keys is 1 at the most (P is up to 2^LAZY)
     void *o, *dq, *dk, *dv;
     int4 *first;                                         // each worker's first piece: z (-1: idle), block, step -- for who joins the parts
     float *lse, *part, *part2, *ml;                      // parts: [slot][tile of the block][store_part], [slot][row of the block][2]
@@ -523,7 +523,8 @@ __device__ __forceinline__ float row_norm(const float *norm, int from, int to) {
 // ---------------------------------------------------------------- forward: 32 QT queries per wave, NW waves, steps of TK keys
 // Where |q| |k| scale of a piece's rows bounds its scores by 48 either way, and |v| is below 2^40, m is 0 throughout: no maximum, no rescaling, and the step is
 // straight-line code in which the products of one half run beside the exponentials of the other.  P stays within 2^+-48 then, and O's sums within 2^88 times the
-// row length (bf16 has float32's exponents; float16 has not and always takes the running maximum).
+// row length (bf16 has float32's exponents; float16 has not and always takes the running maximum).  Beside a running maximum values above 2^80 take P
+// times a smaller power of two, so that sums of values near the range's end stay in it.
 // 2 x 2 x 20480^2 heads of 32, bf16: 351 us (with the running maximum 425), 0.61 PFLOP/s: 20 cycles of vector and 8 of matrix instructions per 64 pairs and
 // SIMD, 25 to 28 in all at the 2.0 GHz the clock falls to.  2 x 16 x 4096 x 8192 heads of 64: 330 us, 0.83 PFLOP/s
 template <class T, int KS, int QT, int TK, int NW>
@@ -555,7 +556,8 @@ __global__ __launch_bounds__(64 * NW, (NW == 4 ? fwd_per_cu<Frag<T>::NP, KS, QT>
             l[t] = 0.f;
         }
         const float c = NP == 3 ? 1.f : a.c;               // (float32: in q's fragments)
-        constexpr float BOUND = Shift<E>::fwd == 0.f ? 48.f : 0.f, V_BOUND = 0x1p40f;
+        constexpr float BOUND = Shift<E>::fwd == 0.f ? 48.f : 0.f, V_BOUND = 0x1p40f, V_LARGE = 0x1p80f;
+        float shift = -Shift<E>::fwd;                      // P is held times 2^-shift
         const char *Kz = a.Kr + (long long)z * a.k_tiles * KS * NP * 1024, *Vz = a.Vt + (long long)z * a.k_tiles * DB * 2 * NP * 1024;
         auto fetch = [&](int step) {
             char *to = lds[step & 1];
@@ -621,7 +623,7 @@ __global__ __launch_bounds__(64 * NW, (NW == 4 ? fwd_per_cu<Frag<T>::NP, KS, QT>
 #pragma unroll
                     for (int t = 0; t < QT; ++t) {
                         float p[8];
-                        const float base = m[t] - Shift<E>::fwd;
+                        const float base = m[t] + shift;
 #pragma unroll
                         for (int e = 0; e < 8; ++e) {
                             const float y = x[t][8 * h + e];
@@ -645,21 +647,22 @@ __global__ __launch_bounds__(64 * NW, (NW == 4 ? fwd_per_cu<Frag<T>::NP, KS, QT>
         if (w.first < last) fetch(w.first);
         const int whole = min(last, n / TK);               // steps without rows behind the last key
         int step = w.first;
+        const float v_norm = BOUND > 0.f ? row_norm(a.vn + (long long)z * a.k_tiles, w.first * SUB, last * SUB) : 0.f;
         if (BOUND > 0.f && row_norm(a.qn + (long long)z * a.q_tiles, w.block * NW * QT, min((w.block + 1) * NW * QT, a.q_tiles)) *
-                                   row_norm(a.kn + (long long)z * a.k_tiles, w.first * SUB, last * SUB) * c <= BOUND &&
-            row_norm(a.vn + (long long)z * a.k_tiles, w.first * SUB, last * SUB) <= V_BOUND) {
+                                   row_norm(a.kn + (long long)z * a.k_tiles, w.first * SUB, last * SUB) * c <= BOUND && v_norm <= V_BOUND) {
 #pragma unroll
             for (int t = 0; t < QT; ++t) m[t] = 0.f;
             for (; step < whole; ++step) run(yes, no, step);
             if (step < last) run(yes, yes, step);
         } else {
+            if (BOUND > 0.f && v_norm > V_LARGE) shift = a.down;     // sums of large values stay in range
             for (; step < whole; ++step) run(no, no, step);
             if (step < last) run(no, yes, step);
         }
 #pragma unroll
         for (int t = 0; t < QT; ++t) {
             const int row = (q0 + t) * 32 + col;
-            const float sum = swap_halves_sum(l[t]), base = m[t] - Shift<E>::fwd;
+            const float sum = swap_halves_sum(l[t]), base = m[t] + shift;
             if (!w.whole) {
                 const long long tile = (long long)w.slot * (NW * QT) + wave * QT + t;
                 if (half == 0) {
@@ -809,7 +812,7 @@ struct FewArgs {
     long long q_sb, q_sn, q_sh, k_sb, k_sn, k_sh, v_sb, v_sn, v_sh, mask_sb;
     const unsigned char *mask;
     int splits;
-    float c;
+    float c, down, up;           // O is summed times `down`, a power of two that keeps sums of large values in range, and taken back by `up`
     void *o;
     float *lse, *part, *ml;
 };
@@ -841,8 +844,8 @@ __global__ __launch_bounds__(64) void xa_few_join_kernel(FewArgs a) {
     }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
     T *to = (T *)a.o + q_row(a.s, z, row) * a.s.d;
-    if (lane < a.s.d) to[lane] = (T)(o0 * inv);
-    if (lane + 64 < a.s.d) to[lane + 64] = (T)(o1 * inv);
+    if (lane < a.s.d) to[lane] = (T)(o0 * inv * a.up);
+    if (lane + 64 < a.s.d) to[lane + 64] = (T)(o1 * inv * a.up);
     if (lane == 0 && a.lse) a.lse[at] = sum == 0.f ? INFINITY : m + log2f(sum);
 }
 
@@ -1193,10 +1196,10 @@ __global__ __launch_bounds__(256) void xa_few_kernel(FewArgs a) {
             }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const float p = on[u] ? __builtin_amdgcn_exp2f(s[u] - m[r]) : 0.f;
+                const float p = on[u] ? __builtin_amdgcn_exp2f(s[u] - m[r]) : 0.f, pd = p * a.down;
                 l[r] += p;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) o[r][e] = fmaf(p, vv[u][e], o[r][e]);
+                for (int e = 0; e < 8; ++e) o[r][e] = fmaf(pd, vv[u][e], o[r][e]);
             }
         }
     }
@@ -1244,7 +1247,7 @@ __global__ __launch_bounds__(256) void xa_few_kernel(FewArgs a) {
                 a.ml[2 * at + 1] = sum;
             }
         } else {
-            ((T *)a.o)[q_row(a.s, z, r) * a.s.d + dim] = (T)(sum == 0.f ? 0.f : x / sum);
+            ((T *)a.o)[q_row(a.s, z, r) * a.s.d + dim] = (T)(sum == 0.f ? 0.f : x / sum * a.up);
             if (dim == 0 && a.lse) a.lse[zr] = sum == 0.f ? INFINITY : up + log2f(sum);
         }
     }
@@ -1512,6 +1515,7 @@ template <class K> int set_lds(K kernel, int bytes) {
     return MD_OK;
 }
 
+float down_of(int keys) { return LAZY + ceilf(log2f((float)std::max(1, keys))); }
 unsigned grid8(long long blocks) { return (unsigned)((blocks + 7) / 8 * 8); }
 
 template <class T, int R> int launch_few(const FewArgs &f, int d, bool vec, hipStream_t s) {
@@ -1535,6 +1539,7 @@ template <class T> int run_few(const md_attn_desc &a, const Plan &p, const Shape
     f.mask = (const unsigned char *)a.key_mask;
     f.splits = p.splits;
     f.c = a.scale * LOG2E;
+    f.down = exp2f(-down_of(a.Nk)), f.up = exp2f(down_of(a.Nk));
     f.o = a.o, f.lse = a.lse;
     f.part = (float *)(ws + p.part), f.ml = (float *)(ws + p.ml);
     const bool vec = aligned_rows(a.k, sizeof(T), a.d, a.k_sb, a.k_sn, a.k_sh) && aligned_rows(a.v, sizeof(T), a.d, a.v_sb, a.v_sn, a.v_sh);
@@ -1622,6 +1627,7 @@ template <class T, int KS> int run_fwd(const md_attn_desc &a, const Plan &p, con
     t.qn = (float *)(ws + p.qn), t.kn = (float *)(ws + p.kn), t.vn = (float *)(ws + p.vn);
     t.Qr = ws + p.Qr, t.Kr = ws + p.Kr, t.Vt = ws + p.Vt;
     t.c = fmaxf(fabsf(a.scale) * LOG2E, 1.2e-38f);         // not 0: the scores of rows behind the last key are -inf
+    t.down = down_of(a.Nk);
     t.o = a.o, t.lse = a.lse;
     const unsigned grid = grid8(t.workers);
     if (p.fwd.nw == 1) xa_fwd_kernel<T, KS, 1, TK, 1><<<grid, 64, 0, s>>>(t);

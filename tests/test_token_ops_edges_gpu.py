@@ -173,7 +173,7 @@ def test_scores_beyond_the_range_below(dtype, Nq):
     assert bool(torch.isfinite(got["dq"]).all())
 
 
-@pytest.mark.parametrize("Nq", [40])
+@pytest.mark.parametrize("Nq", [2, 40])
 @pytest.mark.parametrize("size", [1e12, 1e20, 3.3e38])
 def test_float32_values_beyond_the_pieces(size, Nq):
     """large q against small k and the other way round, and large v and g: the products are ordinary numbers whatever the operands' own size.  Gradients of the small
@@ -234,6 +234,20 @@ def test_the_bound_on_the_scores_holds_at_its_ends(dtype):
         q, k = torch.full((1, 64, 1, 16), 1.4, device="cuda", dtype=dt), torch.full((1, 200, 1, 16), 1.4, device="cuda", dtype=dt)
         v = (randn(g, 1, 200, 1, 16) + 3).to(dt) * 1e28
         ref.within(ops.cross_attention(q, k, v, None, 1.0), *ref.cross_attention(q, k, v, None, 1.0)["o"], "large values")
+
+
+@pytest.mark.parametrize("qscale", [0.3, 20.0])
+@pytest.mark.parametrize("Nq", [2, 40, 300])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_sums_of_large_values_stay_in_range(dtype, Nq, qscale):
+    """values near the range's end: any number of them weighs no more than one, though their plain sum passes the range"""
+    from movedepth_amd import ops
+
+    g, dt = gen(13), DT[dtype]
+    q, k = randn(g, 1, Nq, 2, 16, dtype=dt, scale=qscale), randn(g, 1, 4000, 2, 16, dtype=dt)
+    v = (randn(g, 1, 4000, 2, 16).sign() * 0.5 + 1).to(dt) * 2.0 ** 126
+    with torch.no_grad():
+        ref.within(ops.cross_attention(q, k, v, None, 1.0), *ref.cross_attention(q, k, v, None, 1.0)["o"], "o")
 
 
 # --------------------------------------------------------------------------- the trainer
