@@ -21,7 +21,7 @@
 // float32 runs on the bf16 instructions too: every operand as the sum of three bf16 pieces (8 + 8 + 8 bits), six products of pieces whose
 // magnitudes matter to 2^-24, which is 6 / 16 of what the float32 matrix instruction costs.  2-byte types: P and dS are rounded to
 // the type before their products (half a step relative).  float16 holds P times 2^7 (forward) or 2^15 (backward) and dS times a power
-// of two from the largest |g| |v|, so that the small weights of long rows do not fall below its range.
+// of two from |g| |v| (ds_scale), so that the small weights of long rows do not fall below its range.
 #include <algorithm>
 #include <type_traits>
 
@@ -193,14 +193,13 @@ struct PackJob {
     int vec;                     // 16-byte loads: d and all strides are multiples of 8 elements, x is aligned
     float factor;
     float *norm;                 // no less than the largest |row| (after `factor`) of each tile, or null
-    unsigned *amax;              // largest |row|^2 as float bits, or null
 };
 struct PackArgs {
     PackJob job[4];
     int blocks[5];               // jobs' first workgroups; behind the last job: rows of masked keys to be zeroed in dk, dv
     int jobs, first;             // first: of this launch's workgroups
     Shape s;
-    const void *o;               // with `stat`: of job 0 (the gradient g) also -lse and -D = -g . o, per tile 32 + 32 floats in 1 KB
+    const void *o;               // with `stat`: of job 0 (the gradient g) also -lse, -D = -g . o and (with a norm) |row|, per tile 3 x 32 floats in 1 KB
     const float *lse;
     char *stat;
     const unsigned char *mask;
@@ -301,20 +300,19 @@ __global__ __launch_bounds__(64) void xa_pack_kernel(PackArgs a) {
         if (half == 0) st[col] = i < s.M ? -a.lse[(long long)z * s.M + i] : -INFINITY;
         else st[32 + col] = -D;
     }
-    if (job.amax || job.norm) {
+    if (job.norm) {
         // NaN elements do not count: what they meet is NaN whatever the bound
         float q = 0.f;
         for (int e = half * 8 * KS; e < (half + 1) * 8 * KS; ++e) {
             const float x = (float)rows[col * LD + e], more = fmaf(x, x, q);
             q = more == more ? more : q;
         }
-        q = md_wave_max(swap_halves_sum(q));
-        if (lane == 0 && job.norm) job.norm[at] = sqrtf(q + LOST_SQUARES) * fabsf(job.factor);
-        if (lane == 0 && job.amax) atomicMax(job.amax, __float_as_uint(q));       // non-negative floats order as their bits; a maximum does not depend on the order
+        q = sqrtf(swap_halves_sum(q) + LOST_SQUARES) * fabsf(job.factor);
+        if (j == 0 && a.stat && half == 0) ((float *)(a.stat + at * 1024))[64 + col] = q;
+        q = md_wave_max(q);
+        if (lane == 0) job.norm[at] = q;
     }
 }
-
-__global__ void xa_clear_kernel(unsigned *p) { p[threadIdx.x] = 0u; }
 
 // ---------------------------------------------------------------- accumulators to memory
 // A lane holds 4 neighbouring dims of its row in each 4 registers: one 8- or 16-byte store where the rows allow it.
@@ -368,7 +366,7 @@ template <int DB> __device__ __forceinline__ void add_part(const float *from, in
 struct TileArgs {
     Shape s;
     const char *Qr, *Kr, *Vt;                          // forward
-    const float *qn, *kn, *vn;                         // largest row norm of each tile of 32
+    const float *qn, *kn, *vn, *gn;                    // largest row norm of each tile of 32
     const char *Qt, *Kt, *Vr, *Gr, *Gt, *stat;         // backward
     int q_tiles, k_tiles, workers, rows, step;          // `step`: keys per step; 0: blocks are of keys, a step is a tile of 32 queries
     long long units;                                    // all of them; with a mask the device counts
@@ -376,7 +374,6 @@ struct TileArgs {
     void *o, *dq, *dk, *dv;
     int4 *first;                                         // each worker's first piece: z (-1: idle), block, step -- for who joins the parts
     float *lse, *part, *part2, *ml;                      // parts: [slot][tile of the block][store_part], [slot][row of the block][2]
-    const unsigned *amax;
 };
 
 struct Line {                                          // of one sequence: blocks of a z, steps of a block
@@ -850,13 +847,14 @@ __global__ __launch_bounds__(64) void xa_few_join_kernel(FewArgs a) {
 }
 
 // ---------------------------------------------------------------- backward
-// float16: dS times 2^k, |dS| 2^k < 2^15: |dS| <= |g v - D| <= 2 max|g| max|v|
-template <class E> __device__ __forceinline__ float ds_scale(const unsigned *amax) {
+// float16: dS times 2^k, |dS| 2^k < 2^15: |dS| <= |g v - D| <= 2 |g| |v|, with the largest |v| of the z's keys and the |g| of the query (dq, where a lane owns
+// one) or the largest of the piece's queries (dk and dv, whose sums run over them).  So a query's dq, and a sequence's dk and dv, are as exact beside gradients
+// of any other size: with one k for the call, rows 2^-20 of the largest came out 2 % off.
+template <class E> __device__ __forceinline__ float ds_scale(float g, float v) {
     if constexpr (Shift<E>::bwd == 0.f) return 1.f;
-    const float sq = 4.f * __uint_as_float(amax[0]) * __uint_as_float(amax[1]);
-    if (!(sq > 0.f) || sq > 1e37f) return 1.f;
-    const int e2 = (int)(__float_as_uint(sq) >> 23) - 127;             // 2^e2 <= sq < 2^(e2 + 1)
-    int k = 14 - ((e2 + 2) >> 1);
+    const float most = 2.f * g * v;
+    if (!(most > 0.f) || most > 1e30f) return 1.f;
+    int k = 14 - ((int)(__float_as_uint(most) >> 23) - 127);           // 2^(14 - k) <= most < 2^(15 - k)
     k = k < -60 ? -60 : k > 60 ? 60 : k;
     return __uint_as_float((unsigned)(127 + k) << 23);
 }
@@ -874,15 +872,15 @@ __global__ __launch_bounds__(64 * NW, (NW == 4 ? dq_per_cu<Frag<T>::NP, KS, QT>(
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, half = lane >> 5;
     const int worker = die_order(blockIdx.x, gridDim.x);
     if (worker >= a.workers) return;
-    const float up = ds_scale<E>(a.amax);
     Piece w;
     for (Walk walk(a, worker); walk.next(a, w);) {
         const int z = w.z, n = keys_of(a.s, z), first = w.first, last = min(w.last, (n + TK - 1) / TK);
+        const float v_norm = Shift<E>::bwd != 0.f ? row_norm(a.vn + (long long)z * a.k_tiles, 0, a.k_tiles) : 0.f;
         const int q0 = (w.block * NW + wave) * QT;
 
         v8 q[QT][KS][NP], g[QT][KS][NP];
         f32x16 dq[QT][DB];
-        float lse[QT], D[QT];                              // negated
+        float lse[QT], D[QT], up[QT];                      // the first two negated
 #pragma unroll
         for (int t = 0; t < QT; ++t) {
             const long long tile = (long long)z * a.q_tiles + (q0 + t < a.q_tiles ? q0 + t : a.q_tiles - 1);
@@ -895,6 +893,7 @@ __global__ __launch_bounds__(64 * NW, (NW == 4 ? dq_per_cu<Frag<T>::NP, KS, QT>(
             for (int b = 0; b < DB; ++b) dq[t][b] = (f32x16)0.f;
             lse[t] = ((const float *)(a.stat + tile * 1024))[col];
             D[t] = ((const float *)(a.stat + tile * 1024))[32 + col];
+            up[t] = Shift<E>::bwd != 0.f ? ds_scale<E>(((const float *)(a.stat + tile * 1024))[64 + col], v_norm) : 1.f;
         }
         const char *Kz = a.Kr + (long long)z * a.k_tiles * KS * NP * 1024, *Vz = a.Vr + (long long)z * a.k_tiles * KS * NP * 1024;
         const char *Tz = a.Kt + (long long)z * a.k_tiles * DB * 2 * NP * 1024;
@@ -938,7 +937,7 @@ __global__ __launch_bounds__(64 * NW, (NW == 4 ? dq_per_cu<Frag<T>::NP, KS, QT>(
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
                         ds[e] = __builtin_amdgcn_exp2f(fmaf(s[t][8 * h + e], a.c, lse[t])) * dp[t][8 * h + e];
-                        if constexpr (Shift<E>::bwd != 0.f) ds[e] *= up;
+                        if constexpr (Shift<E>::bwd != 0.f) ds[e] *= up[t];
                     }
                     split8<E, NP>(ds, f[t]);
                 }
@@ -957,10 +956,10 @@ __global__ __launch_bounds__(64 * NW, (NW == 4 ? dq_per_cu<Frag<T>::NP, KS, QT>(
         int step = first;
         for (; step < whole; ++step) run(std::false_type(), step);
         if (step < last) run(std::true_type(), step);
-        const float back = a.scale / up;
 #pragma unroll
         for (int t = 0; t < QT; ++t) {
             const int row = (q0 + t) * 32 + col;
+            const float back = a.scale / up[t];
             if (!w.whole) store_part<DB>(a.part + ((long long)w.slot * (NW * QT) + wave * QT + t) * DB * 1024, lane, dq[t], back);
             else if (row < a.s.M) store_row<T, DB>((T *)a.dq + q_row(a.s, z, row) * a.s.d, a.s.d, half, dq[t], back);
         }
@@ -986,10 +985,12 @@ __global__ __launch_bounds__(64 * NW, (NW == 4 ? dkv_per_cu<Frag<T>::NP, KS>() :
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, half = lane >> 5;
     const int worker = die_order(blockIdx.x, gridDim.x);
     if (worker >= a.workers) return;
-    const float up = ds_scale<E>(a.amax);
     Piece w;
     for (Walk walk(a, worker); walk.next(a, w);) {
         const int z = w.z, n = keys_of(a.s, z), first = w.first, last = min(w.last, a.q_tiles);
+        float up = 1.f;
+        if constexpr (Shift<E>::bwd != 0.f)
+            up = ds_scale<E>(row_norm(a.gn + (long long)z * a.q_tiles, first, last), row_norm(a.vn + (long long)z * a.k_tiles, 0, a.k_tiles));
         const int k0 = (w.block * NW + wave) * KT;
 
         v8 kf[KT][KS][NP], vf[KT][KS][NP];
@@ -1411,7 +1412,7 @@ struct Plan {
     bool few;
     int splits;                                   // few rows: of the keys
     Tiles fwd, dq, dkv;
-    size_t idx, cnt, qn, kn, vn, gn, Qr, Kr, Vt, Qt, Kt, Vr, Gr, Gt, stat, amax, part, ml, bytes;
+    size_t idx, cnt, qn, kn, vn, gn, Qr, Kr, Vt, Qt, Kt, Vr, Gr, Gt, stat, part, ml, bytes;
 };
 
 // Workgroups that the chip holds at once, so that they all run to the end together -- unless that left them fewer than `least` steps: then one block of rows
@@ -1484,7 +1485,6 @@ template <int NP, int KS> Plan plan_of(const md_attn_desc &a, bool backward) {
         p.Gr = take(qR);
         p.Gt = take(qT);
         p.stat = take((size_t)p.Z * p.q_tiles * kb);
-        p.amax = take(256);
         p.dq = tiles_for(p.Z, p.q_tiles, qt, DQ_KEYS, (a.Nk + DQ_KEYS - 1) / DQ_KEYS, 256 / DQ_KEYS, qt == 2 ? dq_per_cu<NP, KS, 2>() : dq_per_cu<NP, KS, 1>(), masked);
         p.dkv = tiles_for(p.Z, (a.Nk + 31) / 32, key_tiles<NP, KS>(), 0, p.q_tiles, 8, dkv_per_cu<NP, KS>(), masked);
         const size_t nq = p.dq.join ? (size_t)2 * p.dq.workers * p.dq.rows * p.DB * 32 * 4 : 0, nk = p.dkv.join ? (size_t)2 * p.dkv.workers * p.dkv.rows * p.DB * 32 * 4 : 0;
@@ -1661,14 +1661,8 @@ template <class T, int KS> int run_bwd(const md_attn_desc &a, const Plan &p, con
     k.job[2] = job_of(a.k, a.k_sb, a.k_sn, a.k_sh, sizeof(T), a.d, ws + p.Kr, ws + p.Kt, p.k_tiles, 0, 1.f);
     k.job[3] = job_of(a.v, a.v_sb, a.v_sn, a.v_sh, sizeof(T), a.d, ws + p.Vr, nullptr, p.k_tiles, 0, 1.f);
     k.o = a.o, k.lse = a.lse, k.stat = ws + p.stat;
-    if (NP == 3)
-        k.job[0].norm = (float *)(ws + p.gn), k.job[1].norm = (float *)(ws + p.qn), k.job[2].norm = (float *)(ws + p.kn), k.job[3].norm = (float *)(ws + p.vn);
-    if (a.dtype == 2) {
-        unsigned *amax = (unsigned *)(ws + p.amax);
-        xa_clear_kernel<<<1, 2, 0, s>>>(amax);
-        MD_CHECK_LAUNCH("md_cross_attn_bwd: clear");
-        k.job[0].amax = amax, k.job[3].amax = amax + 1;
-    }
+    if (NP == 3 || Shift<typename Frag<T>::E>::bwd != 0.f) k.job[0].norm = (float *)(ws + p.gn), k.job[3].norm = (float *)(ws + p.vn);
+    if (NP == 3) k.job[1].norm = (float *)(ws + p.qn), k.job[2].norm = (float *)(ws + p.kn);
     long long zero = 0;
     if (a.key_mask && a.dk) {
         k.mask = (const unsigned char *)a.key_mask, k.mask_sb = a.mask_sb, k.dk = a.dk, k.dv = a.dv;
@@ -1680,7 +1674,7 @@ template <class T, int KS> int run_bwd(const md_attn_desc &a, const Plan &p, con
         t.Qr = ws + p.Qr, t.Kr = ws + p.Kr, t.Vr = ws + p.Vr, t.Qt = ws + p.Qt, t.Kt = ws + p.Kt, t.Gr = ws + p.Gr, t.Gt = ws + p.Gt, t.stat = ws + p.stat;
         t.c = fmaxf(fabsf(a.scale) * LOG2E, 1.2e-38f);
         t.dq = a.dq, t.dk = a.dk, t.dv = a.dv;
-        t.amax = (const unsigned *)(ws + p.amax);
+        t.vn = (const float *)(ws + p.vn), t.gn = (const float *)(ws + p.gn);
         return t;
     };
     if (a.dq && p.M) {

@@ -250,6 +250,25 @@ def test_sums_of_large_values_stay_in_range(dtype, Nq, qscale):
         ref.within(ops.cross_attention(q, k, v, None, 1.0), *ref.cross_attention(q, k, v, None, 1.0)["o"], "o")
 
 
+# --------------------------------------------------------------------------- float16 gradients of different sizes
+@pytest.mark.parametrize("kind", ["sequences", "rows", "heads"])
+def test_cross_attention_float16_gradients_of_different_sizes(kind):
+    """one half of the gradient is 1e6 times the other: the small half's results are as exact as the large one's.  Norm-wise against 64 bits: dS and the result are each
+    rounded to the type once, and o, which D is formed from; 2^-11 each at most, taken four times for the elements near zero"""
+    g = gen(11)
+    q, go = randn(g, 2, 64, 2, 64, dtype=torch.float16), randn(g, 2, 64, 2, 64)
+    k, v = randn(g, 2, 1024, 2, 64, dtype=torch.float16), randn(g, 2, 1024, 2, 64, dtype=torch.float16)
+    part = {"sequences": (slice(1, 2),), "rows": (slice(None), slice(1, None, 2)), "heads": (slice(None), slice(None), slice(1, 2))}[kind]
+    size = torch.full_like(go, 8e3)
+    size[part] = 8e-3
+    go = (go * size).half()
+    got, want = base.run_attention(q, k, v, None, 0.125, go), ref.cross_attention(q, k, v, None, 0.125, go)
+    for name in ("dq",) if kind == "rows" else ("dq", "dk", "dv"):
+        assert relative(got[name][part], want[name][0][part]) <= 4 * ref.u_of(torch.float16), name
+    for name in ("dq", "dk", "dv"):
+        assert relative(got[name], want[name][0]) <= 4 * ref.u_of(torch.float16), name
+
+
 # --------------------------------------------------------------------------- the trainer
 def test_the_erased_region_does_not_come_back_through_the_other_frames(monkeypatch):
     """--match_attention: in the pass whose reference image has a rectangle erased nothing may depend on what stood there; both sides of its cost volume are compared
