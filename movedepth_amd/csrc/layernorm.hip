@@ -1,6 +1,8 @@
 // Layer norm over the last axis, forward and backward.  m = mean x, r = (mean (x - m)^2 + eps)^(-1/2), n = (x - m) r, y = w n + b;
 // h = g w:  dx = r (h - mean h - n mean(h n)),  dw = sum_rows g n,  db = sum_rows g.
-// Every sum is held in 32 bits; the mean is taken off before squaring, so a large common offset costs no digits of the variance.
+// Every sum is held in 32 bits; the mean is taken off before squaring, so a large common offset costs no digits of the variance.  What the mean's own rounding leaves
+// is the deviations' mean: it comes with the sum of their squares and is taken off both (a constant row of 1000.1 would otherwise deviate by its mean's
+// rounding, 6e-5, which 1 / sqrt(eps) makes 0.02).
 // With 8-bit codes (md_types.hpp) in place of x the backward's n is (x8 - m) r, with m and r those of x itself.
 //
 // Bound by memory: each row is read once into registers (16 bytes per lane and access at any alignment, so odd row lengths run like the others), and a
@@ -12,8 +14,8 @@
 
 namespace {
 
-// sum over the TPR lanes of a row (TPR 256: over the workgroup, through shared memory; `slot` alternates so that one barrier is enough)
-template <int TPR> __device__ __forceinline__ float row_sum(float v, float *shared, int slot) {
+// sum over the TPR lanes of a row
+template <int TPR> __device__ __forceinline__ float lanes_sum(float v) {
 #define LN_DPP_ADD(ctrl) v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), ctrl, 0xF, 0xF, true))
     LN_DPP_ADD(0xB1);
     LN_DPP_ADD(0x4E);
@@ -22,10 +24,27 @@ template <int TPR> __device__ __forceinline__ float row_sum(float v, float *shar
 #undef LN_DPP_ADD
     if constexpr (TPR >= 32) v += __shfl_xor(v, 16);
     if constexpr (TPR >= 64) v += __shfl_xor(v, 32);
+    return v;
+}
+// ... and of two values (TPR 256: over the workgroup, through shared memory; calls alternate between slots 0 and 1, so that one barrier each is enough)
+template <int TPR> __device__ __forceinline__ void row_sum2(float &v, float &w, float *shared, int slot) {
+    v = lanes_sum<TPR>(v);
+    w = lanes_sum<TPR>(w);
     if constexpr (TPR == 256) {
-        if ((threadIdx.x & 63) == 0) shared[slot * 4 + (threadIdx.x >> 6)] = v;
+        float *at = shared + slot * 8;
+        if ((threadIdx.x & 63) == 0) at[threadIdx.x >> 6] = v, at[4 + (threadIdx.x >> 6)] = w;
         __syncthreads();
-        v = (shared[slot * 4] + shared[slot * 4 + 1]) + (shared[slot * 4 + 2] + shared[slot * 4 + 3]);
+        v = (at[0] + at[1]) + (at[2] + at[3]);
+        w = (at[4] + at[5]) + (at[6] + at[7]);
+    }
+}
+template <int TPR> __device__ __forceinline__ float row_sum(float v, float *shared, int slot) {
+    v = lanes_sum<TPR>(v);
+    if constexpr (TPR == 256) {
+        float *at = shared + slot * 8;
+        if ((threadIdx.x & 63) == 0) at[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = (at[0] + at[1]) + (at[2] + at[3]);
     }
     return v;
 }
@@ -35,7 +54,7 @@ __global__ __launch_bounds__(256) void ln_fwd_kernel(const T *__restrict__ x, lo
                                                      int rows, int C, float eps, T *__restrict__ y, float *__restrict__ stat,
                                                      signed char *__restrict__ codes, signed char *__restrict__ scales) {
     constexpr int W = Wide<T>::n, RPB = 256 / TPR;
-    __shared__ float shared[8];
+    __shared__ float shared[16];
     const int sub = threadIdx.x % TPR;
     float wv[NV][W], bv[NV][W];
 #pragma unroll
@@ -81,21 +100,25 @@ __global__ __launch_bounds__(256) void ln_fwd_kernel(const T *__restrict__ x, lo
         for (int i = 0; i < NV; ++i)
 #pragma unroll
             for (int j = 0; j < W; ++j) s += v[i][j];
-        const float mean = row_sum<TPR>(s, shared, 0) * inv;
+        const float first = row_sum<TPR>(s, shared, 0) * inv;
+        float rest = 0.f;
         s = 0.f;
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
             for (int j = 0; j < W; ++j) {
-                v[i][j] = (i * TPR + sub) * W + j < C ? v[i][j] - mean : 0.f;
+                v[i][j] = (i * TPR + sub) * W + j < C ? v[i][j] - first : 0.f;
                 s = fmaf(v[i][j], v[i][j], s);
+                rest += v[i][j];
             }
-        const float rstd = 1.f / sqrtf(row_sum<TPR>(s, shared, 1) * inv + eps);
+        row_sum2<TPR>(s, rest, shared, 1);
+        rest *= inv;
+        const float mean = first + rest, rstd = 1.f / sqrtf(fmaxf(fmaf(-rest, rest, s * inv), 0.f) + eps);
         if (!live) continue;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
 #pragma unroll
-            for (int j = 0; j < W; ++j) v[i][j] = fmaf(v[i][j] * rstd, wv[i][j], bv[i][j]);
+            for (int j = 0; j < W; ++j) v[i][j] = fmaf((v[i][j] - rest) * rstd, wv[i][j], bv[i][j]);
             md_store_wide<T>(y + row * C, (i * TPR + sub) * W, C, v[i]);
         }
         if (stat && sub == 0) {
@@ -112,7 +135,7 @@ __global__ __launch_bounds__(256) void ln_bwd_kernel(const T *__restrict__ g, lo
                                                      const float *__restrict__ stat, const float *__restrict__ w, int rows, int C, T *__restrict__ dx,
                                                      float *__restrict__ part) {
     constexpr int W = Wide<T>::n, RPB = 256 / TPR;
-    __shared__ float shared[RPB > 1 ? 256 * W : 8];
+    __shared__ float shared[RPB > 1 ? 256 * W : 16];
     const int sub = threadIdx.x % TPR;
     float wv[NV][W], dw[NV][W], db[NV][W];
 #pragma unroll
@@ -225,17 +248,21 @@ __global__ __launch_bounds__(LONG) void ln_long_fwd_kernel(const T *__restrict__
 #pragma unroll
         for (int j = 0; j < W; ++j) s += v[j];
     }
-    const float mean = block_sum(s, shared) / (float)C;
+    const float first = block_sum(s, shared) / (float)C;
+    float rest = 0.f;
     s = 0.f;
     for (int c = threadIdx.x * W; c < C; c += LONG * W) {
         md_load_wide<T>(x, c, C, v);
 #pragma unroll
         for (int j = 0; j < W; ++j) {
-            const float d = c + j < C ? v[j] - mean : 0.f;
+            const float d = c + j < C ? v[j] - first : 0.f;
             s = fmaf(d, d, s);
+            rest += d;
         }
     }
-    const float rstd = 1.f / sqrtf(block_sum(s, shared) / (float)C + eps);
+    s = block_sum(s, shared) / (float)C;
+    rest = block_sum(rest, shared) / (float)C;
+    const float mean = first + rest, rstd = 1.f / sqrtf(fmaxf(fmaf(-rest, rest, s), 0.f) + eps);
     const int groups = (C + MD_ACT8_GROUP - 1) / MD_ACT8_GROUP, rounds = (C + LONG * W - 1) / (LONG * W);
     for (int i = 0; i < rounds; ++i) {                    // whole rounds: a group's lanes exchange its maximum
         const int c = (i * LONG + threadIdx.x) * W;
@@ -249,7 +276,7 @@ __global__ __launch_bounds__(LONG) void ln_long_fwd_kernel(const T *__restrict__
         }
 #pragma unroll
         for (int j = 0; j < W; ++j)
-            if (c + j < C) v[j] = fmaf((v[j] - mean) * rstd, w ? w[c + j] : 1.f, b ? b[c + j] : 0.f);
+            if (c + j < C) v[j] = fmaf((v[j] - first - rest) * rstd, w ? w[c + j] : 1.f, b ? b[c + j] : 0.f);
         md_store_wide<T>(y + row * C, c, C, v);
     }
     if (stat && threadIdx.x == 0) {

@@ -269,6 +269,41 @@ def test_cross_attention_float16_gradients_of_different_sizes(kind):
         assert relative(got[name], want[name][0]) <= 4 * ref.u_of(torch.float16), name
 
 
+# --------------------------------------------------------------------------- layer norm
+@pytest.mark.parametrize("C", [8, 48, 96, 777, 2056, 3000, 5000])
+def test_layer_norm_of_rows_without_deviation(C):
+    """a constant row is its own mean: y is b however far from zero it lies.  The mean's error, at most k = C / 64 + 24 roundings of the sum and the division's, is
+    itself found as the mean of the deviations, off by as many roundings of it, and multiplied by 1 / sqrt(eps)"""
+    from movedepth_amd import ops
+
+    g = gen(12)
+    x = torch.tensor([0.0, 3.0, 1000.1, -12345.678, 3.3e5, 1.7e6], device="cuda")[:, None].expand(6, C).contiguous().requires_grad_()
+    w, b, go = randn(g, C), randn(g, C), randn(g, 6, C)
+    y = ops.layer_norm(x, w, b)
+    k = (C / 64 + 26) * ref.U32
+    tol = w.abs().double().cpu() * x.detach().abs().double().cpu() * k * k * 1e-5 ** -0.5 + 4 * ref.U32 * b.abs().double().cpu()
+    ref.within(y, b.double().cpu().expand(6, C), tol, "y")
+    dx, = torch.autograd.grad(y, x, go)
+    h = (go * w).double().cpu()
+    want = (h - h.mean(1, keepdim=True)) * 1e-5 ** -0.5
+    assert relative(dx, want) <= 1e-5
+
+
+@pytest.mark.parametrize("act_bits", [0, 8])
+@pytest.mark.parametrize("C", [24, 777, 3000, 5000])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+def test_layer_norm_keeps_what_is_not_finite_in_its_row(bad, C, act_bits):
+    g = gen(14)
+    x, w, b, go = randn(g, 9, C), randn(g, C), randn(g, C), randn(g, 9, C)
+    rows = [i for i in range(9) if i != 4]
+    want = ref.layer_norm(x[rows], w, b, 1e-5, go[rows], act_bits)
+    x[4, C // 2] = bad
+    got = base.run_layer_norm(x, w, b, 1e-5, go, act_bits)
+    assert bool(torch.isnan(got["y"][4]).all()) and bool(torch.isnan(got["dx"][4]).all()) and bool(torch.isnan(got["dw"]).all())
+    check({n: got[n][rows] for n in ("y", "dx")}, {n: want[n] for n in ("y", "dx")}, "the other rows")
+    assert bool(torch.isfinite(got["db"]).all())
+
+
 # --------------------------------------------------------------------------- the trainer
 def test_the_erased_region_does_not_come_back_through_the_other_frames(monkeypatch):
     """--match_attention: in the pass whose reference image has a rectangle erased nothing may depend on what stood there; both sides of its cost volume are compared
