@@ -1479,6 +1479,13 @@ def _wants_grad(*tensors):
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
+def _refuse_tangents(what, *tensors):
+    """the operators have no forward-mode derivative: a dual tensor would lose its tangent on the inference path"""
+    fw = torch.autograd.forward_ad
+    if fw._current_level >= 0 and any(t is not None and fw.unpack_dual(t).tangent is not None for t in tensors):
+        raise _lib.MovedepthHipError("%s: no forward-mode derivative (an argument is a dual tensor)" % what)
+
+
 _NO_GUARD = contextlib.nullcontext()
 
 
@@ -1534,8 +1541,9 @@ def act8_pack(x):
     """x (any shape; float32, bfloat16 or float16) -> Act8, 1 + 1/32 bytes per element: whole numbers of [-127, 127] times a power of two
     that 32 neighbours in memory share -- the least one that keeps the largest of them at 127 or below, so the error is at most half a
     step: 2^-7 of the group's largest magnitude (at the far end of the type's range, where that power would overflow, up to one part in
-    128 of the value).  32 neighbours that hold an infinity or a NaN come back as NaN.  No gradient."""
+    128 of the value).  32 neighbours that hold an infinity or a NaN come back as NaN.  No gradient, in either mode."""
     _token_check(x, "x", "act8_pack")
+    _refuse_tangents("act8_pack", x)
     with torch.no_grad(), _on(x.device):
         x = x.detach()
         if not _is_dense(x):
@@ -1694,6 +1702,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, act_bits=0):
         raise _lib.MovedepthHipError("layer_norm: act_bits = %r (0 or 8)" % (act_bits,))
     if not eps >= 0:
         raise _lib.MovedepthHipError("layer_norm: eps = %r" % (eps,))
+    _refuse_tangents("layer_norm", x, weight, bias)
     if not _wants_grad(x, weight, bias):
         return _layer_norm_fwd(x, weight, bias, float(eps), 0, False)[0]
     return _LayerNorm.apply(x, weight, bias, float(eps), int(act_bits))
@@ -1795,6 +1804,7 @@ def cross_attention(q, k, v, key_mask=None, scale=None):
         raise _lib.MovedepthHipError("cross_attention: key_mask %s %s on %s (bool (%d, %d) on %s: True where a key takes part)"
                                      % (key_mask.dtype, tuple(key_mask.shape), key_mask.device, B, k.shape[1], q.device))
     scale = float(d ** -0.5 if scale is None else scale)
+    _refuse_tangents("cross_attention", q, k, v)
     if not _wants_grad(q, k, v):
         return _cross_attention_fwd(q, k, v, key_mask, scale, False)[0]
     return _CrossAttention.apply(q, k, v, key_mask, scale)

@@ -102,3 +102,22 @@ def test_second_derivatives_through_tensors_left_alone():
             return torch.sigmoid(t * t) * t
 
     assert torch.autograd.gradgradcheck(f, (x,))
+
+
+def test_tangents_are_seen():
+    import torch.autograd.forward_ad as fw
+
+    from movedepth_amd import _lib, ops
+
+    x = torch.randn(3)
+    ops._refuse_tangents("op", x, None)
+    with fw.dual_level():
+        ops._refuse_tangents("op", x, None)
+        d = fw.make_dual(x, x)
+        for ts in ((d,), (None, x, d)):
+            with pytest.raises(_lib.MovedepthHipError, match="op.*forward"):
+                ops._refuse_tangents("op", *ts)
+        with torch.no_grad(), pytest.raises(_lib.MovedepthHipError):
+            ops._refuse_tangents("op", d)
+    with pytest.raises(_lib.MovedepthHipError):
+        torch.func.jvp(lambda t: (ops._refuse_tangents("op", t), t)[1], (x,), (x,))

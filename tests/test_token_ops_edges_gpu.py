@@ -304,6 +304,23 @@ def test_layer_norm_keeps_what_is_not_finite_in_its_row(bad, C, act_bits):
     assert bool(torch.isfinite(got["db"]).all())
 
 
+# --------------------------------------------------------------------------- forward mode
+def test_forward_mode_is_refused():
+    import torch.autograd.forward_ad as fw
+
+    from movedepth_amd import ops
+
+    x = torch.ones(4, 16, device="cuda")
+    t = torch.ones(1, 4, 1, 16, device="cuda")
+    for no_grad in (False, True):
+        with fw.dual_level(), torch.set_grad_enabled(not no_grad):
+            for call in (lambda: ops.layer_norm(fw.make_dual(x, x)), lambda: ops.layer_norm(x, fw.make_dual(x[0], x[0])), lambda: ops.cross_attention(fw.make_dual(t, t), t, t),
+                         lambda: ops.cross_attention(t, t, fw.make_dual(t, t))):
+                with pytest.raises(RuntimeError):
+                    call()
+            ops.layer_norm(x)
+
+
 # --------------------------------------------------------------------------- the trainer
 def test_the_erased_region_does_not_come_back_through_the_other_frames(monkeypatch):
     """--match_attention: in the pass whose reference image has a rectangle erased nothing may depend on what stood there; both sides of its cost volume are compared
