@@ -321,6 +321,15 @@ def test_forward_mode_is_refused():
             ops.layer_norm(x)
 
 
+# --------------------------------------------------------------------------- sizes of the framework's own mixed-precision path
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("kind", ["none", "random"])
+def test_cross_attention_small_heads_in_two_bytes(kind, dtype):
+    """two heads of 16 over thousands of tokens"""
+    base.attention_case(1, 500, 5120, 2, 2, 16, dtype, kind)
+    base.attention_case(1, 2500, 300, 2, 2, 16, dtype, kind)
+
+
 # --------------------------------------------------------------------------- the trainer
 def test_the_erased_region_does_not_come_back_through_the_other_frames(monkeypatch):
     """--match_attention: in the pass whose reference image has a rectangle erased nothing may depend on what stood there; both sides of its cost volume are compared
@@ -365,3 +374,64 @@ def test_the_erased_region_does_not_come_back_through_the_other_frames(monkeypat
     assert float((r0 - r1).abs().max()) > 0.1 * float(r0.abs().max())          # the first pass sees the difference
     for (r0, s0), (r1, s1) in zip(keep["plain"][n:], keep["changed"][n:]):
         assert float((r0 - r1).abs().max()) <= 1e-4 * float(r0.abs().max()) and float((s0 - s1).abs().max()) <= 1e-4 * float(s0.abs().max())
+
+
+def eight_bits(t):
+    """t through 8 bits in the order of its storage, in torch operations on whole groups (definition: 32 neighbours, the least power of two that leaves the largest at
+    127 or below)"""
+    flat = t.detach().as_strided((t.numel(),), (1,), t.storage_offset()).double()
+    part = torch.nn.functional.pad(flat, (0, -t.numel() % 32)).view(-1, 32)
+    mant, ex = torch.frexp(part.abs().amax(1, keepdim=True))
+    step = torch.ldexp(torch.ones_like(mant), (ex - 7 + (mant * 128 >= 127.5).int()).clamp(-126, 121))
+    out = torch.empty_strided(t.shape, t.stride(), device=t.device, dtype=t.dtype)
+    out.as_strided((t.numel(),), (1,)).copy_((torch.round(part / step).clamp(-127, 127) * step).view(-1)[:t.numel()])
+    return out
+
+
+def test_trainer_keeps_the_regularisers_activations_in_8_bits(monkeypatch):
+    """--act_bits 8: the gradients of all that the regulariser's backward pass reaches are those of a run that keeps its activations as 8-bit values made by torch
+    operations, and not the plain step's.  The activations of two runs differ by about 2e-6 of their largest (library sums in an order that changes), so one in
+    2e-6 * 127.5 = 2.5e-4 rounds to the next 8-bit step, 1 / 64 of its group's largest, at most sqrt(32) / 64 of the root mean square: sqrt(2.5e-4) * 0.09 = 1.4e-3
+    norm-wise; where that step is the one next to zero (2 of 127) a ReLU lets a gradient pass or not: sqrt(2.5e-4 * 2 / 127) = 2e-3.  Together below 5e-3; a
+    wrong stride would be off by the gradient's whole size"""
+    from movedepth_amd import ops
+
+    real_context, real_pack, packed, by_hand = ops.saved_act8, ops.act8_pack, [], []
+    limit = 4096
+
+    def pack(t):
+        packed.append(t.numel())
+        return real_pack(t)
+
+    def by_torch(weights=(), **kw):
+        own = {w.data_ptr() for w in weights}
+
+        def save(t):
+            if t.dtype != torch.float32 or t.numel() < limit or t.data_ptr() in own or not ops._is_dense(t):
+                return t.detach()
+            by_hand.append(t.numel())
+            return eight_bits(t)
+
+        return torch.autograd.graph.saved_tensors_hooks(save, lambda t: t)
+
+    _, _, t = base.step(["--match_attention", "2"])
+    torch.nn.init.normal_(t.models["match_attn"].out.weight, std=0.2)
+    state = {n: m.state_dict() for n, m in t.models.items()}
+    _, plain, _ = base.step(["--match_attention", "2"], models=state)
+    args = ["--match_attention", "2", "--act_bits", "8"]
+    monkeypatch.setattr(ops, "act8_pack", pack)
+    monkeypatch.setattr(ops, "saved_act8", lambda min_numel=None, **kw: real_context(min_numel=limit, **kw))
+    _, got, _ = base.step(args, models=state)
+    assert len(packed) >= 20 and max(packed) >= 2 * 16 * 16 * 16 * 32          # two passes through the regulariser
+    monkeypatch.setattr(ops, "saved_act8", by_torch)
+    _, want, _ = base.step(args, models=state)
+    assert packed == by_hand                                  # the same tensors in the same order
+    names = [n for n in want if n.split(".")[0] in ("reg3d", "mvs_encoder", "match_attn") and want[n] is not None and bool(want[n].any())]
+    assert len([n for n in names if n.startswith("reg3d")]) >= 10
+    for n in names:
+        assert relative(got[n], want[n]) <= 5e-3, n
+    # the last layer's weight gradient is a sum over rounded activations, nothing behind it is: off by the rounding, at most half a step = 1 / 127.5 of the largest
+    # of 32 neighbours, which is at most sqrt(32) times their root mean square
+    off = [relative(r["reg3d.prob.weight"], plain["reg3d.prob.weight"]) for r in (got, want)]
+    print("last layer's weight gradient off by %.3g, by %.3g with torch's 8 bits" % tuple(off))
+    assert 10 * relative(got["reg3d.prob.weight"], want["reg3d.prob.weight"]) < min(off) and max(off) <= 32 ** 0.5 / 127.5
