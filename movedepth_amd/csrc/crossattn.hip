@@ -1259,8 +1259,8 @@ __global__ __launch_bounds__(256) void xa_few_kernel(FewArgs a) {
 // either sign, where the sum of their exact values would not.  Rows of the tile kernels' operands up to 2^36 keep every product and sum of both passes finite (dS K:
 // 2^36 to the third, times 2, times 2^17 rows); a z with a row beyond, an infinite one among them, is computed again here, from the formula in
 // float32 arithmetic and from the tensors themselves.  Such rows are not met in earnest, so this is the simplest kernel: a wave takes a row, its lanes
-// 64 rows of the other side and then the row's dims.  Otherwise a workgroup reads the tiles' norms of its z and ends: 5 us forward and 6 backward, of 1430 for
-// 6 x 2 x 7680^2 heads of 16.
+// 64 rows of the other side and then the row's dims (6 x 2 x 7680^2 heads of 16, both passes: 0.2 s).  Otherwise a workgroup reads the tiles' norms of its z and
+// ends: 5 us forward and 6 backward, of 1480.
 struct BeyondArgs {
     Shape s;
     const float *q, *k, *v, *g;
@@ -1281,6 +1281,7 @@ __device__ __forceinline__ bool beyond(const BeyondArgs &a, int z) {       // ev
 }
 __device__ __forceinline__ float beyond_dot(const float *x, const float *y, int d, float f) {
     float s = 0.f;
+#pragma unroll 8
     for (int e = 0; e < d; ++e) s = fmaf(x[e] * f, y[e], s);
     return s;
 }
@@ -1312,7 +1313,9 @@ __global__ __launch_bounds__(256) void xa_beyond_fwd_kernel(BeyondArgs a) {
         const float inv = l == 0.f ? 0.f : 1.f / l;
         for (int i0 = 0; i0 < n; i0 += 64) {
             const float p = i0 + lane < n ? exp2f(score(i0 + lane) - m) * inv : 0.f;     // normalised first: sums of large values stay in range
-            for (int i = 0; i < 64 && i0 + i < n; ++i) {
+            const int some = min(64, n - i0);
+#pragma unroll 8
+            for (int i = 0; i < some; ++i) {
                 const float pi = __shfl(p, i), *v = at.v + at.key(a.s, i0 + i) * a.v_sn;
                 if (lane < d) o0 = fmaf(pi, v[lane], o0);
                 if (lane + 64 < d) o1 = fmaf(pi, v[lane + 64], o1);
@@ -1346,7 +1349,9 @@ __global__ __launch_bounds__(256) void xa_beyond_bwd_kernel(BeyondArgs a) {
             for (int i0 = 0; i0 < n; i0 += 64) {
                 float p = 0.f, ds = 0.f;
                 if (i0 + lane < n) pair(q, g, r, i0 + lane, p, ds);
-                for (int i = 0; i < 64 && i0 + i < n; ++i) {
+                const int some = min(64, n - i0);
+#pragma unroll 8
+                for (int i = 0; i < some; ++i) {
                     const float di = __shfl(ds, i), *k = at.k + at.key(a.s, i0 + i) * a.k_sn;
                     if (lane < d) x0 = fmaf(di, k[lane], x0);
                     if (lane + 64 < d) x1 = fmaf(di, k[lane + 64], x1);
@@ -1361,7 +1366,9 @@ __global__ __launch_bounds__(256) void xa_beyond_bwd_kernel(BeyondArgs a) {
                 float p = 0.f, ds = 0.f;
                 if (r0 + lane < a.s.M)
                     pair(at.query(at.q, a.q_sn, a.q_sh, r0 + lane), at.query(at.g, a.g_sn, a.g_sh, r0 + lane), r0 + lane, i, p, ds);
-                for (int r = 0; r < 64 && r0 + r < a.s.M; ++r) {
+                const int some = min(64, a.s.M - r0);
+#pragma unroll 4
+                for (int r = 0; r < some; ++r) {
                     const float di = __shfl(ds, r), pi = __shfl(p, r);
                     const float *q = at.query(at.q, a.q_sn, a.q_sh, r0 + r), *g = at.query(at.g, a.g_sn, a.g_sh, r0 + r);
                     if (lane < d) x0 = fmaf(di, q[lane], x0), y0 = fmaf(pi, g[lane], y0);
@@ -1607,7 +1614,7 @@ BeyondArgs beyond_args(const md_attn_desc &a, const Plan &p, const Shape &sh, ch
     b.q_sb = a.q_sb, b.q_sn = a.q_sn, b.q_sh = a.q_sh, b.k_sb = a.k_sb, b.k_sn = a.k_sn, b.k_sh = a.k_sh, b.v_sb = a.v_sb, b.v_sn = a.v_sn, b.v_sh = a.v_sh;
     b.qn = (const float *)(ws + p.qn), b.kn = (const float *)(ws + p.kn), b.vn = (const float *)(ws + p.vn);
     b.q_tiles = p.q_tiles, b.k_tiles = p.k_tiles;
-    b.blocks = (int)std::max<long long>(1, std::min<long long>((rows + 3) / 4, CUS / p.Z));
+    b.blocks = (int)std::max<long long>(1, std::min<long long>((rows + 3) / 4, 4 * CUS / p.Z));
     b.c = a.scale * LOG2E, b.scale = a.scale;
     return b;
 }
