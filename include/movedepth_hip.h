@@ -407,7 +407,8 @@ int md_layer_norm_bwd(const void *g, long long ldg, const void *x, long long ldx
 
 /* 8-bit activations: every 32 neighbours share a scale 2^e, e the least exponent for which the largest of them rounds to 127 or
  * less; value = n * 2^e, n in [-127, 127].  n is x * 2^-e correctly rounded (ties to even) and n * 2^e is exact in x's type, so
- * packing what came back gives the same codes.  e stays in [-126, 121] (float16: [-24, 9]; n is cut off at 127 at the upper end).
+ * packing what came back gives the same codes.  e stays in [-126, 121] (float16: [-24, 9]; n is cut off at 127 at the upper end); within it the error is at
+ * most half a step, 1 / 127.5 of the largest.
  * A group that holds a NaN or an infinity comes back as NaN.  codes [n] int8, scales [ceil(n / 32)] int8 (e; -128 = NaN). */
 int md_act8_pack(const void *x, int dtype, long long n, void *codes, void *scales, md_stream_t stream);
 int md_act8_unpack(const void *codes, const void *scales, int dtype, long long n, void *x, md_stream_t stream);
@@ -417,6 +418,7 @@ int md_act8_unpack(const void *codes, const void *scales, int dtype, long long n
  * row; a query left without a key gets o = 0 and gives no gradients; dk, dv of masked keys are 0.  A valid key whose score is -inf weighs 0, and a
  * query whose scores are all -inf is as one without a key; otherwise infinities and NaN go the way of the formula in IEEE arithmetic.
  * The last axis of q, k, v, g is contiguous, *_sb / *_sn / *_sh are the strides of sequence, token and head in elements (0 allowed);
+ * 2-byte types: the softmax weights, and backward the scores' gradients, are rounded to the type before their products; all sums are float32.
  * o, dq [B][Nq][Hq][d] and dk, dv [B][Nk][Hk][d] are contiguous.  lse [B][Hq][Nq]: log2 of the softmax denominator including its
  * maximum, +inf without a key; written by the forward pass (or NULL there), read by the backward pass.  dq may be NULL, dk and dv both may.
  * ws: md_cross_attn_ws_bytes(desc, backward) bytes, 256-byte aligned.

@@ -20,7 +20,10 @@
 //
 // float32 runs on the bf16 instructions too: every operand as the sum of three bf16 pieces (8 + 8 + 8 bits), six products of pieces whose
 // magnitudes matter to 2^-24, which is 6 / 16 of what the float32 matrix instruction costs.  2-byte types: P and dS are rounded to
-// the type before their products (half a step relative).  float16 holds P times 2^7 (forward) or 2^15 (backward) and dS times a power
+// the type before their products (half a step relative), as the matrix instruction takes them: o, dq, dk and dv then carry two roundings of that size instead of
+// one (bf16, norm-wise: 2.5e-3 against 1.7e-3).  Two pieces of P and dS would halve that and cost 35 to 50 % (both passes, bf16: 1.28 to 1.86 ms for 2 x 2 x 20480^2
+// heads of 32, 1.40 to 1.90 for 2 x 16 x 4096 x 8192 heads of 64).  l sums P as it is before that rounding, so that `lse`, from which the backward pass takes P again, is that of
+// the exact weights; D is formed in 32 bits from o as it was stored.  float16 holds P times 2^7 (forward) or 2^15 (backward) and dS times a power
 // of two from |g| |v| (ds_scale), so that the small weights of long rows do not fall below its range.
 #include <algorithm>
 #include <type_traits>
@@ -968,7 +971,8 @@ __global__ __launch_bounds__(64 * NW, (NW == 4 ? dq_per_cu<Frag<T>::NP, KS, QT>(
 
 // dk, dv: 32 KT keys per wave, steps of 32 queries.  A lane owns a key here: S = Q K^T, dV^T += g^T P, dK^T += Q^T dS; lse and D of a step's queries lie
 // across a lane's registers and come from LDS with the fragments.  2 x 2 x 20480^2 heads of 32, bf16: 563 us (57 % of the vector and 40 % of the matrix pipe's
-// cycles); 2 x 16 x 4096 x 8192 heads of 64: 659 us, 0.83 PFLOP/s, bound by the fragments it reads from LDS (24 KB per 32 x 32 pairs, about 60 % of 128 bytes a cycle)
+// cycles); 2 x 16 x 4096 x 8192 heads of 64: 659 us, 0.83 PFLOP/s, with no pipe full (matrix 43 %, vector 36 %, LDS 32 % of the cycles): three waves a SIMD, and within a wave
+// S and g V^T, the exponentials and the products behind them follow one another, for a second key tile to run beside them spills or leaves one wave (945 us)
 template <class T, int KS>
 struct DkvLds {
     static constexpr int NP = Frag<T>::NP, DB = (KS + 1) / 2, CHUNKS = 2 * KS * NP + 4 * DB * NP + 1;

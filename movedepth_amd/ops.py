@@ -1539,9 +1539,10 @@ def _is_dense(t):
 
 def act8_pack(x):
     """x (any shape; float32, bfloat16 or float16) -> Act8, 1 + 1/32 bytes per element: whole numbers of [-127, 127] times a power of two
-    that 32 neighbours in memory share -- the least one that keeps the largest of them at 127 or below, so the error is at most half a
-    step: 2^-7 of the group's largest magnitude (at the far end of the type's range, where that power would overflow, up to one part in
-    128 of the value).  32 neighbours that hold an infinity or a NaN come back as NaN.  No gradient, in either mode."""
+    that 32 neighbours in memory share -- the least one that keeps the largest of them at 127 or below.  The error is at most half a step, 1 / 127.5 of the
+    group's largest magnitude (which lies at 63.75 steps or more), but at the ends of the type's range: where the power would overflow the largest values
+    lose up to one part in 128, and it is no less than 2^-126 (float16: 2^-24), so that float32 and bfloat16 groups below about 2^-120
+    are rounded to multiples of that, to zero from 2^-127 down.  32 neighbours that hold an infinity or a NaN come back as NaN.  No gradient, in either mode."""
     _token_check(x, "x", "act8_pack")
     _refuse_tangents("act8_pack", x)
     with torch.no_grad(), _on(x.device):
@@ -1787,7 +1788,9 @@ def cross_attention(q, k, v, key_mask=None, scale=None):
     strides (the last axis is copied if it is not contiguous).  key_mask (B, Nk) bool, True where a key takes part: what stands in the
     other rows of k and v is not used, whatever it is, and their gradients are 0; a query without any key gets zeros and gives no gradients.
     A key whose score is -inf weighs 0, and a query whose scores are all -inf is as one without a key.
-    Softmax statistics and sums are float32; with 2-byte types the softmax weights are rounded to that type before the product with v."""
+    Softmax statistics and sums are float32; with 2-byte types the softmax weights are rounded to that type before their products with v and (backward) g, and the
+    gradient of the scores before its products with k and q, half a step each; the backward pass takes o as it was returned.  No second and no
+    forward-mode derivatives."""
     for t, nm in ((q, "q"), (k, "k"), (v, "v")):
         _token_check(t, nm, "cross_attention")
         if t.dim() != 4:
