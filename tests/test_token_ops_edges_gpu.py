@@ -197,6 +197,38 @@ def test_float32_values_beyond_the_pieces(size, Nq):
         check(base.run_attention(q, k, v / size, mask, 0.3, go * size), ref.cross_attention(q, k, v / size, mask, 0.3, go * size), "large g")
 
 
+@pytest.mark.parametrize("need", ["qkv", "q", "kv"])
+@pytest.mark.parametrize("d", [7, 40, 100])
+def test_float32_rows_beyond_the_pieces_in_every_layout(d, need):
+    """shared key heads, views of a joint projection, a mask with a sequence without keys, an expanded gradient, some of the gradients only; one sequence holds the large rows,
+    and the others have the bits that they have without it"""
+    from movedepth_amd import ops
+
+    g = gen(15)
+    q = randn(g, 3, 6, 50, d).transpose(1, 2)
+    kv = randn(g, 3, 130, 2, 2, d)
+    mask = (torch.rand(3, 130, generator=g) < 0.7).cuda()
+    mask[1] = False
+    go = randn(g, 1, 50, 6, 1).expand(3, 50, 6, d)
+
+    def run():
+        ts = {"q": q, "k": kv[:, :, 0], "v": kv[:, :, 1]}
+        ts = {n: t.detach().requires_grad_(n in need) for n, t in ts.items()}
+        o = ops.cross_attention(**ts, key_mask=mask, scale=0.2)
+        names = [n for n in ts if n in need]
+        return dict(zip(["o"] + ["d" + n for n in names], [o.detach(), *torch.autograd.grad(o, [ts[n] for n in names], go)]))
+
+    plain = run()
+    kv[2, 3, 0, :, 0], mask[2, 3], q[2, ..., 0] = float("-inf"), True, 1.5
+    seen = mask.clone()
+    seen[2, 3] = False
+    got, want = run(), ref.cross_attention(q, kv[:, :, 0], kv[:, :, 1], seen, 0.2, go)
+    for n in got:
+        assert torch.equal(got[n][:2], plain[n][:2]), n
+        skip = 1 if n == "dq" else 0                              # (its first element is a weight of 0 times -inf)
+        ref.within(got[n][..., skip:], want[n][0][..., skip:], want[n][1][..., skip:], n)
+
+
 @pytest.mark.parametrize("Nq", [1, 40])
 @pytest.mark.parametrize("dtype", DT)
 def test_an_infinite_value_reaches_its_own_column(dtype, Nq):
