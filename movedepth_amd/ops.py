@@ -1692,7 +1692,8 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, act_bits=0):
     """(x - mean) / sqrt(var + eps) * weight + bias over the last axis (biased variance, as torch's layer_norm).  x (..., C) float32, bfloat16 or
     float16, read in place where its rows are evenly spaced; statistics, sums and parameter gradients in float32; weight and bias (C,) or None.
     act_bits=8: the backward pass reads x from 8 bits (act8_pack's format, groups of 32 along the last axis) written by the forward
-    kernel instead of keeping x; the result does not change."""
+    kernel instead of keeping x; the result does not change.  The rounding is of x's size, not of its deviations': rows whose mean is far above these (30 times
+    and more), and rows of a few elements, keep little of them, and their gradients are off by as much.  No second and no forward-mode derivatives."""
     _token_check(x, "x", "layer_norm")
     if x.dim() < 1 or not 1 <= x.shape[-1] <= 1 << 20:
         raise _lib.MovedepthHipError("layer_norm: x %s (at least one axis, 1 .. 2^20 elements in the last)" % (tuple(x.shape),))
